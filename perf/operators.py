@@ -155,7 +155,7 @@ def _prepare_attn(c, seed):
         import cudatransformer_amd as ct
 
         # The batch's plan, which a program makes once for all of a model's layers and both directions.
-        s["plan"] = ct.packed_plan(s["lens"], device="cuda")
+        s["plan"] = ct.packed_plan(s["lens"], c["hq"], c["hkv"], device="cuda")
     return s
 
 
