@@ -4,6 +4,7 @@ Layers of this package
   * ``libctattn.so``   -- HIP kernels for gfx950 behind a C-ABI (``include/ctattn.h``).
   * ``cuda_transformer`` -- C++ host module (pybind11) mirroring the reference's
     ``Tensor`` / ``FlashAttentionLayer`` API on top of that C-ABI.
+  * ``packed``         -- attention on packed sequences of different lengths.
   * ``_capi``          -- ctypes binding of the same C-ABI over torch device tensors
     (torch is plumbing: memory and streams).
 
@@ -31,6 +32,15 @@ from ._capi import (  # noqa: E402
     set_policy,
     sgd_update,
 )
+from .packed import (  # noqa: E402
+    PackedAttentionFunction,
+    PackedPlan,
+    flash_attention_packed,
+    flash_attn_packed_bwd,
+    flash_attn_packed_fwd,
+    packed_bwd_workspace_bytes,
+    packed_plan,
+)
 
 __all__ = [
     "BF16",
@@ -39,10 +49,17 @@ __all__ = [
     "POLICY_DETERMINISTIC",
     "POLICY_GENERIC",
     "FlashAttentionFunction",
+    "PackedAttentionFunction",
+    "PackedPlan",
     "bwd_workspace_bytes",
     "flash_attention",
+    "flash_attention_packed",
     "flash_attn_bwd",
     "flash_attn_fwd",
+    "flash_attn_packed_bwd",
+    "flash_attn_packed_fwd",
+    "packed_bwd_workspace_bytes",
+    "packed_plan",
     "out_proj_bwd",
     "out_proj_fwd",
     "qkv_proj_bwd",

@@ -121,6 +121,11 @@ def load() -> ctypes.CDLL:
         "ctattn_tensor_reduce": ([c_int, c_int, vp, i64, i64, i64, vp, vp, i64, vp], c_int),
         "ctattn_tensor_permute": ([c_int, vp, c_int, vp, vp, vp, vp], c_int),
         "ctattn_tensor_kron": ([c_int, vp, vp, c_int, vp, vp, vp, vp], c_int),
+        "ctattn_packed_plan_bytes": ([vp, i64, i64], i64),
+        "ctattn_packed_plan": ([vp, i64, i64, vp, i64], c_int),
+        "ctattn_packed_fwd": ([c_int] + [vp] * 8 + [i64] * 4 + [c_int, vp], c_int),
+        "ctattn_packed_bwd_workspace_bytes": ([c_int, vp] + [i64] * 3, i64),
+        "ctattn_packed_bwd": ([c_int] + [vp] * 10 + [i64] + [vp] * 3 + [i64] * 4 + [c_int, vp], c_int),
         "ctattn_tensor_matmul": ([c_int, vp, vp, vp] + [i64] * 5 + [vp], c_int),
     }
     for name, (args, res) in sigs.items():

@@ -576,6 +576,63 @@ CTATTN_API int ctattn_tensor_kron(int dtype, const void *a, const void *b, int n
 CTATTN_API int ctattn_tensor_matmul(int dtype, const void *a, const void *b, void *c, int64_t batch,
                                     int64_t batch_b, int64_t M, int64_t K, int64_t N, void *stream);
 
+/* ---- attention on packed sequences -----------------------------------------------------
+ *
+ * Sequences of different lengths lie one behind the other in [rows, heads, d] tensors, in rows
+ * 0 .. tokens - 1; each attends to itself alone.  Hq query heads share Hkv key / value heads,
+ * query head h using key head h / (Hq / Hkv).  No counterpart in the reference, whose attention
+ * takes [B, H, T, d] with one length and equal head counts.
+ *
+ * The batch's plan says where sequences begin and which tiles to work on, in which order.
+ * ctattn_packed_plan writes it into host memory from the lengths (any of them may be 0); the
+ * caller copies it to the device (16-byte aligned) and gives both copies to every call, which
+ * reads sizes from the host's and offsets from the device's.  It serves any number of calls,
+ * layers and both directions, causal or not, for one Hq / Hkv, and must stay valid and unchanged
+ * until the stream has finished with them.
+ */
+
+/* Bytes of the plan of nseq sequences of seqlens[i] tokens with group = Hq / Hkv (1 .. 4096), or -1
+ * on invalid arguments: negative lengths, or tokens * group above 2^31 - 2^20. */
+CTATTN_API int64_t ctattn_packed_plan_bytes(const int64_t *seqlens, int64_t nseq, int64_t group);
+
+/* Writes the plan to `out`, HOST memory of at least ctattn_packed_plan_bytes bytes. */
+CTATTN_API int ctattn_packed_plan(const int64_t *seqlens, int64_t nseq, int64_t group, void *out, int64_t bytes);
+
+/*
+ * Forward: for each row i of a sequence and query head, O = softmax(q K^T / sqrt(d)) V over the keys
+ * of that sequence (causal != 0: up to and including i), and lse [tokens, Hq], contiguous (fp64 for
+ * CTATTN_F64, else fp32; may be NULL).  q and o are [rows, Hq, d], k and v [rows, Hkv, d], rows >=
+ * the plan's tokens; rows behind the last sequence are neither read nor written.  `strides` (HOST)
+ * holds, in elements, the row and the head stride of q, k, v and o; the d elements of a head are
+ * contiguous, and the outputs' elements must not overlap.
+ *   - bf16, fp16 (d a multiple of 8) and fp32 (a multiple of 4) run on MFMA kernels for d <= 128 and
+ *     Hq / Hkv <= 128 when pointers and strides are multiples of 16 bytes; other calls, f64, and every
+ *     call under CTATTN_POLICY_GENERIC take generic kernels (same results, much slower).
+ *   - a NaN or an infinity in a sequence's keys or values may reach any row of that sequence and head
+ *     group, and no other sequence.
+ */
+CTATTN_API int ctattn_packed_fwd(int dtype, const void *q, const void *k, const void *v, void *o, void *lse,
+                                 const int64_t *strides, const void *plan_host, const void *plan, int64_t rows,
+                                 int64_t hq, int64_t hkv, int64_t d, int causal, void *stream);
+
+/* Bytes of device workspace ctattn_packed_bwd needs, or -1 on invalid arguments: a few bytes per
+ * token and query head. */
+CTATTN_API int64_t ctattn_packed_bwd_workspace_bytes(int dtype, const void *plan_host, int64_t hq, int64_t hkv,
+                                                     int64_t d);
+
+/*
+ * Backward: dq, dk, dv from the forward's o and lse and the upstream dout [rows, Hq, d]; dk and dv sum
+ * over the query heads that share a key head.  They are overwritten in rows 0 .. tokens - 1 and left
+ * alone behind them.  `strides` holds the row and head strides of q, k, v, o, dout, dq, dk, dv.  No
+ * atomics: the same inputs give the same bits.  The workspace (16-byte aligned) is scratch, free
+ * again when the stream has passed the call.
+ */
+CTATTN_API int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, const void *o,
+                                 const void *dout, const void *lse, void *dq, void *dk, void *dv, void *workspace,
+                                 int64_t workspace_bytes, const int64_t *strides, const void *plan_host,
+                                 const void *plan, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int causal,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif
