@@ -5,6 +5,7 @@ Layers of this package
   * ``cuda_transformer`` -- C++ host module (pybind11) mirroring the reference's
     ``Tensor`` / ``FlashAttentionLayer`` API on top of that C-ABI.
   * ``packed``         -- attention on packed sequences of different lengths.
+  * ``embedding``      -- scaled token lookup with a reproducible gradient.
   * ``_capi``          -- ctypes binding of the same C-ABI over torch device tensors
     (torch is plumbing: memory and streams).
 
@@ -32,6 +33,13 @@ from ._capi import (  # noqa: E402
     set_policy,
     sgd_update,
 )
+from .embedding import (  # noqa: E402
+    EmbeddingLookupFunction,
+    embedding,
+    embedding_grad,
+    embedding_grad_workspace_bytes,
+    embedding_lookup,
+)
 from .packed import (  # noqa: E402
     PackedAttentionFunction,
     PackedPlan,
@@ -48,10 +56,15 @@ __all__ = [
     "POLICY_AUTO",
     "POLICY_DETERMINISTIC",
     "POLICY_GENERIC",
+    "EmbeddingLookupFunction",
     "FlashAttentionFunction",
     "PackedAttentionFunction",
     "PackedPlan",
     "bwd_workspace_bytes",
+    "embedding",
+    "embedding_grad",
+    "embedding_grad_workspace_bytes",
+    "embedding_lookup",
     "flash_attention",
     "flash_attention_packed",
     "flash_attn_bwd",

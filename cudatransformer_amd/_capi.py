@@ -10,6 +10,7 @@ imports torch first for that reason.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -126,6 +127,9 @@ def load() -> ctypes.CDLL:
         "ctattn_packed_fwd": ([c_int] + [vp] * 8 + [i64] * 4 + [c_int, vp], c_int),
         "ctattn_packed_bwd_workspace_bytes": ([c_int, vp] + [i64] * 3, i64),
         "ctattn_packed_bwd": ([c_int] + [vp] * 10 + [i64] + [vp] * 3 + [i64] * 4 + [c_int, vp], c_int),
+        "ctattn_embedding_lookup": ([c_int, c_int, vp, vp, vp, f64] + [i64] * 3 + [vp], c_int),
+        "ctattn_embedding_grad_workspace_bytes": ([c_int] + [i64] * 3, i64),
+        "ctattn_embedding_grad": ([c_int, c_int, vp, vp, vp, f64, c_int, vp] + [i64] * 4 + [vp], c_int),
         "ctattn_tensor_matmul": ([c_int, vp, vp, vp] + [i64] * 5 + [vp], c_int),
     }
     for name, (args, res) in sigs.items():
@@ -164,6 +168,23 @@ def _stream_handle(stream) -> int:
     if _current_raw_stream is None:
         return int(torch.cuda.current_stream().cuda_stream)
     return _current_raw_stream(torch.cuda.current_device())
+
+
+@contextlib.contextmanager
+def _other_device_or_stream(device, stream):
+    with torch.cuda.device(device):
+        if stream is None:
+            yield
+        else:
+            with torch.cuda.stream(stream):  # what is allocated for the call belongs to its stream
+                yield
+
+
+def on_device(device, stream=None):
+    """Context in which the tensors' device is current and, if given, `stream` its current stream."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return _other_device_or_stream(device, stream)
 
 
 def _check_qkv(name, *ts):

@@ -6,29 +6,11 @@ batch's plan from its lengths, once for all layers and both directions.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
 
-from ._capi import _DTYPE_CODE, _check, _ptr, _stat_dtype, _stream_handle, last_error, load
-
-
-@contextlib.contextmanager
-def _other_device_or_stream(device, stream):
-    with torch.cuda.device(device):
-        if stream is None:
-            yield
-        else:
-            with torch.cuda.stream(stream):  # what is allocated for the call belongs to its stream
-                yield
-
-
-def on_device(device, stream=None):
-    """Context in which the tensors' device is current and, if given, `stream` its current stream."""
-    if stream is None and device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return _other_device_or_stream(device, stream)
+from ._capi import _DTYPE_CODE, _check, _ptr, _stat_dtype, _stream_handle, last_error, load, on_device
 
 
 class PackedPlan:

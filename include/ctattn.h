@@ -633,6 +633,32 @@ CTATTN_API int ctattn_packed_bwd(int dtype, const void *q, const void *k, const 
                                  const void *plan, int64_t rows, int64_t hq, int64_t hkv, int64_t d, int causal,
                                  void *stream);
 
+/* ---- scaled embedding, gradient by sorted tokens ---------------------------------------- */
+
+/*
+ * out[i][:] = scale * table[ids[i]][:] for n ids (id_dtype CTATTN_I32 or CTATTN_I64), table [vocab][D], out
+ * [n][D], both contiguous of type dtype (f32, bf16, f16, f64); an id outside [0, vocab) gives a row of
+ * zeros.  Computed in fp32 (fp64 for f64) and rounded once.  No counterpart in the reference, whose
+ * lookup has no scale (ctattn_embedding_fwd).
+ */
+CTATTN_API int ctattn_embedding_lookup(int dtype, int id_dtype, const void *ids, const void *table, void *out,
+                                       double scale, int64_t n, int64_t D, int64_t vocab, void *stream);
+
+/* Bytes of device workspace ctattn_embedding_grad needs, or -1 on invalid arguments. */
+CTATTN_API int64_t ctattn_embedding_grad_workspace_bytes(int dtype, int64_t n, int64_t D, int64_t vocab);
+
+/*
+ * dtable[v][:] = scale * sum of dout[i][:] over all i with ids[i] = v, every row of dtable [vocab][D] written
+ * (rows without a token with zeros); accumulate != 0 adds to what dtable holds instead.  Ids outside
+ * [0, vocab) add nothing.  Tokens are sorted by id and summed in the order of their positions, in fp32
+ * (fp64 for f64), with one rounding per element: no atomics on values, the same inputs give the same
+ * bits, any D and alignment.  ctattn_embedding_bwd, the reference's counterpart, adds into dtable with
+ * atomics.  The workspace (16-byte aligned) is scratch, free again when the stream has passed the call.
+ */
+CTATTN_API int ctattn_embedding_grad(int dtype, int id_dtype, const void *ids, const void *dout, void *dtable,
+                                     double scale, int accumulate, void *workspace, int64_t workspace_bytes,
+                                     int64_t n, int64_t D, int64_t vocab, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
