@@ -6,6 +6,7 @@ Layers of this package
     ``Tensor`` / ``FlashAttentionLayer`` API on top of that C-ABI.
   * ``packed``         -- attention on packed sequences of different lengths.
   * ``embedding``      -- scaled token lookup with a reproducible gradient.
+  * ``muon``           -- Newton-Schulz orthogonalisation and the Muon step.
   * ``_capi``          -- ctypes binding of the same C-ABI over torch device tensors
     (torch is plumbing: memory and streams).
 
@@ -40,6 +41,7 @@ from .embedding import (  # noqa: E402
     embedding_grad_workspace_bytes,
     embedding_lookup,
 )
+from .muon import muon_update, newton_schulz, newton_schulz_workspace_bytes  # noqa: E402
 from .packed import (  # noqa: E402
     PackedAttentionFunction,
     PackedPlan,
@@ -71,6 +73,9 @@ __all__ = [
     "flash_attn_fwd",
     "flash_attn_packed_bwd",
     "flash_attn_packed_fwd",
+    "muon_update",
+    "newton_schulz",
+    "newton_schulz_workspace_bytes",
     "packed_bwd_workspace_bytes",
     "packed_plan",
     "out_proj_bwd",

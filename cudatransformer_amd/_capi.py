@@ -130,6 +130,11 @@ def load() -> ctypes.CDLL:
         "ctattn_embedding_lookup": ([c_int, c_int, vp, vp, vp, f64] + [i64] * 3 + [vp], c_int),
         "ctattn_embedding_grad_workspace_bytes": ([c_int] + [i64] * 3, i64),
         "ctattn_embedding_grad": ([c_int, c_int, vp, vp, vp, f64, c_int, vp] + [i64] * 4 + [vp], c_int),
+        "ctattn_newton_schulz_workspace_bytes": ([c_int] + [i64] * 3, i64),
+        "ctattn_newton_schulz": ([c_int] + [vp] * 3 + [i64] * 4 + [c_int] + [f64] * 4 + [vp], c_int),
+        "ctattn_muon_update_workspace_bytes": ([c_int] + [i64] * 3, i64),
+        "ctattn_muon_update_multi": ([c_int, c_int] + [vp] * 4 + [i64] * 3 + [f64] * 2 + [c_int] + [f64] * 2 + [c_int]
+                                     + [f64] * 4 + [vp], c_int),
         "ctattn_tensor_matmul": ([c_int, vp, vp, vp] + [i64] * 5 + [vp], c_int),
     }
     for name, (args, res) in sigs.items():

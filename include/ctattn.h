@@ -659,6 +659,38 @@ CTATTN_API int ctattn_embedding_grad(int dtype, int id_dtype, const void *ids, c
                                      double scale, int accumulate, void *workspace, int64_t workspace_bytes,
                                      int64_t n, int64_t D, int64_t vocab, void *stream);
 
+/* ---- orthogonalised updates (Muon) ------------------------------------------------------ */
+
+/*
+ * Newton-Schulz iteration on `mats` matrices [rows][cols], one behind the other in x and out (which may be
+ * x): X = G / (|G|_F + eps), then `steps` (1 .. 100) times X <- a X + (b X X^T + c (X X^T)^2) X, products on
+ * the shorter side.  With a = 3.4445, b = -4.7750, c = 2.0315 five steps bring every singular value that is
+ * not tiny near one.  dtype f32, bf16 or f16 (storage; f64 is refused); the iteration itself runs in
+ * fp32 precision whatever the storage (factors of 22 significant bits, fp32 sums) and is rounded once.
+ * Coefficients up to 64 in absolute value; an iteration whose values pass 255 ends in infinities or NaN, as
+ * do a NaN or an infinity in G for its matrix.  No atomics: the same inputs give the same bits.  The workspace
+ * (256-byte aligned) is scratch.  No counterpart in the reference.
+ */
+CTATTN_API int64_t ctattn_newton_schulz_workspace_bytes(int dtype, int64_t mats, int64_t rows, int64_t cols);
+CTATTN_API int ctattn_newton_schulz(int dtype, const void *x, void *out, void *workspace, int64_t workspace_bytes,
+                                    int64_t mats, int64_t rows, int64_t cols, int steps, double a, double b, double c,
+                                    double eps, void *stream);
+
+/*
+ * One Muon step on `count` matrices [rows][cols] given by HOST tables of device pointers, in place:
+ *   m <- momentum m + g;  u = nesterov ? g + momentum m : m
+ *   p <- (1 - lr weight_decay) p - lr scale NewtonSchulz(u)
+ * param and grad of type dtype, moment fp32 whatever the dtype; no tensor may overlap another.  The update of
+ * p happens in the last product's epilogue.  64 matrices a batch, through one workspace.  Stands beside
+ * ctattn_adam_update_multi; no counterpart in the reference.
+ */
+CTATTN_API int64_t ctattn_muon_update_workspace_bytes(int dtype, int64_t count, int64_t rows, int64_t cols);
+CTATTN_API int ctattn_muon_update_multi(int dtype, int count, void *const *param, const void *const *grad,
+                                        void *const *moment, void *workspace, int64_t workspace_bytes, int64_t rows,
+                                        int64_t cols, double lr, double momentum, int nesterov, double weight_decay,
+                                        double scale, int steps, double a, double b, double c, double eps,
+                                        void *stream);
+
 #ifdef __cplusplus
 }
 #endif
