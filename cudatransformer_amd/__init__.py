@@ -41,7 +41,7 @@ from .embedding import (  # noqa: E402
     embedding_grad_workspace_bytes,
     embedding_lookup,
 )
-from .muon import muon_update, newton_schulz, newton_schulz_workspace_bytes  # noqa: E402
+from .muon import Muon, muon_update, newton_schulz, newton_schulz_workspace_bytes  # noqa: E402
 from .packed import (  # noqa: E402
     PackedAttentionFunction,
     PackedPlan,
@@ -60,6 +60,7 @@ __all__ = [
     "POLICY_GENERIC",
     "EmbeddingLookupFunction",
     "FlashAttentionFunction",
+    "Muon",
     "PackedAttentionFunction",
     "PackedPlan",
     "bwd_workspace_bytes",

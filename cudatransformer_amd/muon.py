@@ -105,4 +105,37 @@ def muon_update(params, grads, moments, lr: float = 0.02, momentum: float = 0.95
             _check(rc, "ctattn_muon_update_multi")
 
 
-__all__ = ["muon_update", "newton_schulz", "newton_schulz_workspace_bytes"]
+class Muon(torch.optim.Optimizer):
+    """Muon over matrices (2-D parameters; embeddings and vectors belong to another optimizer): muon_update of
+    every parameter that has a gradient, matrices of one shape and dtype together."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5):
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError(f"Muon: parameters must be matrices, got {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            kinds = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if "moment" not in self.state[p]:
+                    self.state[p]["moment"] = torch.zeros_like(p, dtype=torch.float32)
+                kinds.setdefault((p.dtype, p.device), []).append(p)
+            for ps in kinds.values():
+                muon_update(ps, [p.grad.contiguous() for p in ps], [self.state[p]["moment"] for p in ps], lr=group["lr"],
+                            momentum=group["momentum"], nesterov=group["nesterov"], weight_decay=group["weight_decay"],
+                            steps=group["steps"])
+        return loss
+
+
+__all__ = ["Muon", "muon_update", "newton_schulz", "newton_schulz_workspace_bytes"]

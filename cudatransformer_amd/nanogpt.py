@@ -20,6 +20,11 @@ Deliberate departures from the reference: causal attention (config 5), textbook 
 (the reference increments its step twice, ``AdamOptimizer.cu:75,95``), mean cross-entropy
 over all tokens on logits (mathematically -log softmax), weights initialised N(0, 0.02^2)
 (the reference initialises every weight to zero, ``LinearLayer.cu:28``).
+
+Beyond the reference: key / value heads shared by query heads (``n_kv_heads``), a scaled token
+embedding (``embedding_scale``), and batches of whole documents packed behind each other
+(``forward(ids, plan)``), on the packed attention and the sorted embedding gradient; the blocks'
+matrices can be trained with ``muon.Muon`` (``muon_parameters``).
 """
 from __future__ import annotations
 
@@ -28,6 +33,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ._capi import flash_attention
+from .embedding import embedding
+from .packed import flash_attention_packed
 
 CONFIG5 = dict(vocab=65, max_seq_len=256, d_model=384, n_heads=6, head_dim=64, mlp_dim=1536,
                n_layers=6, batch=16, seq_len=256, lr=3e-4)
@@ -45,20 +52,40 @@ _ACTIVATIONS = {
 class Attention(nn.Module):
     """QKV projection -> attention core -> output projection (AttentionLayer.cu:75-102)."""
 
-    def __init__(self, d_model, n_heads, head_dim, causal, attention):
+    def __init__(self, d_model, n_heads, head_dim, causal, attention, n_kv_heads=None):
         super().__init__()
         self.n_heads, self.head_dim, self.causal, self.attention = n_heads, head_dim, causal, attention
+        self.n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if self.n_kv_heads < 1 or n_heads % self.n_kv_heads != 0:
+            raise ValueError(f"{n_heads} query heads on {n_kv_heads} key heads")
         inner = n_heads * head_dim
         self.q = nn.Linear(d_model, inner)
-        self.k = nn.Linear(d_model, inner)
-        self.v = nn.Linear(d_model, inner)
+        self.k = nn.Linear(d_model, self.n_kv_heads * head_dim)
+        self.v = nn.Linear(d_model, self.n_kv_heads * head_dim)
         self.o = nn.Linear(inner, d_model)
 
-    def forward(self, x):
+    def forward_packed(self, x, plan):
+        """x [tokens, d_model], documents behind each other; each attends to itself."""
+        n = x.shape[0]
+        q, k, v = (f(x).view(n, -1, self.head_dim) for f in (self.q, self.k, self.v))
+        if self.attention == "ctattn":
+            o = flash_attention_packed(q, k, v, plan, self.causal)
+        else:
+            group = self.n_heads // self.n_kv_heads
+            k, v = (y.repeat_interleave(group, dim=1) for y in (k, v))
+            parts = zip(*(y.transpose(0, 1).split(plan.seqlens, dim=1) for y in (q, k, v)))
+            o = torch.cat([F.scaled_dot_product_attention(*p, is_causal=self.causal) for p in parts], dim=1).transpose(0, 1)
+        return self.o(o.reshape(n, self.n_heads * self.head_dim))
+
+    def forward(self, x, plan=None):
+        if plan is not None:
+            return self.forward_packed(x, plan)
         b, t, _ = x.shape
         # [B, T, H*d] -> [B, H, T, d]: the layout attention_qkv_kernels.cu:112-120 writes.
-        split = lambda y: y.view(b, t, self.n_heads, self.head_dim).transpose(1, 2).contiguous()  # noqa: E731
+        split = lambda y: y.view(b, t, -1, self.head_dim).transpose(1, 2).contiguous()  # noqa: E731
         q, k, v = split(self.q(x)), split(self.k(x)), split(self.v(x))
+        if self.n_kv_heads != self.n_heads:
+            k, v = (y.repeat_interleave(self.n_heads // self.n_kv_heads, dim=1) for y in (k, v))
         if self.attention == "ctattn":
             o = flash_attention(q, k, v, self.causal)
         else:
@@ -69,35 +96,40 @@ class Attention(nn.Module):
 class Block(nn.Module):
     """LayerNorm -> Attention -> LayerNorm -> MLP, no residuals (TransformerBlockLayer.cu:60-66)."""
 
-    def __init__(self, d_model, n_heads, head_dim, mlp_dim, causal, attention, activation="gelu"):
+    def __init__(self, d_model, n_heads, head_dim, mlp_dim, causal, attention, activation="gelu", n_kv_heads=None):
         super().__init__()
         if activation not in _ACTIVATIONS:
             raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}")
         self.act = _ACTIVATIONS[activation]
         self.ln1 = nn.LayerNorm(d_model, eps=1e-5)
-        self.attn = Attention(d_model, n_heads, head_dim, causal, attention)
+        self.attn = Attention(d_model, n_heads, head_dim, causal, attention, n_kv_heads)
         self.ln2 = nn.LayerNorm(d_model, eps=1e-5)
         self.fc1 = nn.Linear(d_model, mlp_dim)
         self.fc2 = nn.Linear(mlp_dim, d_model)
 
-    def forward(self, x):
-        x = self.attn(self.ln1(x))
+    def forward(self, x, plan=None):
+        x = self.attn(self.ln1(x), plan)
         return self.fc2(self.act(self.fc1(self.ln2(x))))
 
 
 class NanoGPT(nn.Module):
     def __init__(self, vocab, max_seq_len, d_model, n_heads, head_dim, mlp_dim, n_layers,
-                 causal=True, attention="ctattn", activation="gelu", **_):
+                 causal=True, attention="ctattn", activation="gelu", n_kv_heads=None, embedding_scale=1.0, **_):
         super().__init__()
         if attention not in ("ctattn", "sdpa"):
             raise ValueError("attention must be 'ctattn' or 'sdpa'")
         self.config = dict(vocab=vocab, max_seq_len=max_seq_len, d_model=d_model, n_heads=n_heads,
                            head_dim=head_dim, mlp_dim=mlp_dim, n_layers=n_layers, causal=causal,
                            activation=activation)
+        if n_kv_heads is not None and n_kv_heads != n_heads:
+            self.config["n_kv_heads"] = n_kv_heads
+        if embedding_scale != 1.0:
+            self.config["embedding_scale"] = embedding_scale
+        self.attention, self.embedding_scale = attention, embedding_scale
         self.tok = nn.Embedding(vocab, d_model)
         self.pos = nn.Embedding(max_seq_len, d_model)
         self.blocks = nn.ModuleList(
-            Block(d_model, n_heads, head_dim, mlp_dim, causal, attention, activation) for _ in range(n_layers))
+            Block(d_model, n_heads, head_dim, mlp_dim, causal, attention, activation, n_kv_heads) for _ in range(n_layers))
         self.unembed = nn.Linear(d_model, vocab, bias=False)
 
     def init_weights(self, seed: int):
@@ -114,15 +146,30 @@ class NanoGPT(nn.Module):
                     p.copy_(torch.randn(p.shape, generator=g, dtype=torch.float64).to(p.dtype) * 0.02)
         return self
 
-    def forward(self, ids):
-        t = ids.shape[1]
-        x = self.tok(ids) + self.pos(torch.arange(t, device=ids.device))
+    def forward(self, ids, plan=None):
+        """Logits of ids [B, T], or with a plan (packed.packed_plan) of ids [tokens], whole documents behind
+        each other: positions restart with each and none attends to another."""
+        if plan is None:
+            positions = torch.arange(ids.shape[1], device=ids.device)
+        else:
+            if ids.dim() != 1 or ids.shape[0] != plan.tokens:
+                raise ValueError(f"ids must be [{plan.tokens}], got {tuple(ids.shape)}")
+            if max(plan.seqlens, default=0) > self.config["max_seq_len"]:
+                raise ValueError(f"a document of {max(plan.seqlens)} tokens, {self.config['max_seq_len']} at most")
+            positions = plan.positions(ids.device)
+        if plan is not None and self.attention == "ctattn":
+            x = embedding(ids, self.tok.weight, self.embedding_scale)
+        else:
+            x = self.tok(ids)
+            if self.embedding_scale != 1.0:
+                x = x * self.embedding_scale
+        x = x + self.pos(positions)
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x, plan)
         return self.unembed(x)
 
-    def loss(self, ids, targets):
-        logits = self.forward(ids)
+    def loss(self, ids, targets, plan=None):
+        logits = self.forward(ids, plan)
         return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
 
 
@@ -159,6 +206,8 @@ def to_native(model: "NanoGPT", checkpoint_gap: int = 0, temperature: float = 1.
     from . import cuda_transformer as ctm
 
     c = model.config
+    if "n_kv_heads" in c or "embedding_scale" in c:
+        raise ValueError("the native model has as many key heads as query heads and no embedding scale")
     tensor = getattr(ctm, f"{dtype}Tensor")
     nat = getattr(ctm, f"{dtype}NanoGPT")(c["vocab"], c["max_seq_len"], c["d_model"], c["n_heads"], c["head_dim"], c["mlp_dim"],
                            c["n_layers"], checkpoint_gap=checkpoint_gap, temperature=temperature,
@@ -177,11 +226,30 @@ def make_batch(batch, seq_len, vocab, seed: int):
     return ids[:, :-1].contiguous(), ids[:, 1:].contiguous()
 
 
-def train_step(model, opt, ids, targets):
-    opt.zero_grad(set_to_none=True)
-    loss = model.loss(ids, targets)
+def make_packed_batch(seqlens, vocab, seed: int):
+    """Uniform random documents of these lengths behind each other, and next-token targets; a document's last
+    token predicts one more."""
+    g = torch.Generator().manual_seed(seed)
+    docs = [torch.randint(0, vocab, (n + 1,), generator=g) for n in seqlens]
+    return torch.cat([d[:-1] for d in docs]), torch.cat([d[1:] for d in docs])
+
+
+def muon_parameters(model):
+    """(matrices of the blocks, everything else): what Muon updates, and what Adam does."""
+    inside = [p for blk in model.blocks for p in blk.parameters() if p.dim() == 2]
+    chosen = {id(p) for p in inside}
+    return inside, [p for p in model.parameters() if id(p) not in chosen]
+
+
+def train_step(model, opt, ids, targets, plan=None):
+    """One step of an optimizer, or of several (a list); with a plan on packed documents."""
+    opts = opt if isinstance(opt, (list, tuple)) else [opt]
+    for o in opts:
+        o.zero_grad(set_to_none=True)
+    loss = model.loss(ids, targets, plan)
     loss.backward()
-    opt.step()
+    for o in opts:
+        o.step()
     return loss.detach()
 
 
@@ -200,5 +268,5 @@ def model_flops_per_step(cfg=CONFIG5) -> float:
     return dense + attention_flops_per_step(cfg)
 
 
-__all__ = ["CONFIG5", "NanoGPT", "make_batch", "train_step", "attention_flops_per_step",
+__all__ = ["CONFIG5", "NanoGPT", "make_batch", "make_packed_batch", "muon_parameters", "train_step", "attention_flops_per_step",
            "model_flops_per_step"]

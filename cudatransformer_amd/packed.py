@@ -35,6 +35,7 @@ class PackedPlan:
         need = lib.ctattn_packed_plan_bytes(lens, n, self.group)
         if need < 0:
             raise ValueError(last_error())
+        self._positions = {}
         self.device = torch.device(device)
         if self.device.type != "cuda":
             # A plan for the host alone: its lengths and offsets, no device copy to run kernels with.
@@ -57,6 +58,14 @@ class PackedPlan:
         for n in self.seqlens:
             out.append(out[-1] + n)
         return out
+
+    def positions(self, device=None):
+        """int64 [tokens]: each token's position in its sequence (made on first use for a device, then kept)."""
+        device = self.device if device is None else torch.device(device)
+        if device not in self._positions:
+            p = torch.cat([torch.arange(n) for n in self.seqlens]) if self.seqlens else torch.empty(0, dtype=torch.int64)
+            self._positions[device] = p.to(device)
+        return self._positions[device]
 
     def _pointers(self, handle: int):
         if handle != self._stream:
