@@ -14,8 +14,9 @@
 // of an entry's usual 1 / sqrt(c).  One fp16 term alone would not do: five steps amplify a
 // direction by up to a^5 = 485, and its rounding with it.
 //
-// Layout: factors lie in rows of groups [32 hi | 32 lo] (128 bytes), so that one K step of a tile row is
-// one 128-byte line; rows and columns are padded with zeros to 128 and no product checks a bound.
+// Layout: a factor's 128 x 32 blocks lie one behind the other, each a run of 128 rows [32 hi | 32 lo] (128 bytes
+// a row, 16 KiB), so that one K step of a tile is one contiguous read.  A product's 32 x 32
+// block is then a run of 4 KiB as well.  Rows and columns are padded with zeros to 128 and no product checks a bound.
 // X is kept in both orders (X for A, X^T for B X): each product's operands then have the contraction
 // contiguous, and the writing product has the tile in registers in either order anyway.
 #include "attn_bf16_tiles.h"
@@ -36,7 +37,7 @@ constexpr int kPad = 128;         // rows and columns are padded to it
 constexpr int kGroup = 32;        // elements of a [hi | lo] group
 constexpr int kRowBytes = 128;    // bytes of a group: one K step of a row
 constexpr int kMaxMats = 64;      // matrices of a launch
-constexpr int kNormBlocks = 64;   // partial sums of squares per matrix
+constexpr int kNormBlocks = 1024;  // partial sums of squares per matrix at most
 
 // Matrices of one shape: in one buffer, `stride` elements apart, or by pointers.
 struct Mats {
@@ -55,18 +56,54 @@ struct Update {
     float momentum, keep, lr;  // p <- keep p - lr X
 };
 
-// hi and lo of 256 x.
-__device__ __forceinline__ uint32_t split(float x) {
-    const _Float16 hi = _Float16(x);
-    const _Float16 lo = _Float16(x - float(hi));
-    return uint32_t(__builtin_bit_cast(uint16_t, hi)) | uint32_t(__builtin_bit_cast(uint16_t, lo)) << 16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+// hi and lo of 4 values that hold 256 x.
+struct Four {
+    u16x4 hi, lo;
+};
+__device__ __forceinline__ Four split4(f32x4 x) {
+    const f16x4 hi = __builtin_convertvector(x, f16x4);
+    const f32x4 back = __builtin_convertvector(hi, f32x4);
+    const f16x4 lo = __builtin_convertvector(x - back, f16x4);
+    return {__builtin_bit_cast(u16x4, hi), __builtin_bit_cast(u16x4, lo)};
 }
-__device__ __forceinline__ float joined(uint16_t hi, uint16_t lo) {
-    return float(__builtin_bit_cast(_Float16, hi)) + float(__builtin_bit_cast(_Float16, lo));
+__device__ __forceinline__ f32x4 join4(u16x4 hi, u16x4 lo) {
+    return __builtin_convertvector(__builtin_bit_cast(f16x4, hi), f32x4) +
+           __builtin_convertvector(__builtin_bit_cast(f16x4, lo), f32x4);
 }
-// Byte offset of element (i, k)'s hi in a factor with `pitch` bytes a row; lo is 64 bytes on.
-__device__ __forceinline__ int64_t factor_at(int64_t i, int64_t k, int64_t pitch) {
-    return i * pitch + (k / kGroup) * kRowBytes + (k % kGroup) * 2;
+
+// A 32 x 32 block of a factor in LDS: 32 rows [32 hi | 32 lo], chunks of 16 bytes swizzled as in Tile<64>
+// (4 KiB, on 1 KiB).  put4: elements c .. c + 3 (c a multiple of 4) of a row.
+__device__ __forceinline__ void block_put4(uint32_t blk, int row, int c, const Four &v) {
+    const uint32_t in = uint32_t(2 * (c & 4));
+    *(__attribute__((address_space(3))) u16x4 *)(uintptr_t)(blk + uint32_t(Tile<64>::off(row, c >> 3)) + in) = v.hi;
+    *(__attribute__((address_space(3))) u16x4 *)(uintptr_t)(blk + uint32_t(Tile<64>::off(row, 4 + (c >> 3))) + in) = v.lo;
+}
+// Writes the block's transpose to `to` (the 4 KiB run of a factor's block): ds_read_b64_tr_b16 gives lane l of a
+// group of 16 column l of 4 rows, so two of them are 8 elements of one row of the transpose.
+__device__ __forceinline__ void block_transposed(uint32_t blk, char *to, int lane) {
+    const int s = lane & 15, half = lane >> 5;
+    const int chunk = 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
+#pragma unroll
+    for (int part = 0; part < 2; ++part)  // hi, lo
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 16) {
+            i16x4 x[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int row = r0 + 8 * half + 4 * u + (s >> 2);
+                const uint32_t at = blk + uint32_t(Tile<64>::off(row, chunk + 4 * part) + 8 * (s & 1));
+                x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)at);
+            }
+            const i16x8 y = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
+            *reinterpret_cast<i16x8 *>(to + (lane & 31) * kRowBytes + 64 * part + 2 * (r0 + 8 * half)) = y;
+        }
+}
+// Byte offset of element (i, k)'s hi in a factor of `groups` K steps a row; lo is 64 bytes on.
+__device__ __forceinline__ int64_t factor_at(uint32_t i, uint32_t k, int groups) {
+    return int64_t((i / kPad) * uint32_t(groups) + k / kGroup) * (kPad * kRowBytes) + (i % kPad) * kRowBytes + (k % kGroup) * 2;
 }
 
 // ---- the update and its norm ----
@@ -77,18 +114,30 @@ __device__ __forceinline__ float update_value(const Update &u, const T *g, const
     return u.nesterov ? fmaf(u.momentum, m[i], to_f32(g[i])) : m[i];
 }
 
-// Sums of squares in fp64 (fp32 squares would overflow from 1.8e19 on), kNormBlocks a matrix; the Muon step
-// advances its moment here.
-template <typename T>
+// Sums of squares in fp64 (fp32 squares would overflow from 1.8e19 on), up to kNormBlocks a matrix; the Muon
+// step advances its moment here.  Runs of 16 bytes of G where its matrices lie on them.
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void norm_kernel(Mats g, Mats m, Update u, int64_t n, double *__restrict__ part) {
+    struct alignas(sizeof(T) * VEC) Run {
+        T v[VEC];
+    };
     const int mat = blockIdx.y;
     const T *gp = g.at<const T>(mat);
     float *mp = u.muon ? m.at<float>(mat) : nullptr;
     double s = 0;
-    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += int64_t(gridDim.x) * blockDim.x) {
-        if (u.muon) mp[i] = fmaf(u.momentum, mp[i], to_f32(gp[i]));
-        const double x = update_value(u, gp, mp, i);
-        s += x * x;
+    for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n / VEC; i += int64_t(gridDim.x) * blockDim.x) {
+        const Run r = reinterpret_cast<const Run *>(gp)[i];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int64_t at = i * VEC + e;
+            float x = to_f32(r.v[e]);
+            if (u.muon) {
+                const float mv = fmaf(u.momentum, mp[at], x);
+                mp[at] = mv;
+                x = u.nesterov ? fmaf(u.momentum, mv, x) : mv;
+            }
+            s += double(x) * double(x);
+        }
     }
     s = wave_sum(s);
     __shared__ double w[4];
@@ -104,50 +153,61 @@ struct Shape {
     int tall;            // X = G^T
 };
 
-// X and X^T as factors: one workgroup per 64 x 64 tile of X.
-template <typename T>
+// X and X^T as factors: a wave per 32 x 32 block of G, whose rows it reads 4 elements a lane, 8 lanes a row.  The block
+// goes to the factor with G's order of rows as it is read, and through LDS to the other.
+template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Shape s, double eps,
                                                    const double *__restrict__ part, int blocks, char *__restrict__ x,
                                                    char *__restrict__ xt, int64_t bytes) {
-    __shared__ uint32_t tile[64][65];
+    __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
     __shared__ float inv_s;
-    const int mat = blockIdx.z;
-    if (threadIdx.x < kWave) {
-        const double ss = wave_sum(int(threadIdx.x) < blocks ? part[int64_t(mat) * kNormBlocks + threadIdx.x] : 0.0);
-        if (threadIdx.x == 0) inv_s = float(double(kScale) / (sqrt(ss) + eps));
+    __shared__ double sums[4];
+    const int mat = blockIdx.z, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    {
+        double ss = 0;
+        for (int i = threadIdx.x; i < blocks; i += 256) ss += part[int64_t(mat) * kNormBlocks + i];
+        ss = wave_sum(ss);
+        if (lane == 0) sums[wave] = ss;
+        __syncthreads();
+        if (threadIdx.x == 0) inv_s = float(double(kScale) / (sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + eps));
     }
     __syncthreads();
     const float inv = inv_s;
     const T *gp = g.at<const T>(mat);
     const float *mp = u.muon ? m.at<const float>(mat) : nullptr;
-    const int64_t i0 = int64_t(blockIdx.y) * 64, k0 = int64_t(blockIdx.x) * 64;  // row and column of X
-    const int a = threadIdx.x % 64, b0 = threadIdx.x / 64;
-    for (int b = b0; b < 64; b += 4) {
-        const int i = s.tall ? a : b, k = s.tall ? b : a;  // along G's rows
-        float v = 0.f;
-        if (i0 + i < s.r && k0 + k < s.c)
-            v = update_value(u, gp, mp, s.tall ? (k0 + k) * s.cols + i0 + i : (i0 + i) * s.cols + k0 + k) * inv;
-        tile[i][k] = split(v);
-    }
-    __syncthreads();
-    // Row `line` of the tile (of its transpose), 16 elements a thread: 32 bytes of hi, 32 of lo.
-    const int line = threadIdx.x / 4, part16 = threadIdx.x % 4 * 16;
-    for (int t = 0; t < 2; ++t) {
-        u16x8 hi[2], lo[2];
+    // G's padded shape; its row blocks in y, four column blocks a workgroup in x.
+    const int gcols = int(s.tall ? s.rp : s.cp);
+    const int j0 = (int(blockIdx.x) * 4 + wave) * 32, i0 = int(blockIdx.y) * 32;
+    if (j0 >= gcols) return;
+    char *same = (s.tall ? xt : x) + mat * bytes + factor_at(i0, j0, gcols / kGroup);
+    char *other = (s.tall ? x : xt) + mat * bytes + factor_at(j0, i0, int(s.tall ? s.cp : s.rp) / kGroup);
+    const uint32_t blk = lds_addr(smem) + uint32_t(wave * 4096);
+    struct alignas(sizeof(T) * 4) Run {
+        T v[4];
+    };
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const uint32_t w = t == 0 ? tile[line][part16 + e] : tile[part16 + e][line];
-            hi[e / 8][e % 8] = uint16_t(w);
-            lo[e / 8][e % 8] = uint16_t(w >> 16);
-        }
-        char *to = (t == 0 ? x : xt) + mat * bytes +
-                   (t == 0 ? factor_at(i0 + line, k0 + part16, 4 * s.cp) : factor_at(k0 + line, i0 + part16, 4 * s.rp));
+    for (int q = 0; q < 4; ++q) {
+        const int line = 8 * q + lane / 8, c = 4 * (lane % 8);
+        const int64_t i = i0 + line, j = j0 + c, at = i * s.cols + j;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (VEC && i < s.rows && j + 3 < s.cols) {
+            const Run r = *reinterpret_cast<const Run *>(gp + at);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            *reinterpret_cast<u16x8 *>(to + 16 * h) = hi[h];
-            *reinterpret_cast<u16x8 *>(to + 64 + 16 * h) = lo[h];
+            for (int e = 0; e < 4; ++e) v[e] = u.muon ? update_value(u, gp, mp, at + e) : to_f32(r.v[e]);
+        } else if (i < s.rows) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < s.cols) v[e] = update_value(u, gp, mp, at + e);
         }
+        v = v * inv;
+        const Four f = split4(v);
+        *reinterpret_cast<u16x4 *>(same + line * kRowBytes + 2 * c) = f.hi;
+        *reinterpret_cast<u16x4 *>(same + line * kRowBytes + 2 * c + 64) = f.lo;
+        block_put4(blk, line, c, f);
     }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_transposed(blk, other, lane);
 }
 
 // ---- products ----
@@ -159,9 +219,10 @@ struct Gemm {
     int64_t kp;
     int tiles_m, tiles_n;        // kGram, kPoly: tiles_m (tiles_m + 1) / 2 lower tiles
     int mats, splits;
-    float *part;                 // splits > 1: sums of a split's tiles, 128 x 128 each
+    float *part;                 // splits > 1: a tile's sums for each split
     char *o, *ot;                // the product as a factor, and its transpose (kApply)
-    int64_t o_bytes, o_pitch, ot_pitch;
+    int64_t o_bytes;
+    int o_groups, ot_groups;     // their K steps a row
     const char *gram;            // kPoly: A, for b A
     float pa, pb, pc;
     Mats out;                    // kLast
@@ -169,7 +230,23 @@ struct Gemm {
     Shape s;
 };
 
-constexpr int kTile = 128;
+// Tile shapes of a product: BM x BN elements by WM x WN waves, K steps of 32 (rows of 128 bytes) through
+// STAGES LDS buffers.  One workgroup fills a CU either way (128 KiB of LDS).
+struct SmallTile {  // 8 waves of 64 x 32, two a SIMD: three steps of loads in flight
+    static constexpr int BM = 128, WM = 2, WN = 4, STAGES = 4;
+};
+struct LargeTile {  // 8 waves of 128 x 64, two a SIMD: half the operand bytes per product
+    static constexpr int BM = 256, WM = 2, WN = 4, STAGES = 2;
+};
+template <typename C> struct Tiling : C {
+    static constexpr int WAVES = C::WM * C::WN;
+    static constexpr int MT = C::BM / C::WM / 32, NT = C::BM / C::WN / 32;  // 32 x 32 blocks of a wave
+    static constexpr int TB = C::BM * kRowBytes;                            // one operand's tile of a step
+    static constexpr int LDS = 2 * C::STAGES * TB;
+    static constexpr int NL = TB / (WAVES * kWave * 16);                    // loads of a lane per operand and step
+    static constexpr int BLOCKS = (C::BM / 32) * (C::BM / 32);
+    static constexpr int WPE = WAVES / 4;
+};
 
 __device__ __forceinline__ void lower_tile(int t, int &ti, int &tj) {
     ti = int((sqrtf(8.f * float(t) + 1.f) - 1.f) * 0.5f);
@@ -178,83 +255,64 @@ __device__ __forceinline__ void lower_tile(int t, int &ti, int &tj) {
     tj = t - ti * (ti + 1) / 2;
 }
 
-// What a 32 x 32 block of sums becomes, by one wave.  sum(r): register r of lane (col, half) is row
-// acc_row(r, half), column col.  buf: 32 x 33 words of the wave's own.  (i0, j0): the block's place in the product.
+// What a 32 x 32 block of sums becomes, by one wave: register r of lane (col, half) is row acc_row(r, half),
+// column col.  buf: LDS address of 4.25 KiB of the wave's own, on 1 KiB.  (i0, j0): the block's place in the
+// product, multiples of 32, so that the block of a factor is a run of 4 KiB, 128 bytes a row.
+constexpr int kBufBytes = 5120;
 template <typename T, int P>
-__device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &acc, int64_t i0, int64_t j0, bool mirror,
-                                      uint32_t *buf, int lane) {
+__device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &acc, int i0, int j0, bool mirror,
+                                      uint32_t buf, int lane) {
     const int col = lane & 31, half = lane >> 5;
     if constexpr (P == kLast) {
-        float *f = reinterpret_cast<float *>(buf);
+        typedef __attribute__((address_space(3))) float lds_float;
+        lds_float *f = (lds_float *)(uintptr_t)buf;
 #pragma unroll
         for (int r = 0; r < 16; ++r) f[acc_row(r, half) * 33 + col] = acc[r] * (1.f / (kScale * kScale));
-        __builtin_amdgcn_wave_barrier();
-        T *out = g.out.at<T>(mat);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        // Along the output's rows: X's row i0 + line, or for a tall matrix X's column j0 + line.
+        const int64_t row0 = g.s.tall ? j0 : i0;
+        const int64_t at = (g.s.tall ? i0 : j0) + col;
+        T *to = g.out.at<T>(mat) + (row0 + half) * g.s.cols + at;
+        const int step = g.s.tall ? 1 : 33, across = g.s.tall ? 33 : 1;
+        if (at < g.s.cols) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const int line = 2 * q + half;
-            // Along the output's rows: X's row i, or for a tall matrix X's column j.
-            const int64_t i = g.s.tall ? i0 + col : i0 + line, j = g.s.tall ? j0 + line : j0 + col;
-            const float v = g.s.tall ? f[col * 33 + line] : f[line * 33 + col];
-            if (i < g.s.r && j < g.s.c) {
-                T *to = out + (g.s.tall ? j * g.s.cols + i : i * g.s.cols + j);
-                *to = from_f32<T>(g.u.muon ? fmaf(-g.u.lr, v, g.u.keep * to_f32(*to)) : v);
+            for (int q = 0; q < 16; ++q, to += 2 * g.s.cols) {
+                const int line = 2 * q + half;
+                const float v = f[line * step + col * across];
+                if (row0 + line < g.s.rows) *to = from_f32<T>(g.u.muon ? fmaf(-g.u.lr, v, g.u.keep * to_f32(*to)) : v);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
-        char *o = g.o + mat * g.o_bytes;
-        uint32_t w[16];
-        if constexpr (P == kPoly) {
-            const char *A = g.gram + mat * g.o_bytes;
+        // Four elements of row j0 + col of the transpose at a time, straight from the registers; the block as it is
+        // through LDS, where the transpose is transposed.
+        const int64_t at = factor_at(j0, i0, P == kApply ? g.ot_groups : g.o_groups) + mat * g.o_bytes + col * kRowBytes + 8 * half;
+        char *t = (P == kApply ? g.ot : g.o) + at;
+        // a I on the diagonal of the rows that exist.
+        const int diag = P == kPoly && i0 == j0 && i0 + col < g.s.r ? col - 4 * half : -1;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t i = i0 + acc_row(r, half), j = j0 + col;
-                const uint16_t *p = reinterpret_cast<const uint16_t *>(A + factor_at(i, j, g.o_pitch));
-                float v = fmaf(g.pb, joined(p[0], p[32]), g.pc * (acc[r] * (1.f / kScale)));
-                if (i == j && i < g.s.r) v += g.pa * kScale;
-                w[r] = split(v);
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w[r] = split(acc[r] * (1.f / kScale));
-        }
-        // Transposed, straight from the registers: 4 elements of row j0 + col.
-        char *t = P == kApply ? g.ot + mat * g.o_bytes : o;
-        const int64_t t_pitch = P == kApply ? g.ot_pitch : g.o_pitch;
-        if (P == kApply || mirror) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                u16x4 hi, lo;
+        for (int q = 0; q < 4; ++q) {
+            f32x4 v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+            v = v * (1.f / kScale);
+            if constexpr (P == kPoly) {  // A is symmetric: its row j0 + col
+                const f32x4 A = join4(*reinterpret_cast<const u16x4 *>(g.gram + at + 16 * q),
+                                      *reinterpret_cast<const u16x4 *>(g.gram + at + 16 * q + 64));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    hi[e] = uint16_t(w[4 * q + e]);
-                    lo[e] = uint16_t(w[4 * q + e] >> 16);
+                    v[e] = fmaf(g.pb, A[e], g.pc * v[e]);
+                    if (8 * q + e == diag) v[e] += g.pa * kScale;
                 }
-                char *to = t + factor_at(j0 + col, i0 + 8 * q + 4 * half, t_pitch);
-                *reinterpret_cast<u16x4 *>(to) = hi;
-                *reinterpret_cast<u16x4 *>(to + 64) = lo;
             }
+            const Four f = split4(v);
+            if (P == kApply || mirror) {
+                *reinterpret_cast<u16x4 *>(t + 16 * q) = f.hi;
+                *reinterpret_cast<u16x4 *>(t + 16 * q + 64) = f.lo;
+            }
+            block_put4(buf, col, 8 * q + 4 * half, f);
         }
-        // As it is, through LDS: 16 elements of a row a lane.
-#pragma unroll
-        for (int r = 0; r < 16; ++r) buf[acc_row(r, half) * 33 + col] = w[r];
-        __builtin_amdgcn_wave_barrier();
-        const int line = lane / 2, at = lane % 2 * 16;
-        u16x8 hi[2], lo[2];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const uint32_t x = buf[line * 33 + at + e];
-            hi[e / 8][e % 8] = uint16_t(x);
-            lo[e / 8][e % 8] = uint16_t(x >> 16);
-        }
-        char *to = o + factor_at(i0 + line, j0 + at, g.o_pitch);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            *reinterpret_cast<u16x8 *>(to + 16 * h) = hi[h];
-            *reinterpret_cast<u16x8 *>(to + 64 + 16 * h) = lo[h];
-        }
-        __builtin_amdgcn_wave_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        block_transposed(buf, g.o + mat * g.o_bytes + factor_at(i0, j0, g.o_groups), lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next block's writes follow these reads
     }
 }
 
@@ -265,133 +323,185 @@ __device__ __forceinline__ int64_t xcd_item(int64_t n) {
     return (blockIdx.x % 8) * q + blockIdx.x / 8;
 }
 
-// A workgroup of 4 waves: a 128 x 128 tile of a b^T, wave (w / 2, w % 2) its 64 x 64 quarter, K in steps of
-// 32 (rows of 128 bytes) through two LDS buffers.
-template <typename T, int P>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void product_kernel(Gemm g) {
-    constexpr int TB = kTile * kRowBytes;  // one operand's tile
-    __shared__ __attribute__((aligned(1024))) char smem[4 * TB];
+// A workgroup: one tile of a b^T over its split of K.  A step's operands are read into registers in two
+// halves of 16 of the contraction, the second while the first is multiplied, and the next step's
+// first half, after the barrier that publishes it, while the second is.
+template <typename T, int P, typename TC>
+__global__ __launch_bounds__(Tiling<TC>::WAVES *kWave) __attribute__((amdgpu_waves_per_eu(Tiling<TC>::WPE, Tiling<TC>::WPE)))
+void product_kernel(Gemm g) {
+    using C = Tiling<TC>;
+    constexpr int MT = C::MT, NT = C::NT, TB = C::TB, NL = C::NL;
+    __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
     const uint32_t L = lds_addr(smem);
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wm = wave / 2, wn = wave % 2, col = lane & 31, half = lane >> 5;
+    const int wm = wave / C::WN, wn = wave % C::WN, col = lane & 31, half = lane >> 5;
     constexpr bool SYM = P == kGram || P == kPoly;
     const int tiles = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
     const int64_t item = xcd_item(int64_t(g.mats) * tiles * g.splits);
     if (item >= int64_t(g.mats) * tiles * g.splits) return;
-    const int split_i = int(item % g.splits);
-    const int t = int(item / g.splits % tiles), mat = int(item / g.splits / tiles);
+    const int t = int(item % tiles), split_i = int(item / tiles % g.splits), mat = int(item / tiles / g.splits);
     int ti, tj;
     if (SYM) lower_tile(t, ti, tj);
     else ti = t % g.tiles_m, tj = t / g.tiles_m;
 
-    const int64_t pitch = 4 * g.kp;
+    constexpr int BLOCK = kPad * kRowBytes;
     const int steps_all = int(g.kp / kGroup);
     const int per = (steps_all + g.splits - 1) / g.splits;
-    const int k0 = split_i * per, k1 = min(steps_all, k0 + per);
-    const char *ga = g.a + mat * g.a_bytes + int64_t(ti) * kTile * pitch;
-    const char *gb = g.b + mat * g.b_bytes + int64_t(tj) * kTile * pitch;
-    // This lane's chunks: 4 of each operand's tile, rows 8 apart per wave load.
-    constexpr int NL = TB / (4 * kWave * 16);
-    int64_t src[NL];
+    const int k0 = min(steps_all, split_i * per), k1 = min(steps_all, k0 + per);
+    const int64_t panel = int64_t(steps_all) * BLOCK;  // 128 rows
+    const char *ga = g.a + mat * g.a_bytes + int64_t(ti) * (C::BM / kPad) * panel;
+    const char *gb = g.b + mat * g.b_bytes + int64_t(tj) * (C::BM / kPad) * panel;
+    int64_t src[NL];  // this lane's 16-byte chunks of a step
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
         const int p = (wave * NL + i) * kWave + lane;
-        src[i] = int64_t(p / 8) * pitch + 16 * ((p % 8) ^ Tile<64>::swz(p / 8));
+        src[i] = (p / 8 / kPad) * panel + (p / 8 % kPad) * kRowBytes + 16 * ((p % 8) ^ Tile<64>::swz(p / 8));
     }
+    auto buffer = [&](int k) __attribute__((always_inline)) { return L + uint32_t((k - k0) % C::STAGES) * 2 * TB; };
     auto issue = [&](int k) __attribute__((always_inline)) {
-        const uint32_t to = L + uint32_t((k - k0) & 1) * 2 * TB;
+        const uint32_t to = buffer(k);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t dst = to + uint32_t((wave * NL + i) * kWave * 16);
-            const char *pa = ga + src[i] + int64_t(k) * kRowBytes, *pb = gb + src[i] + int64_t(k) * kRowBytes;
+            const char *pa = ga + src[i] + int64_t(k) * BLOCK, *pb = gb + src[i] + int64_t(k) * BLOCK;
             asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(pa),
                          "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
             asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(pb),
                          "s"(__builtin_amdgcn_readfirstlane(dst + TB)) : "memory", "m0");
         }
     };
-    floatx16 acc[2][2];
+    // Waits until step k's loads are in, given that later ones up to step `last` are under way.
+    auto await = [&](int k, int last) __attribute__((always_inline)) {
+        static_assert(2 * NL * 2 <= 63, "vmcnt");
+        const int later = last - k;
+        if (later <= 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (later == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NL) : "memory");
+    };
+    floatx16 acc[MT][NT];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) acc[m][n] = zero16();
-    const uint32_t ra = uint32_t(Tile<64>::off(64 * wm + col, half)), rb = uint32_t(Tile<64>::off(64 * wn + col, half)) + TB;
-    if (k0 < k1) issue(k0);
-    for (int k = k0; k < k1; ++k) {
-        wait_loads();
+        for (int n = 0; n < NT; ++n) acc[m][n] = zero16();
+    const uint32_t ra = uint32_t(Tile<64>::off(32 * MT * wm + col, half)), rb = uint32_t(Tile<64>::off(32 * NT * wn + col, half)) + TB;
+    struct Half {
+        f16x8 ah[MT], al[MT], bh[NT], bl[NT];
+    };
+    auto read = [&](Half &x, int k, int s) __attribute__((always_inline)) {  // chunks 2 s + half of hi, 4 on of lo
+        const uint32_t base = buffer(k);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t p = base + rb + uint32_t(32 * n * kRowBytes);
+            x.bh[n] = lds_b128<f16x8>(p ^ uint32_t(s << 5));
+            x.bl[n] = lds_b128<f16x8>(p ^ uint32_t((s + 2) << 5));
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const uint32_t p = base + ra + uint32_t(32 * m * kRowBytes);
+            x.ah[m] = lds_b128<f16x8>(p ^ uint32_t(s << 5));
+            x.al[m] = lds_b128<f16x8>(p ^ uint32_t((s + 2) << 5));
+        }
+    };
+    auto cross = [&](const Half &x) __attribute__((always_inline)) {  // lo hi
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[m][n] = F16Fmt::mfma(x.al[m], x.bh[n], acc[m][n]);
+    };
+    auto rest = [&](const Half &x) __attribute__((always_inline)) {  // hi lo, hi hi
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[m][n] = F16Fmt::mfma(x.ah[m], x.bl[n], acc[m][n]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[m][n] = F16Fmt::mfma(x.ah[m], x.bh[n], acc[m][n]);
+    };
+    // Keeps LDS reads and products in the order they are written in.
+    auto keep_order = [&]() __attribute__((always_inline)) {
+        asm volatile("" ::: "memory");
+        read_fence();
+    };
+    if (k0 < k1) {
+        int last = min(k1 - 1, k0 + C::STAGES - 2);  // the last step whose loads are under way
+        for (int k = k0; k <= last; ++k) issue(k);
+        await(k0, last);
         lds_barrier();
-        if (k + 1 < k1) issue(k + 1);
-        const uint32_t base = L + uint32_t((k - k0) & 1) * 2 * TB;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {  // 16 of the contraction: chunks 2 s + half of hi, 4 more on of lo
-            f16x8 ah[2], al[2], bh[2], bl[2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const uint32_t pa = base + ra + uint32_t(32 * m * kRowBytes), pb = base + rb + uint32_t(32 * m * kRowBytes);
-                ah[m] = lds_b128<f16x8>(pa ^ uint32_t(s << 5));
-                al[m] = lds_b128<f16x8>(pa ^ uint32_t((s + 2) << 5));
-                bh[m] = lds_b128<f16x8>(pb ^ uint32_t(s << 5));
-                bl[m] = lds_b128<f16x8>(pb ^ uint32_t((s + 2) << 5));
+        if (last + 1 < k1) issue(++last);
+        Half x, y;
+        read(x, k0, 0);
+        for (int k = k0; k < k1; ++k) {
+            cross(x);
+            keep_order();
+            read(y, k, 1);
+            keep_order();
+            rest(x);
+            keep_order();
+            cross(y);
+            keep_order();
+            if (k + 1 < k1) {
+                // Every wave has step k in registers: its buffer takes the next loads.
+                await(k + 1, last);
+                lds_barrier();
+                if (last + 1 < k1) issue(++last);
+                read(x, k + 1, 0);
             }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    acc[m][n] = F16Fmt::mfma(al[m], bh[n], acc[m][n]);
-                    acc[m][n] = F16Fmt::mfma(ah[m], bl[n], acc[m][n]);
-                    acc[m][n] = F16Fmt::mfma(ah[m], bh[n], acc[m][n]);
-                }
+            keep_order();
+            rest(y);
         }
     }
     if (g.splits > 1) {
         // This split's sums, in register order: the joining wave reads them back the same way.
-        float *to = g.part + ((int64_t(mat) * tiles + t) * g.splits + split_i) * kTile * kTile + wave * 64 * 64;
+        float *to = g.part + ((int64_t(mat) * tiles + t) * g.splits + split_i) * C::BM * C::BM + wave * (MT * NT * 1024);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<floatx4 *>(to + (((m * 2 + n) * 4 + q) * kWave + lane) * 4) =
+                    *reinterpret_cast<floatx4 *>(to + (((m * NT + n) * 4 + q) * kWave + lane) * 4) =
                         floatx4{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
         return;
     }
     lds_barrier();  // every wave is done with the tiles
-    uint32_t *buf = reinterpret_cast<uint32_t *>(smem) + wave * 32 * 33;
+    const uint32_t buf = L + uint32_t(wave * kBufBytes);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-            leave<T, P>(g, mat, acc[m][n], int64_t(ti) * kTile + 64 * wm + 32 * m, int64_t(tj) * kTile + 64 * wn + 32 * n,
+        for (int n = 0; n < NT; ++n)
+            leave<T, P>(g, mat, acc[m][n], ti * C::BM + 32 * (MT * wm + m), tj * C::BM + 32 * (NT * wn + n),
                         SYM && ti != tj, buf, lane);
 }
 
 // Joins the splits' sums in order: one wave per 32 x 32 block of a tile.
-template <typename T, int P>
+template <typename T, int P, typename TC>
 __global__ __launch_bounds__(256) void join_product_kernel(Gemm g) {
+    using C = Tiling<TC>;
     constexpr bool SYM = P == kGram || P == kPoly;
-    __shared__ uint32_t buf[4][32 * 33];
+    __shared__ __attribute__((aligned(1024))) char buf[4 * kBufBytes];
     const int lane = threadIdx.x & (kWave - 1);
     const int tiles = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-    const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;  // block 0 .. 15 of a tile
-    const int t = int(w / 16 % tiles), mat = int(w / 16 / tiles), blk = int(w % 16);
+    const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / kWave;
+    const int t = int(w / C::BLOCKS % tiles), mat = int(w / C::BLOCKS / tiles), blk = int(w % C::BLOCKS);
     if (mat >= g.mats) return;
     int ti, tj;
     if (SYM) lower_tile(t, ti, tj);
     else ti = t % g.tiles_m, tj = t / g.tiles_m;
-    const int wave = blk / 4, m = blk / 2 % 2, n = blk % 2;
+    const int wave = blk / (C::MT * C::NT), m = blk / C::NT % C::MT, n = blk % C::NT;
     floatx16 acc = zero16();
-    const float *from = g.part + (int64_t(mat) * tiles + t) * g.splits * kTile * kTile + wave * 64 * 64;
-    for (int s = 0; s < g.splits; ++s, from += kTile * kTile)
+    const float *from = g.part + (int64_t(mat) * tiles + t) * g.splits * C::BM * C::BM + blk * 1024;
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const floatx4 x = *reinterpret_cast<const floatx4 *>(from + (((m * 2 + n) * 4 + q) * kWave + lane) * 4);
+            const floatx4 x = *reinterpret_cast<const floatx4 *>(from + int64_t(s) * C::BM * C::BM + (q * kWave + lane) * 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[4 * q + e] += x[e];
         }
-    leave<T, P>(g, mat, acc, int64_t(ti) * kTile + 64 * (wave / 2) + 32 * m, int64_t(tj) * kTile + 64 * (wave % 2) + 32 * n,
-                SYM && ti != tj, buf[threadIdx.x / kWave], lane);
+    leave<T, P>(g, mat, acc, ti * C::BM + 32 * (C::MT * (wave / C::WN) + m),
+                tj * C::BM + 32 * (C::NT * (wave % C::WN) + n), SYM && ti != tj, lds_addr(buf) + uint32_t(threadIdx.x / kWave * kBufBytes), lane);
 }
 
 // ---- sizes and launches ----
@@ -401,15 +511,29 @@ struct Layout {
     int64_t off_norm, off_x, off_xt[2], off_a, off_b, off_part, bytes;
 };
 
-// Workgroups that a launch should have at least; K steps that a split should keep.
-constexpr int kWantGroups = 512;
-constexpr int kMinSteps = 8;
-
-int splits_of(int64_t tiles, int64_t kp) {
-    const int64_t steps = kp / kGroup;
-    int64_t s = kWantGroups / std::max<int64_t>(tiles, 1);
-    s = std::min(s, steps / kMinSteps);
-    return int(std::max<int64_t>(1, std::min<int64_t>(s, 32)));
+// How a product runs: the tile shape and the splits of K with the least estimated time, one workgroup a CU at a
+// time on 256 CUs.  A step of a small tile takes 0.62 us, of a large one 2.5; a workgroup's start and end 12 or 13; joining
+// costs a launch and the splits' sums there and back.
+struct Choice {
+    bool large;
+    int splits;
+};
+Choice choose(bool sym, int64_t mats, int64_t m, int64_t n, int64_t kp) {
+    Choice best{false, 1};
+    double least = 1e30;
+    for (int large = 0; large < 2; ++large) {
+        const int64_t bm = large ? LargeTile::BM : SmallTile::BM;
+        if (m % bm != 0 || n % bm != 0) continue;
+        const int64_t tiles = mats * (sym ? (m / bm) * (m / bm + 1) / 2 : (m / bm) * (n / bm)), steps = kp / kGroup;
+        for (int64_t s = 1; s <= 32 && s * 4 <= steps; ++s) {
+            const double rounds = double((tiles * s + 255) / 256);
+            double us = rounds * (double((steps + s - 1) / s) * (large ? 2.5 : 0.62) + (large ? 13 : 12));
+            if (s > 1) us += 4 + double(tiles * s) * double(bm * bm) * 8 / 6e6;
+            if (us < least) least = us, best = {large != 0, int(s)};
+            if (tiles * s > 512) break;
+        }
+    }
+    return best;
 }
 
 Layout layout(int64_t mats, int64_t rows, int64_t cols) {
@@ -419,7 +543,11 @@ Layout layout(int64_t mats, int64_t rows, int64_t cols) {
     l.s.tall = rows > cols;
     l.s.r = std::min(rows, cols);
     l.s.c = std::max(rows, cols);
-    auto pad = [](int64_t x) { return (x + kPad - 1) / kPad * kPad; };
+    // Sides from 1024 on to the large tile.
+    auto pad = [](int64_t x) {
+        const int64_t to = x >= 1024 ? LargeTile::BM : kPad;
+        return (x + to - 1) / to * to;
+    };
     l.s.rp = pad(l.s.r);
     l.s.cp = pad(l.s.c);
     l.x_bytes = l.s.rp * l.s.cp * 4;
@@ -436,27 +564,37 @@ Layout layout(int64_t mats, int64_t rows, int64_t cols) {
     l.off_xt[1] = take(mats * l.x_bytes);
     l.off_a = take(mats * l.a_bytes);
     l.off_b = take(mats * l.a_bytes);
-    const int64_t tm = l.s.rp / kTile, tn = l.s.cp / kTile, sym = mats * (tm * (tm + 1) / 2), full = mats * tm * tn;
-    auto part = [&](int64_t tiles, int64_t kp) {
-        const int s = splits_of(tiles, kp);
-        return s > 1 ? tiles * s * kTile * kTile * int64_t(4) : 0;
+    auto part = [&](bool sym, int64_t n, int64_t kp) {
+        const Choice ch = choose(sym, mats, l.s.rp, n, kp);
+        const int64_t bm = ch.large ? LargeTile::BM : SmallTile::BM, tm = l.s.rp / bm;
+        return ch.splits > 1 ? mats * (sym ? tm * (tm + 1) / 2 : tm * (n / bm)) * ch.splits * bm * bm * int64_t(4) : 0;
     };
-    l.off_part = take(std::max({part(sym, l.s.cp), part(sym, l.s.rp), part(full, l.s.rp)}));
+    l.off_part = take(std::max({part(true, l.s.rp, l.s.cp), part(true, l.s.rp, l.s.rp), part(false, l.s.cp, l.s.rp)}));
     l.bytes = at;
     return l;
 }
 
-template <typename T, int P> hipError_t product(Gemm g, hipStream_t st) {
-    constexpr bool SYM = P == kGram || P == kPoly;
-    const int64_t tiles = int64_t(g.mats) * (SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n);
-    g.splits = splits_of(tiles, g.kp);
-    const int64_t groups = (tiles * g.splits + 7) / 8 * 8;
-    if (!grid_fits(groups, 256) || !grid_fits(tiles * 4, 256)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((product_kernel<T, P>), dim3(unsigned(groups)), dim3(256), 0, st, g);
+template <typename T, int P, typename TC> hipError_t run_product(const Gemm &g, int64_t tiles, hipStream_t st) {
+    using C = Tiling<TC>;
+    const int64_t groups = (tiles * g.splits + 7) / 8 * 8, joins = (tiles * C::BLOCKS + 3) / 4;
+    if (!grid_fits(groups, C::WAVES * kWave) || !grid_fits(joins, 256)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((product_kernel<T, P, TC>), dim3(unsigned(groups)), dim3(C::WAVES * kWave), 0, st, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || g.splits == 1) return e;
-    hipLaunchKernelGGL((join_product_kernel<T, P>), dim3(unsigned(tiles * 4)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((join_product_kernel<T, P, TC>), dim3(unsigned(joins)), dim3(256), 0, st, g);
     return hipGetLastError();
+}
+
+// a [m rows] b [n rows]^T.
+template <typename T, int P> hipError_t product(Gemm g, int64_t m, int64_t n, hipStream_t st) {
+    constexpr bool SYM = P == kGram || P == kPoly;
+    const Choice ch = choose(SYM, g.mats, m, n, g.kp);
+    const int64_t bm = ch.large ? LargeTile::BM : SmallTile::BM;
+    g.splits = ch.splits;
+    g.tiles_m = int(m / bm);
+    g.tiles_n = int(n / bm);
+    const int64_t tiles = int64_t(g.mats) * (SYM ? int64_t(g.tiles_m) * (g.tiles_m + 1) / 2 : int64_t(g.tiles_m) * g.tiles_n);
+    return ch.large ? run_product<T, P, LargeTile>(g, tiles, st) : run_product<T, P, SmallTile>(g, tiles, st);
 }
 
 struct Args {
@@ -469,12 +607,25 @@ struct Args {
 template <typename T> hipError_t orthogonalise(const Args &x, const Layout &l, char *ws, hipStream_t st) {
     double *norm = reinterpret_cast<double *>(ws + l.off_norm);
     const int64_t n = l.s.rows * l.s.cols;
-    const int blocks = int(std::min<int64_t>(kNormBlocks, (n + 1023) / 1024));
-    hipLaunchKernelGGL(norm_kernel<T>, dim3(unsigned(blocks), unsigned(x.mats)), dim3(256), 0, st, x.g, x.m, x.u, n, norm);
+    const int blocks = int(std::max<int64_t>(1, std::min<int64_t>(kNormBlocks, n / 4096)));
+    constexpr int V = 16 / int(sizeof(T));
+    uintptr_t at = reinterpret_cast<uintptr_t>(x.g.base);
+    if (!x.g.base)
+        for (int i = 0; i < x.mats; ++i) at |= reinterpret_cast<uintptr_t>(x.g.p[i]);
+    if (n % V == 0 && at % 16 == 0)
+        hipLaunchKernelGGL((norm_kernel<T, V>), dim3(unsigned(blocks), unsigned(x.mats)), dim3(256), 0, st, x.g, x.m, x.u, n, norm);
+    else
+        hipLaunchKernelGGL((norm_kernel<T, 1>), dim3(unsigned(blocks), unsigned(x.mats)), dim3(256), 0, st, x.g, x.m, x.u, n, norm);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(split_kernel<T>, dim3(unsigned(l.s.cp / 64), unsigned(l.s.rp / 64), unsigned(x.mats)), dim3(256), 0,
-                       st, x.g, x.m, x.u, l.s, x.eps, norm, blocks, ws + l.off_x, ws + l.off_xt[0], l.x_bytes);
+    const int64_t gr = l.s.tall ? l.s.cp : l.s.rp, gc = l.s.tall ? l.s.rp : l.s.cp;  // G's padded shape
+    const dim3 grid(unsigned(gc / 128), unsigned(gr / 32), unsigned(x.mats));
+    auto split_g = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x.g, x.m, x.u, l.s, x.eps, norm, blocks, ws + l.off_x,
+                           ws + l.off_xt[0], l.x_bytes);
+    };
+    if (l.s.cols % 4 == 0 && at % 16 == 0) split_g(split_kernel<T, true>);
+    else split_g(split_kernel<T, false>);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     Gemm g{};
     g.mats = x.mats;
@@ -490,26 +641,24 @@ template <typename T> hipError_t orthogonalise(const Args &x, const Layout &l, c
         g.a = g.b = ws + l.off_x;
         g.a_bytes = g.b_bytes = l.x_bytes;
         g.kp = l.s.cp;
-        g.tiles_m = g.tiles_n = int(l.s.rp / kTile);
         g.o = ws + l.off_a;
         g.o_bytes = l.a_bytes;
-        g.o_pitch = 4 * l.s.rp;
-        if ((e = product<T, kGram>(g, st)) != hipSuccess) return e;
+        g.o_groups = int(l.s.rp / kGroup);
+        if ((e = product<T, kGram>(g, l.s.rp, l.s.rp, st)) != hipSuccess) return e;
         g.a = g.b = g.gram = ws + l.off_a;
         g.a_bytes = g.b_bytes = l.a_bytes;
         g.kp = l.s.rp;
         g.o = ws + l.off_b;
-        if ((e = product<T, kPoly>(g, st)) != hipSuccess) return e;
+        if ((e = product<T, kPoly>(g, l.s.rp, l.s.rp, st)) != hipSuccess) return e;
         g.a = ws + l.off_b;
         g.b = xt;
         g.b_bytes = l.x_bytes;
-        g.tiles_n = int(l.s.cp / kTile);
         g.o = ws + l.off_x;
         g.ot = ws + l.off_xt[(i + 1) % 2];
         g.o_bytes = l.x_bytes;
-        g.o_pitch = 4 * l.s.cp;
-        g.ot_pitch = 4 * l.s.rp;
-        e = i + 1 == x.steps ? product<T, kLast>(g, st) : product<T, kApply>(g, st);
+        g.o_groups = int(l.s.cp / kGroup);
+        g.ot_groups = int(l.s.rp / kGroup);
+        e = i + 1 == x.steps ? product<T, kLast>(g, l.s.rp, l.s.cp, st) : product<T, kApply>(g, l.s.rp, l.s.cp, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -521,6 +670,13 @@ hipError_t typed(int dtype, const Args &x, const Layout &l, char *ws, hipStream_
         case CTATTN_BF16: return orthogonalise<bf16_t>(x, l, ws, st);
         default: return orthogonalise<f16_t>(x, l, ws, st);
     }
+}
+
+// Bytes for `count` matrices in batches of kMaxMats: the last, smaller batch may split its products more.
+int64_t batches_bytes(int64_t count, int64_t rows, int64_t cols) {
+    int64_t need = layout(std::min<int64_t>(count, kMaxMats), rows, cols).bytes;
+    if (count > kMaxMats && count % kMaxMats != 0) need = std::max(need, layout(count % kMaxMats, rows, cols).bytes);
+    return need;
 }
 
 using capi::fail;
@@ -590,7 +746,7 @@ int ctattn_newton_schulz(int dtype, const void *x, void *out, void *workspace, i
 
 int64_t ctattn_muon_update_workspace_bytes(int dtype, int64_t count, int64_t rows, int64_t cols) {
     if (check("ctattn_muon_update_workspace_bytes", dtype, count, rows, cols, 1, 0, 0, 0, 0) != 0) return -1;
-    return count == 0 ? 0 : layout(std::min<int64_t>(count, kMaxMats), rows, cols).bytes;
+    return count == 0 ? 0 : batches_bytes(count, rows, cols);
 }
 
 int ctattn_muon_update_multi(int dtype, int count, void *const *param, const void *const *grad, void *const *moment,
@@ -603,7 +759,7 @@ int ctattn_muon_update_multi(int dtype, int count, void *const *param, const voi
     if (!param || !grad || !moment) return fail(hipErrorInvalidValue, "%s: null pointer table", fn);
     for (int i = 0; i < count; ++i)
         if (!param[i] || !grad[i] || !moment[i]) return fail(hipErrorInvalidValue, "%s: null pointer in matrix %d", fn, i);
-    if (int rc = check_workspace(fn, workspace, workspace_bytes, layout(std::min(count, kMaxMats), rows, cols).bytes)) return rc;
+    if (int rc = check_workspace(fn, workspace, workspace_bytes, batches_bytes(count, rows, cols))) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int i0 = 0; i0 < count; i0 += kMaxMats) {
         Args y{};

@@ -210,7 +210,8 @@ def test_c_entry_refusals():
     need = lib.ctattn_newton_schulz_workspace_bytes(0, 1, 8, 6)
     assert need > 0 and ns(size=need - 1) == 1 and lib.ctattn_newton_schulz_workspace_bytes(0, 1, 0, 6) == -1
     need = lib.ctattn_muon_update_workspace_bytes(1, 100, 8, 6)
-    assert need == lib.ctattn_muon_update_workspace_bytes(1, 64, 8, 6) > 0
+    # Batches of 64 and the rest.
+    assert need == max(lib.ctattn_muon_update_workspace_bytes(1, n, 8, 6) for n in (64, 36)) > 0
     one = (ctypes.c_void_p * 1)(64)
     none = (ctypes.c_void_p * 1)(None)
 
