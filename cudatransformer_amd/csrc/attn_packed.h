@@ -24,8 +24,8 @@ struct PackedItem {
     int32_t seq;
 };
 // Tile kinds: rows of (token, head of the group) for the forward and dQ, keys for dK / dV.
-enum PackedTile { kRows64 = 0, kRows128, kRows256, kKeys64, kKeys128, kPackedTiles };
-constexpr int kPackedTileSize[kPackedTiles] = {64, 128, 256, 64, 128};
+enum PackedTile { kRows32 = 0, kRows64, kRows128, kKeys32, kKeys64, kKeys128, kPackedTiles };
+constexpr int kPackedTileSize[kPackedTiles] = {32, 64, 128, 32, 64, 128};
 
 struct PackedTable {
     int64_t offset;  // bytes from the start of the buffer
@@ -36,7 +36,7 @@ struct PackedHeader {
     int64_t bytes;
     int64_t nseq, tokens, max_len, group;
     int64_t cu_offset;
-    int64_t reserved;
+    int64_t pairs, pairs_causal;  // (query token, key) pairs within sequences, unmasked and causal
     PackedTable table[2][kPackedTiles];  // [causal][kind]
 };
 constexpr int64_t kPackedMagic = 0x63746b6470616b31ll;

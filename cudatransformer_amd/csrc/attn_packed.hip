@@ -29,6 +29,7 @@ namespace {
 using namespace packedtile;
 
 constexpr float kRaise = 8.0f;       // raise the running maximum when a block exceeds it by 2^8
+constexpr float kLowest = -3.402823466e38f;  // the running maximum before any score (finite: m - m is 0, not NaN)
 constexpr float kPsumLimit = 256.f;  // a lane's share of a block's P below which no P exceeds 2^8
 
 // Byte strides and pointers of one [tokens, heads, d] tensor.
@@ -46,23 +47,32 @@ struct FwdArgs {
     float c;                        // log2(e) / sqrt(d)
 };
 
-template <typename F, int D> struct FwdCfg {
+// How a workgroup's 4 waves share its work: RS slices of 32 rows x KS slices of 32 KT keys of every block.
+// KS > 1: the waves of a row slice hold sums over different keys and join them at the end; for grids that
+// would leave CUs idle, or wait for the one workgroup with the longest sequence.
+template <int RS_, int KS_, int KT_> struct Waves {
+    static constexpr int RS = RS_, KS = KS_, KT = KT_;
+    static_assert(RS * KS == 4, "4 waves");
+    static constexpr PackedTile ROWS = RS == 4 ? kRows128 : RS == 2 ? kRows64 : kRows32;
+};
+template <typename F, int D, typename W> struct FwdCfg : W {
     static constexpr int NW = 4;
-    static constexpr int BM = 32 * NW;
-    static constexpr int BN = 64;
-    static constexpr int KT = BN / 32;
+    static constexpr int BM = 32 * W::RS;
+    static constexpr int BN = 32 * W::KT * W::KS;
     static constexpr int DT = D / 32;
     static constexpr int RB = D * F::ES;
     static constexpr int STEPS = RB / 32;
     static constexpr int KB = BN * RB;
-    static constexpr int LDS = 4 * KB;  // buffer b: K at 2 b KB, V behind it
-    static constexpr int WPE = LDS > 80 * 1024 ? 1 : 2;
+    // Two buffers, or with shared keys one where that lets a second workgroup onto the CU.
+    static constexpr int NBUF = W::KS > 1 && 4 * KB > 80 * 1024 ? 1 : 2;
+    static constexpr int LDS = NBUF * 2 * KB;  // buffer b: K at 2 b KB, V behind it
+    static constexpr int WPE = RB > 256 || LDS > 80 * 1024 ? 1 : 2;
 };
 
-template <typename F, int D, bool PAD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D>::WPE, 2))) void packed_fwd_kernel(
+template <typename F, int D, bool PAD, typename W>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D, W>::WPE, 2))) void packed_fwd_kernel(
     FwdArgs a) {
-    using C = FwdCfg<F, D>;
+    using C = FwdCfg<F, D, W>;
     using V = typename F::vec;
     using S = typename F::store;
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
@@ -74,12 +84,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
     const int kvh = blockIdx.x % a.hkv;
     const PackedItem it = a.items[blockIdx.x / a.hkv];
     const int rows = it.len * a.group;
-    const int r0 = it.tile * C::BM;
-    const int row = r0 + 32 * wave + col;
+    const int rs = wave % C::RS, ks = wave / C::RS;
+    const int r0 = it.tile * C::BM, r0w = r0 + 32 * rs;
+    const int row = r0w + col;
     const int token = row / a.group, head = kvh * a.group + row % a.group;
-    const int first_token = (r0 + 32 * wave) / a.group;  // of this wave
-    const int last_token = min((r0 + 32 * wave + 31) / a.group, it.len - 1);
-    const bool wave_rows = r0 + 32 * wave < rows;
+    const int first_token = r0w / a.group;  // of this wave
+    const int last_token = min((r0w + 31) / a.group, it.len - 1);
+    const int koff = 32 * C::KT * ks;       // of this wave's keys in a block
 
     V qb[C::STEPS];
     {
@@ -95,7 +106,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
     floatx16 oacc[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) oacc[dt] = zero16();
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = kLowest, l_run = 0.f;
 
     const uint32_t rk = uint32_t(Tile<C::RB / 2>::off(col, half));
     const uint32_t cv0 = F::template col0<C::RB>(lane), cv1 = F::template col1<C::RB>(lane);
@@ -104,16 +115,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
     const int kend = a.causal ? min(it.len, (min(r0 + C::BM, rows) - 1) / a.group + 1) : it.len;
     const int nkb = (kend + C::BN - 1) / C::BN;
     auto issue = [&](int kb) __attribute__((always_inline)) {
-        const uint32_t t = L + uint32_t((kb & 1) * 2 * C::KB);
+        const uint32_t t = L + uint32_t((kb % C::NBUF) * 2 * C::KB);
         const int j0 = kb * C::BN;
         load_rows<C::RB, C::BN, C::NW, PAD>(t, kb0 + j0 * a.k.row, a.k.row, a.width, it.len - j0, wave, lane);
         load_rows<C::RB, C::BN, C::NW, PAD>(t + C::KB, vb0 + j0 * a.v.row, a.v.row, a.width, it.len - j0, wave, lane);
     };
-    // One 64-key block.  MASK: it crosses the wave's diagonal or the sequence's end.
+    // This wave's keys of a block.  MASK: they cross the wave's diagonal or the sequence's end.
     auto block = [&](auto mask, int kb) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask)::value;
-        const int j0 = kb * C::BN;
-        const uint32_t kt0 = L + uint32_t((kb & 1) * 2 * C::KB);
+        const int j0 = kb * C::BN + koff;
+        const uint32_t kt0 = L + uint32_t((kb % C::NBUF) * 2 * C::KB) + uint32_t(koff * C::RB);
         bool active[C::KT];
         floatx16 sacc[C::KT];
 #pragma unroll
@@ -165,7 +176,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
             }
             top = max_xor32(top) * a.c;
             if (__any(top > m_run + kRaise)) {
-                // Key 0 is in every row's mask and in its first block, so m is finite from there on.
+                // A row that sees none of the wave's keys yet keeps m at the lowest: P = 2^(-inf) = 0.
                 const float m_new = fmaxf(m_run, top);
                 const float resc = fast_exp2(m_run - m_new);
                 m_run = m_new;
@@ -195,17 +206,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
     };
 
     auto step = [&](int kb) __attribute__((always_inline)) {
+        if (C::NBUF == 1 && kb > 0) {
+            lds_barrier();  // every wave is done with the last block
+            issue(kb);
+        }
         // This wave's loads of the block have landed; after the barrier every wave's have, and
-        // every wave is done reading the other buffer.
+        // (two buffers) every wave is done reading the other one.
         wait_loads();
         lds_barrier();
-        if (kb + 1 < nkb) issue(kb + 1);
+        if (C::NBUF == 2 && kb + 1 < nkb) issue(kb + 1);
     };
     // This wave's blocks, in loops without branches inside (one loop over both variants makes the
     // compiler copy the accumulators): [0, jp) whole, [jp, jw) across the diagonal or the end,
     // [jw, nkb) none of its pairs.
-    const int jw = !wave_rows ? 0 : a.causal ? last_token / C::BN + 1 : nkb;
-    const int jp = min(jw, min(it.len, a.causal ? first_token + 1 : it.len) / C::BN);
+    const int kwhole = a.causal ? min(it.len, first_token + 1) : it.len;  // keys that every row of the wave sees
+    const int ksome = a.causal ? last_token + 1 : it.len;                 // and any of them
+    const int jw = r0w < rows && ksome > koff ? (ksome - koff + C::BN - 1) / C::BN : 0;
+    const int jp = min(jw, kwhole >= koff + 32 * C::KT ? (kwhole - koff - 32 * C::KT) / C::BN + 1 : 0);
     issue(0);
     int kb = 0;
     for (; kb < jp; ++kb) {
@@ -218,6 +235,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
     }
     for (; kb < nkb; ++kb) step(kb);
 
+    if constexpr (C::KS > 1) {
+        // The key slices of a row slice join: m = max, O and l weighted by 2^(their m - m).  A slice that
+        // saw no key has the lowest m, weight 0; the first saw key 0.
+        constexpr int NR = C::DT * 16 + 2;
+        static_assert((C::KS - 1) * C::RS * NR * kWave * 4 <= C::LDS, "join buffer");
+        float *jb = reinterpret_cast<float *>(smem);
+        lds_barrier();  // every wave is done with the tiles
+        if (ks > 0) {
+            float *to = jb + ((ks - 1) * C::RS + rs) * NR * kWave + lane;
+#pragma unroll
+            for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) to[(dt * 16 + r) * kWave] = oacc[dt][r];
+            to[(NR - 2) * kWave] = m_run;
+            to[(NR - 1) * kWave] = l_run;
+        }
+        lds_barrier();
+        if (ks > 0) return;
+        const float *from = jb + rs * NR * kWave + lane;
+        float m = m_run, w[C::KS - 1];
+#pragma unroll
+        for (int i = 0; i < C::KS - 1; ++i) m = fmaxf(m, from[i * C::RS * NR * kWave + (NR - 2) * kWave]);
+        const float w0 = fast_exp2(m_run - m);
+        l_run *= w0;
+#pragma unroll
+        for (int i = 0; i < C::KS - 1; ++i) {
+            w[i] = fast_exp2(from[i * C::RS * NR * kWave + (NR - 2) * kWave] - m);
+            l_run += from[i * C::RS * NR * kWave + (NR - 1) * kWave] * w[i];
+        }
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float x = oacc[dt][r] * w0;
+#pragma unroll
+                for (int i = 0; i < C::KS - 1; ++i) x += from[i * C::RS * NR * kWave + (dt * 16 + r) * kWave] * w[i];
+                oacc[dt][r] = x;
+            }
+        m_run = m;
+    }
     const float l_tot = l_run + __shfl_xor(l_run, 32, kWave);
     const float inv_l = 1.f / l_tot;
     if (row < rows) {
@@ -239,40 +296,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
 
 // ---- backward ----
 
-// -delta = -rowsum(dO O) and -L log2(e) of every (token, head), laid out as the kernels walk them: rows
-// (token, head of the group) behind each other for each key head.  16 lanes a row.
-template <typename F>
-__global__ __launch_bounds__(256) void packed_rowstats_kernel(View o, View dout, const float *__restrict__ lse,
-                                                             float *__restrict__ ndelta, float *__restrict__ nl2,
-                                                             int64_t rows, int64_t tokens, int hkv, int group,
-                                                             int width) {
-    using V = typename F::store;
-    constexpr int EC = 16 / F::ES;
-    typedef V vecv __attribute__((ext_vector_type(EC)));
-    const int hq = hkv * group;
-    const int64_t stride = int64_t(gridDim.x) * blockDim.x;
-    for (int64_t t = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; t / 16 < rows; t += stride) {
-        const int64_t row = t / 16, n = row / hq;
-        const int h = int(row % hq);
-        float s = 0.f;
-        for (int c = 16 * int(t % 16); c < width; c += 256) {
-            const vecv x = *reinterpret_cast<const vecv *>(o.at(n, h) + c);
-            const vecv y = *reinterpret_cast<const vecv *>(dout.at(n, h) + c);
-#pragma unroll
-            for (int e = 0; e < EC; ++e) s += F::widen(x[e]) * F::widen(y[e]);
-        }
-        s = group_sum<16>(s);
-        if (t % 16 == 0) {
-            const int64_t at = (int64_t(h / group) * tokens + n) * group + h % group;
-            ndelta[at] = -s;
-            nl2[at] = -lse[row] * kLog2e;
-        }
-    }
-}
-
 struct BwdArgs {
-    View q, k, v, dout, dq, dk, dv;
-    const float *ndelta, *nl2;
+    View q, k, v, o, dout, dq, dk, dv;
+    const float *lse;
+    // -delta = -rowsum(dO O) and -L log2(e) of every (token, head), rows (token, head of the group) behind each
+    // other for each key head, as the dK / dV kernel walks them.  The dQ kernel, which has dO's rows in
+    // registers, runs first and writes them.
+    float *ndelta, *nl2;
     const PackedItem *items;
     int64_t tokens;
     int hkv, group, causal, width;
@@ -280,31 +310,35 @@ struct BwdArgs {
     float c, inv_sqrt_d;
 };
 
-template <typename F, int D> struct KvCfg {
+// KS slices of 32 keys x RS slices of 32 rows, one wave each; the row slices' sums join at the end.
+template <int KS_, int RS_, int NBUF_> struct KvWaves {
+    static constexpr int KS = KS_, RS = RS_, NBUF = NBUF_;
+    static constexpr PackedTile KEYS = KS == 4 ? kKeys128 : KS == 2 ? kKeys64 : kKeys32;
+};
+template <typename F, int D, typename W> struct KvCfg : W {
     static constexpr int RB = D * F::ES;
-    static constexpr bool WIDE = RB > 256;         // fp32 at D = 128: half the keys, one Q buffer
-    static constexpr int KS = WIDE ? 2 : 4;        // key slices of 32
-    static constexpr int NW = 2 * KS;              // x 2 row slices
-    static constexpr int BN = 32 * KS;
-    static constexpr int BM = 64;
-    static constexpr int NBUF = WIDE ? 1 : 2;
+    static constexpr int NW = W::KS * W::RS;
+    static constexpr int BN = 32 * W::KS;
+    static constexpr int BM = 32 * W::RS;
     static constexpr int DT = D / 32;
     static constexpr int STEPS = RB / 32;
     static constexpr int QB = BM * RB;             // Q (or dO) tile
     static constexpr int KB = BN * RB;
-    static constexpr int K_OFF = NBUF * 2 * QB;    // buffer b: Q at 2 b QB, dO behind it
-    static constexpr int V_OFF = K_OFF + KB;
-    static constexpr int S_OFF = V_OFF + KB;       // buffer b: nl2[BM], ndelta[BM]
-    static constexpr int LDS = S_OFF + NBUF * 2 * BM * 4;
-    static constexpr int WPE = WIDE ? 1 : 2;
-    static constexpr PackedTile KIND = WIDE ? kKeys64 : kKeys128;
-    static_assert(KS * DT * 2 * 16 * kWave * 4 <= LDS, "reduction buffer");
+    // One key slice: its K and V rows in registers instead of LDS, where they fit beside dK and dV.
+    static constexpr bool KREG = W::KS == 1 && !(F::ES == 2 && D == 128);
+    static constexpr int K_OFF = W::NBUF * 2 * QB; // buffer b: Q at 2 b QB, dO behind it
+    static constexpr int V_OFF = K_OFF + (KREG ? 0 : KB);
+    static constexpr int S_OFF = V_OFF + (KREG ? 0 : KB);  // buffer b: nl2[BM], ndelta[BM]
+    static constexpr int LDS = S_OFF + W::NBUF * 2 * BM * 4;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    static constexpr int WPE = NW >= 8 || LDS <= 80 * 1024 ? 2 : 1;
+    static_assert(W::KS * W::RS / 2 * DT * 2 * 16 * kWave * 4 <= LDS, "reduction buffer");
 };
 
-template <typename F, int D, bool PAD>
-__global__ __launch_bounds__((64 * KvCfg<F, D>::NW)) __attribute__((amdgpu_waves_per_eu(KvCfg<F, D>::WPE, 2))) void
+template <typename F, int D, bool PAD, typename W>
+__global__ __launch_bounds__((64 * KvCfg<F, D, W>::NW)) __attribute__((amdgpu_waves_per_eu(KvCfg<F, D, W>::WPE, 2))) void
 packed_dkdv_kernel(BwdArgs a) {
-    using C = KvCfg<F, D>;
+    using C = KvCfg<F, D, W>;
     using V = typename F::vec;
     using S = typename F::store;
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
@@ -322,10 +356,23 @@ packed_dkdv_kernel(BwdArgs a) {
     const int key = kw0 + col;
     const int64_t sbase = (int64_t(kvh) * a.tokens + it.start) * a.group;
 
-    load_rows<C::RB, C::BN, C::NW, PAD>(L + C::K_OFF, a.k.at(it.start + k0, kvh), a.k.row, a.width, it.len - k0, wave,
-                                        lane);
-    load_rows<C::RB, C::BN, C::NW, PAD>(L + C::V_OFF, a.v.at(it.start + k0, kvh), a.v.row, a.width, it.len - k0, wave,
-                                        lane);
+    V kreg[C::KREG ? C::STEPS : 1], vreg[C::KREG ? C::STEPS : 1];
+    if constexpr (C::KREG) {
+        const char *pk = a.k.at(it.start + key, kvh), *pv = a.v.at(it.start + key, kvh);
+#pragma unroll
+        for (int s = 0; s < C::STEPS; ++s) {
+            floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+            if (key < it.len && (!PAD || 32 * s + 16 * half < a.width)) {
+                x = *reinterpret_cast<const floatx4 *>(pk + 32 * s + 16 * half);
+                y = *reinterpret_cast<const floatx4 *>(pv + 32 * s + 16 * half);
+            }
+            kreg[s] = __builtin_bit_cast(V, x);
+            vreg[s] = __builtin_bit_cast(V, y);
+        }
+    } else {
+        load_rows<C::RB, C::BN, C::NW, PAD>(L + C::K_OFF, a.k.at(it.start + k0, kvh), a.k.row, a.width, it.len - k0, wave, lane);
+        load_rows<C::RB, C::BN, C::NW, PAD>(L + C::V_OFF, a.v.at(it.start + k0, kvh), a.v.row, a.width, it.len - k0, wave, lane);
+    }
     floatx16 dk[C::DT], dv[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
@@ -358,10 +405,13 @@ packed_dkdv_kernel(BwdArgs a) {
             load_chunk_dma(gq, dst);
             load_chunk_dma(gd, dst + C::QB);
         }
-        if (wave >= C::NW - 2) {
-            const bool is_nl = wave == C::NW - 2;
-            load_dword_dma((is_nl ? a.nl2 : a.ndelta) + sbase + min(r0 + lane, rows - 1),
-                           L + C::S_OFF + uint32_t(buf * 2 * C::BM * 4 + (is_nl ? 0 : C::BM * 4)));
+        // nl2 and ndelta of the block's rows: 64 a load, the last waves' turn.
+        constexpr int SL = (C::BM + kWave - 1) / kWave;
+        static_assert(2 * SL <= C::NW && C::BM % kWave == 0, "row statistics");
+        if (wave >= C::NW - 2 * SL) {
+            const int i = wave - (C::NW - 2 * SL), part = i % SL;
+            load_dword_dma((i < SL ? a.nl2 : a.ndelta) + sbase + min(r0 + part * kWave + lane, rows - 1),
+                           L + C::S_OFF + uint32_t((buf * 2 + i / SL) * C::BM * 4 + part * kWave * 4));
         }
     };
     // One 32-row x 32-key tile: S, dP - delta (its accumulator starts from -delta), P, dS.
@@ -380,22 +430,26 @@ packed_dkdv_kernel(BwdArgs a) {
             V q[2], k[2], g[2], v[2];
             const uint32_t aq = qt + rq;
             q[0] = lds_b128<V>(aq);
-            k[0] = lds_b128<V>(ak);
             g[0] = lds_b128<V>(aq + C::QB);
-            v[0] = lds_b128<V>(ak + C::KB);
+            if (!C::KREG) {
+                k[0] = lds_b128<V>(ak);
+                v[0] = lds_b128<V>(ak + C::KB);
+            }
 #pragma unroll
             for (int st = 0; st < C::STEPS; ++st) {
                 const int cur = st & 1, nxt = cur ^ 1;
                 if (st + 1 < C::STEPS) {
                     const uint32_t xq = aq ^ uint32_t((st + 1) << 5), xk = ak ^ uint32_t((st + 1) << 5);
                     q[nxt] = lds_b128<V>(xq);
-                    k[nxt] = lds_b128<V>(xk);
                     g[nxt] = lds_b128<V>(xq + C::QB);
-                    v[nxt] = lds_b128<V>(xk + C::KB);
+                    if (!C::KREG) {
+                        k[nxt] = lds_b128<V>(xk);
+                        v[nxt] = lds_b128<V>(xk + C::KB);
+                    }
                 }
                 read_fence();
-                s = F::mma(q[cur], k[cur], s);
-                dp = F::mma(g[cur], v[cur], dp);
+                s = F::mma(q[cur], C::KREG ? kreg[C::KREG ? st : 0] : k[cur], s);
+                dp = F::mma(g[cur], C::KREG ? vreg[C::KREG ? st : 0] : v[cur], dp);
             }
         }
         typename F::pvec pb[2], db[2];
@@ -480,19 +534,32 @@ packed_dkdv_kernel(BwdArgs a) {
     }
     for (; qb < nqb; ++qb) step(qb);
 
-    // The second row slice's sums join the first's through LDS.
+    // The row slices' sums join through LDS, the upper half of them added to the lower.
     float *red = reinterpret_cast<float *>(smem);
-    __syncthreads();
-    if (rs == 1) {
 #pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt)
+    for (int h = C::RS / 2; h >= 1; h /= 2) {
+        lds_barrier();
+        float *at = red + ((rs % h) * C::KS + ks) * C::DT * 32 * kWave + lane;
+        if (rs >= h && rs < 2 * h) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                red[(((ks * C::DT + dt) * 2 + 0) * 16 + r) * kWave + lane] = dk[dt][r];
-                red[(((ks * C::DT + dt) * 2 + 1) * 16 + r) * kWave + lane] = dv[dt][r];
-            }
+            for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    at[(dt * 32 + r) * kWave] = dk[dt][r];
+                    at[(dt * 32 + 16 + r) * kWave] = dv[dt][r];
+                }
+        }
+        lds_barrier();
+        if (rs < h) {
+#pragma unroll
+            for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    dk[dt][r] += at[(dt * 32 + r) * kWave];
+                    dv[dt][r] += at[(dt * 32 + 16 + r) * kWave];
+                }
+        }
     }
-    __syncthreads();
     if (rs == 0 && key < it.len) {
         S *dkr = reinterpret_cast<S *>(a.dk.at(it.start + key, kvh));
         S *dvr = reinterpret_cast<S *>(a.dv.at(it.start + key, kvh));
@@ -504,9 +571,8 @@ packed_dkdv_kernel(BwdArgs a) {
                 float xk[4], xv[4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const int r = 4 * g + t;
-                    xk[t] = (dk[dt][r] + red[(((ks * C::DT + dt) * 2 + 0) * 16 + r) * kWave + lane]) * a.inv_sqrt_d;
-                    xv[t] = dv[dt][r] + red[(((ks * C::DT + dt) * 2 + 1) * 16 + r) * kWave + lane];
+                    xk[t] = dk[dt][4 * g + t] * a.inv_sqrt_d;
+                    xv[t] = dv[dt][4 * g + t];
                 }
                 store4<F>(dkr + 32 * dt + 8 * g + 4 * half, xk);
                 store4<F>(dvr + 32 * dt + 8 * g + 4 * half, xv);
@@ -515,22 +581,24 @@ packed_dkdv_kernel(BwdArgs a) {
     }
 }
 
-template <typename F, int D> struct QCfg {
+template <typename F, int D, typename W> struct QCfg : W {
     static constexpr int NW = 4;
-    static constexpr int BM = 32 * NW;
-    static constexpr int BN = 32;
+    static constexpr int BM = 32 * W::RS;
+    static constexpr int BN = 32 * W::KS;
+    static_assert(W::KT == 1, "32 keys of a wave");
     static constexpr int RB = D * F::ES;
     static constexpr int DT = D / 32;
     static constexpr int STEPS = RB / 32;
     static constexpr int KB = BN * RB;
-    static constexpr int LDS = 4 * KB;
-    static constexpr int WPE = RB > 256 ? 1 : 2;
+    static constexpr int NBUF = W::KS > 1 && 4 * KB > 80 * 1024 ? 1 : 2;  // as in the forward
+    static constexpr int LDS = NBUF * 2 * KB;
+    static constexpr int WPE = RB > 256 || LDS > 80 * 1024 ? 1 : 2;
 };
 
-template <typename F, int D, bool PAD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>::WPE, 2))) void packed_dq_kernel(
+template <typename F, int D, bool PAD, typename W>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, W>::WPE, 2))) void packed_dq_kernel(
     BwdArgs a) {
-    using C = QCfg<F, D>;
+    using C = QCfg<F, D, W>;
     using V = typename F::vec;
     using S = typename F::store;
     __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
@@ -542,30 +610,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
     const int kvh = blockIdx.x % a.hkv;
     const PackedItem it = a.items[blockIdx.x / a.hkv];
     const int rows = it.len * a.group;
+    const int rs = wave % C::RS, ks = wave / C::RS, koff = 32 * ks;
     const int r0 = it.tile * C::BM;
-    const int r0w = r0 + 32 * wave;
+    const int r0w = r0 + 32 * rs;
     const int row = r0w + col;
     const int token = row / a.group, head = kvh * a.group + row % a.group;
     const int first_token = r0w / a.group;
     const int last_token = min((r0w + 31) / a.group, it.len - 1);
 
     V qb[C::STEPS], gb[C::STEPS];
+    float nd = 0.f;
     {
         const char *pq = a.q.at(it.start + token, head), *pg = a.dout.at(it.start + token, head);
+        const char *po = a.o.at(it.start + token, head);
 #pragma unroll
         for (int s = 0; s < C::STEPS; ++s) {
-            floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f};
+            floatx4 x = {0.f, 0.f, 0.f, 0.f}, y = {0.f, 0.f, 0.f, 0.f}, z = {0.f, 0.f, 0.f, 0.f};
             if (row < rows && (!PAD || 32 * s + 16 * half < a.width)) {
                 x = *reinterpret_cast<const floatx4 *>(pq + 32 * s + 16 * half);
                 y = *reinterpret_cast<const floatx4 *>(pg + 32 * s + 16 * half);
+                z = *reinterpret_cast<const floatx4 *>(po + 32 * s + 16 * half);
             }
             qb[s] = __builtin_bit_cast(V, x);
             gb[s] = __builtin_bit_cast(V, y);
+            const V ov = __builtin_bit_cast(V, z);
+#pragma unroll
+            for (int e = 0; e < 16 / F::ES; ++e) nd -= float(gb[s][e]) * float(ov[e]);
         }
     }
-    const int64_t sbase = (int64_t(kvh) * a.tokens + it.start) * a.group;
-    const float nl = row < rows ? a.nl2[sbase + row] : 0.f;
-    const float nd = row < rows ? a.ndelta[sbase + row] : 0.f;
+    nd += __shfl_xor(nd, 32, kWave);  // the row's other half
+    float nl = 0.f;
+    if (row < rows) {
+        nl = -a.lse[int64_t(it.start + token) * (a.hkv * a.group) + head] * kLog2e;
+        if (ks == 0 && half == 0) {
+            const int64_t at = (int64_t(kvh) * a.tokens + it.start) * a.group + row;
+            a.ndelta[at] = nd;
+            a.nl2[at] = nl;
+        }
+    }
     floatx16 dq[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) dq[dt] = zero16();
@@ -576,14 +658,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
     const int kend = a.causal ? min(it.len, (min(r0 + C::BM, rows) - 1) / a.group + 1) : it.len;
     const int nkb = (kend + C::BN - 1) / C::BN;
     auto issue = [&](int kb) __attribute__((always_inline)) {
-        const uint32_t t = L + uint32_t((kb & 1) * 2 * C::KB);
+        const uint32_t t = L + uint32_t((kb % C::NBUF) * 2 * C::KB);
         const int j0 = kb * C::BN;
         load_rows<C::RB, C::BN, C::NW, PAD>(t, kb0 + j0 * a.k.row, a.k.row, a.width, it.len - j0, wave, lane);
         load_rows<C::RB, C::BN, C::NW, PAD>(t + C::KB, vb0 + j0 * a.v.row, a.v.row, a.width, it.len - j0, wave, lane);
     };
     auto block = [&](auto mask, int kb) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask)::value;
-        const uint32_t kt = L + uint32_t((kb & 1) * 2 * C::KB);
+        const uint32_t kt = L + uint32_t((kb % C::NBUF) * 2 * C::KB) + uint32_t(koff * C::RB);
         floatx16 s = zero16(), dp;
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = nd;
@@ -608,7 +690,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
         for (int r = 0; r < 16; ++r) {
             float ds = fast_exp2(fmaf(s[r], a.c, nl)) * dp[r];
             if (MASK) {
-                const int key = kb * C::BN + acc_row(r, half);
+                const int key = kb * C::BN + koff + acc_row(r, half);
                 ds = (key >= it.len || (a.causal && key > token)) ? 0.f : ds;
             }
             F::put(db[r / 8], r % 8, ds);
@@ -625,13 +707,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
         }
     };
     auto step = [&](int kb) __attribute__((always_inline)) {
+        if (C::NBUF == 1 && kb > 0) {
+            lds_barrier();
+            issue(kb);
+        }
         wait_loads();
         lds_barrier();
-        if (kb + 1 < nkb) issue(kb + 1);
+        if (C::NBUF == 2 && kb + 1 < nkb) issue(kb + 1);
     };
     // As in the forward; rows past the last one have P = exp2(0 + 0) dP = 0, so they need no mask.
-    const int jw = r0w >= rows ? 0 : a.causal ? last_token / C::BN + 1 : nkb;
-    const int jp = min(jw, min(it.len, a.causal ? first_token + 1 : it.len) / C::BN);
+    const int kwhole = a.causal ? min(it.len, first_token + 1) : it.len;
+    const int ksome = a.causal ? last_token + 1 : it.len;
+    const int jw = r0w < rows && ksome > koff ? (ksome - koff + C::BN - 1) / C::BN : 0;
+    const int jp = min(jw, kwhole >= koff + 32 ? (kwhole - koff - 32) / C::BN + 1 : 0);
     issue(0);
     int kb = 0;
     for (; kb < jp; ++kb) {
@@ -643,6 +731,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
         block(std::true_type{}, kb);
     }
     for (; kb < nkb; ++kb) step(kb);
+    if constexpr (C::KS > 1) {
+        // The key slices' sums join through LDS, the upper half of them added to the lower.
+        static_assert(C::KS / 2 * C::RS * C::DT * 16 * kWave * 4 <= C::LDS, "join buffer");
+        float *jb = reinterpret_cast<float *>(smem);
+#pragma unroll
+        for (int h = C::KS / 2; h >= 1; h /= 2) {
+            lds_barrier();
+            float *at = jb + ((ks % h) * C::RS + rs) * C::DT * 16 * kWave + lane;
+            if (ks >= h && ks < 2 * h) {
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) at[(dt * 16 + r) * kWave] = dq[dt][r];
+            }
+            lds_barrier();
+            if (ks < h) {
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dq[dt][r] += at[(dt * 16 + r) * kWave];
+            }
+        }
+        if (ks > 0) return;
+    }
     if (row < rows) {
         S *p = reinterpret_cast<S *>(a.dq.at(it.start + token, head));
 #pragma unroll
@@ -660,44 +772,83 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D>:
 
 // ---- launches ----
 
+// Whether the grid is short of work for its longest workgroup: that one walks `longest` blocks, and the
+// batch's pairs make fewer than a quarter of as many blocks of `pairs_of_block` for each of the `slots` workgroups that
+// the chip holds at once.  Then smaller tiles, whose waves share the walk, win; else larger ones, which load less for a
+// pair.  Measured, us, causal, larger / smaller tiles, with the ratio:
+//   forward  bf16 d 64: 26 documents of 13.8k tokens, 16/4 heads (1.1) 78 / 155; 8 x 512 16/4 (2) 14 / 25; 4096 4/2 (8)
+//            55 / 28.  d 128: 8192 8/2 (2) 200 / 254; 2048 8/2 (8) 44 / 29.  fp32 d 64: 13 documents of 4k tokens, 6/6 (9)
+//            76 / 36; 16 x 512 12/12 (1.3) 83 / 108.  fp32 d 128: 4 x 1024 8/2 (4) 153 / 104
+//   dK, dV   (whole backward) bf16 d 64: the 26 documents (4.5) 328 / 275; 8 x 512 16/4 (8) 68 / 49; 4096 4/2 (16) 211 /
+//            148; 32 x 512 16/4 (2) 143 / 149; 4 x 2048 16/16 (1) 199 / 232.  d 128: 2048 8/2 (16) 255 / 226;
+//            8192 8/2 (4) 1045 / 1292.  fp32 d 64: the 13 documents (4.7) 244 / 175; 16 x 512 12/12 (0.7) 295 / 315
+//   dQ       (whole backward) bf16 d 64: 4096 4/2 (8) 210 / 169; 4096 16/4 (2) 365 / 370.  fp32 d 64: the 13 documents (9)
+//            244 / 189
+bool short_of_work(const PackedCall &c, int64_t longest, int64_t pairs_of_block, int64_t slots, int64_t ratio = 4) {
+    const double pairs = double(c.causal ? c.host->pairs_causal : c.host->pairs) * double(c.hq);
+    return double(longest) * double(pairs_of_block) * double(slots) >= double(ratio) * pairs;
+}
+
 View view(const void *p, const PackedStride &s, int es) {
     return {static_cast<char *>(const_cast<void *>(p)), s.row * es, s.head * es};
+}
+
+template <typename F, int D, bool PAD, typename W>
+hipError_t fwd_as(const PackedCall &c, FwdArgs a, hipStream_t stream) {
+    const int64_t blocks = c.item_count(W::ROWS) * c.hkv;
+    if (!grid_fits(blocks, 256)) return hipErrorInvalidValue;
+    a.items = c.items(W::ROWS);
+    hipLaunchKernelGGL((packed_fwd_kernel<F, D, PAD, W>), dim3(unsigned(blocks)), dim3(256), 0, stream, a);
+    return hipGetLastError();
 }
 
 template <typename F, int D, bool PAD>
 hipError_t run_fwd(const PackedCall &c, const void *q, const void *k, const void *v, void *o, float *lse,
                    hipStream_t stream) {
-    const int64_t blocks = c.item_count(kRows128) * c.hkv;
-    if (!grid_fits(blocks, 256)) return hipErrorInvalidValue;
     FwdArgs a{view(q, c.sq, F::ES), view(k, c.sk, F::ES), view(v, c.sv, F::ES), view(o, c.so, F::ES), lse,
-              c.items(kRows128), int(c.hkv), int(c.group()), int(c.causal), int(c.d) * F::ES,
-              kLog2e / sqrtf(float(c.d))};
-    hipLaunchKernelGGL((packed_fwd_kernel<F, D, PAD>), dim3(unsigned(blocks)), dim3(256), 0, stream, a);
+              nullptr, int(c.hkv), int(c.group()), int(c.causal), int(c.d) * F::ES, kLog2e / sqrtf(float(c.d))};
+    const bool few = short_of_work(c, (c.host->max_len + 63) / 64, 128 * 64, 2 * device_cus(stream));
+    if constexpr (D * F::ES > 256) return few ? fwd_as<F, D, PAD, Waves<2, 2, 1>>(c, a, stream) : fwd_as<F, D, PAD, Waves<4, 1, 2>>(c, a, stream);
+    else return few ? fwd_as<F, D, PAD, Waves<1, 4, 1>>(c, a, stream) : fwd_as<F, D, PAD, Waves<4, 1, 2>>(c, a, stream);
+}
+
+template <typename F, int D, bool PAD, typename W> hipError_t dkdv_as(const PackedCall &c, BwdArgs a, hipStream_t stream) {
+    const int64_t blocks = c.item_count(W::KEYS) * c.hkv;
+    constexpr int threads = 64 * KvCfg<F, D, W>::NW;
+    if (!grid_fits(blocks, threads)) return hipErrorInvalidValue;
+    a.items = c.items(W::KEYS);
+    hipLaunchKernelGGL((packed_dkdv_kernel<F, D, PAD, W>), dim3(unsigned(blocks)), dim3(threads), 0, stream, a);
+    return hipGetLastError();
+}
+template <typename F, int D, bool PAD, typename W> hipError_t dq_as(const PackedCall &c, BwdArgs a, hipStream_t stream) {
+    const int64_t blocks = c.item_count(W::ROWS) * c.hkv;
+    if (!grid_fits(blocks, 256)) return hipErrorInvalidValue;
+    a.items = c.items(W::ROWS);
+    hipLaunchKernelGGL((packed_dq_kernel<F, D, PAD, W>), dim3(unsigned(blocks)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 template <typename F, int D, bool PAD>
 hipError_t run_bwd(const PackedCall &c, const void *q, const void *k, const void *v, const void *o, const void *dout,
                    const float *lse, float *ws, void *dq, void *dk, void *dv, hipStream_t stream) {
-    using KC = KvCfg<F, D>;
     const int64_t rows = c.tokens() * c.hq;
-    const int64_t kv_blocks = c.item_count(KC::KIND) * c.hkv, q_blocks = c.item_count(kRows128) * c.hkv;
-    if (!grid_fits(kv_blocks, 64 * KC::NW) || !grid_fits(q_blocks, 256)) return hipErrorInvalidValue;
-    BwdArgs a{view(q, c.sq, F::ES), view(k, c.sk, F::ES), view(v, c.sv, F::ES), view(dout, c.sdo, F::ES),
-              view(dq, c.sdq, F::ES), view(dk, c.sdk, F::ES), view(dv, c.sdv, F::ES), ws, ws + rows,
-              c.items(KC::KIND), c.tokens(), int(c.hkv), int(c.group()), int(c.causal), int(c.d) * F::ES,
+    BwdArgs a{view(q, c.sq, F::ES), view(k, c.sk, F::ES), view(v, c.sv, F::ES), view(o, c.so, F::ES),
+              view(dout, c.sdo, F::ES), view(dq, c.sdq, F::ES), view(dk, c.sdk, F::ES), view(dv, c.sdv, F::ES),
+              lse, ws, ws + rows, nullptr, c.tokens(), int(c.hkv), int(c.group()), int(c.causal), int(c.d) * F::ES,
               uint32_t((65536 + c.group() - 1) / c.group()), kLog2e / sqrtf(float(c.d)), 1.f / sqrtf(float(c.d))};
-    hipLaunchKernelGGL((packed_rowstats_kernel<F>), dim3(stride_grid((rows * 16 + 255) / 256, 256)), dim3(256), 0,
-                       stream, view(o, c.so, F::ES), a.dout, lse, ws, ws + rows, rows, c.tokens(), int(c.hkv),
-                       int(c.group()), a.width);
-    hipError_t e = hipGetLastError();
+    constexpr int RB = D * F::ES;
+    const int64_t cus = device_cus(stream);
+    hipError_t e;
+    const bool few_q = short_of_work(c, (c.host->max_len + 63) / 64, 128 * 64, 2 * cus);
+    if constexpr (RB > 256) e = few_q ? dq_as<F, D, PAD, Waves<2, 2, 1>>(c, a, stream) : dq_as<F, D, PAD, Waves<4, 1, 1>>(c, a, stream);
+    else e = few_q ? dq_as<F, D, PAD, Waves<1, 4, 1>>(c, a, stream) : dq_as<F, D, PAD, Waves<4, 1, 1>>(c, a, stream);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((packed_dkdv_kernel<F, D, PAD>), dim3(unsigned(kv_blocks)), dim3(64 * KC::NW), 0, stream, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    a.items = c.items(kRows128);
-    hipLaunchKernelGGL((packed_dq_kernel<F, D, PAD>), dim3(unsigned(q_blocks)), dim3(256), 0, stream, a);
-    return hipGetLastError();
+    // A workgroup of 128 keys walks its first key's rows in blocks of 64; up to 80 KiB of LDS two share a CU.
+    const int64_t walk = (c.host->max_len * c.group() + 63) / 64, slots = RB <= 128 ? 2 * cus : cus;
+    if constexpr (RB > 256) return dkdv_as<F, D, PAD, KvWaves<2, 2, 1>>(c, a, stream);
+    else if constexpr (F::ES == 4) return short_of_work(c, walk, 128 * 64, slots) ? dkdv_as<F, D, PAD, KvWaves<1, 4, 1>>(c, a, stream) : dkdv_as<F, D, PAD, KvWaves<4, 2, 2>>(c, a, stream);
+    else if constexpr (RB <= 128) return short_of_work(c, walk, 128 * 64, slots) ? dkdv_as<F, D, PAD, KvWaves<1, 4, 2>>(c, a, stream) : dkdv_as<F, D, PAD, KvWaves<4, 2, 2>>(c, a, stream);
+    else return short_of_work(c, walk, 128 * 64, slots, 8) ? dkdv_as<F, D, PAD, KvWaves<1, 8, 1>>(c, a, stream) : dkdv_as<F, D, PAD, KvWaves<4, 2, 2>>(c, a, stream);
 }
 
 // The tile width: the next of 32, 64, 128 elements at or above d, rows of another length padded with zeros.

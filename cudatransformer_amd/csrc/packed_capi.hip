@@ -23,7 +23,7 @@ constexpr int64_t kMaxRows = (int64_t(1) << 31) - (int64_t(1) << 20);
 constexpr int64_t kMaxGroup = 4096;
 
 int64_t tiles_of(int64_t len, int64_t group, int kind) {
-    const int64_t n = kind >= kKeys64 ? len : len * group;
+    const int64_t n = kind >= kKeys32 ? len : len * group;
     return (n + kPackedTileSize[kind] - 1) / kPackedTileSize[kind];
 }
 
@@ -45,6 +45,8 @@ int plan_header(const char *fn, const int64_t *lens, int64_t nseq, int64_t group
             return fail(hipErrorInvalidValue, "%s: more than %lld tokens for groups of %lld heads", fn,
                         (long long)(kMaxRows / group), (long long)group);
         h.max_len = std::max(h.max_len, lens[i]);
+        h.pairs += lens[i] * lens[i];  // lengths are below 2^31 and sum to less: at most 2^62
+        h.pairs_causal += lens[i] * (lens[i] + 1) / 2;
         for (int k = 0; k < kPackedTiles; ++k) counts[k] += tiles_of(lens[i], group, k);
     }
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
@@ -64,7 +66,7 @@ int plan_header(const char *fn, const int64_t *lens, int64_t nseq, int64_t group
 int64_t tile_cost(const PackedItem &it, int64_t group, int kind, bool causal) {
     if (!causal) return it.len;
     const int64_t size = kPackedTileSize[kind];
-    if (kind >= kKeys64) return it.len - it.tile * size;
+    if (kind >= kKeys32) return it.len - it.tile * size;
     return std::min<int64_t>(it.len, (it.tile * size + size - 1) / group + 1);
 }
 

@@ -20,7 +20,7 @@ from cudatransformer_amd import _capi
 
 # ---- the plan (host) ------------------------------------------------------------------------
 
-TILE = [64, 128, 256, 64, 128]  # rows of (token, head of the group) three times, then keys
+TILE = [32, 64, 128, 32, 64, 128]  # rows of (token, head of the group) three times, then keys
 
 
 def _plan_tables(lens, group):
@@ -30,11 +30,11 @@ def _plan_tables(lens, group):
     assert need > 0
     buf = np.zeros(need, dtype=np.uint8)
     assert lib.ctattn_packed_plan(arr, len(lens), group, buf.ctypes.data, need) == 0
-    head = buf[:256].view(np.int64)
+    head = buf[:512].view(np.int64)
     cu = buf[head[6]:head[6] + 4 * (len(lens) + 1)].view(np.int32)
     tables = []
-    for i in range(10):
-        at, count = head[8 + 2 * i], head[9 + 2 * i]
+    for i in range(12):
+        at, count = head[9 + 2 * i], head[10 + 2 * i]
         assert at % 16 == 0 and at + 16 * count <= need
         tables.append(buf[at:at + 16 * count].view(np.int32).reshape(-1, 4))
     return head, cu, tables
@@ -44,9 +44,10 @@ def _plan_tables(lens, group):
 def test_plan_covers_every_tile_once(lens, group):
     head, cu, tables = _plan_tables(lens, group)
     assert list(head[2:6]) == [len(lens), sum(lens), max(lens, default=0), group]
+    assert list(head[7:9]) == [sum(n * n for n in lens), sum(n * (n + 1) // 2 for n in lens)]
     assert list(cu) == list(np.concatenate([[0], np.cumsum(lens)]).astype(int))
     for i, table in enumerate(tables):
-        causal, kind = divmod(i, 5)
+        causal, kind = divmod(i, 6)
         rows = [n if kind >= 3 else n * group for n in lens]
         want = {(int(cu[s]), lens[s], t, s) for s in range(len(lens)) for t in range(-(-rows[s] // TILE[kind]))}
         assert {tuple(x) for x in table.tolist()} == want and len(table) == len(want)
@@ -198,6 +199,7 @@ def _run(q, k, v, do, plan, causal):
 
 
 LENS = [1, 0, 33, 64, 65, 127, 2, 129, 200]
+MANY = [120, 65, 128, 1, 100, 33, 127, 129] * 9  # enough of like lengths that larger tiles are taken
 
 
 @gpu
@@ -209,6 +211,24 @@ def test_against_64_bits(dtype, d, hq, hkv, causal):
     x = _inputs(LENS, hq, hkv, d, dtype, seed=d + hq)
     plan = ct.packed_plan(LENS, hq, hkv)
     _check(_run(*x, plan, causal), _reference(*x, LENS, causal), dtype, plan.tokens)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_many_sequences(dtype, d, causal):
+    x = _inputs(MANY, 12, 4, d, dtype, seed=d)
+    plan = ct.packed_plan(MANY, 12, 4)
+    _check(_run(*x, plan, causal), _reference(*x, MANY, causal), dtype, plan.tokens)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 72), (torch.float32, 40), (torch.float16, 24), (torch.float32, 104)])
+def test_many_sequences_between_the_tile_widths(dtype, d):
+    x = _inputs(MANY, 8, 8, d, dtype, seed=d)
+    plan = ct.packed_plan(MANY, 8, 8)
+    _check(_run(*x, plan, True), _reference(*x, MANY, True), dtype, plan.tokens)
 
 
 @gpu
