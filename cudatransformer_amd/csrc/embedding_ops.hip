@@ -10,10 +10,10 @@
 // Steps: (1) the sort, 9 bits of the id a pass, each pass a histogram per block of tokens and a scatter (a
 // batch of up to 4096 tokens is sorted by one workgroup in LDS instead); the table's zeros are written by
 // further workgroups of the same launches, which would leave most of the chip idle.  (2) Pieces of
-// kChunk sorted tokens, one wave per piece and slab of columns, its loads of whole row segments
+// 16 or 32 sorted tokens, one wave per piece and slab of columns, its loads of whole row segments
 // in flight together: a row whose tokens lie within the piece is written at once, sums that go on
-// across the piece's ends are kept.  (3) Those are joined, in order, by a workgroup for each row that
-// has any; a row as frequent as half of the batch is spread over as many waves as any others.
+// across the piece's ends are kept.  (3) Those are joined, in order, by a workgroup for each such row and
+// slab, so that a row as frequent as half of the batch is spread over as many waves as any others.
 // Bound by HBM: the rows of dout once, the table once.
 #include "attn_common.h"
 #include "attn_launch.h"
@@ -194,11 +194,12 @@ __global__ __launch_bounds__(kSmallWaves *kWave) void sort_small_kernel(const I 
     for (int i = threadIdx.x; i < n; i += blockDim.x) sorted[i] = buf[passes & 1][i];
 }
 
-// ---- more tokens: a histogram of each block's tokens ----
+// ---- more tokens: a histogram of each block's tokens for the first pass, zeros for the others', which the
+// scatter of the pass before counts ----
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void hist_kernel(const I *__restrict__ ids, const uint2 *__restrict__ from,
-                                                           int64_t n, int64_t vocab, int pass, int blocks, int per,
-                                                           uint32_t *__restrict__ hist, Fill fill) {
+__global__ __launch_bounds__(kSortThreads) void hist_kernel(const I *__restrict__ ids, int64_t n, int64_t vocab,
+                                                           int passes, int blocks, int per, uint32_t *__restrict__ hist,
+                                                           Fill fill) {
     if (int(blockIdx.x) >= blocks) {
         fill_share(fill, blockIdx.x - blocks, gridDim.x - blocks);
         return;
@@ -207,12 +208,12 @@ __global__ __launch_bounds__(kSortThreads) void hist_kernel(const I *__restrict_
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) h[i] = 0;
     __syncthreads();
     const int64_t lo = int64_t(blockIdx.x) * per, hi = min(n, lo + per);
-    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) {
-        const uint32_t key = pass == 0 ? key_of(ids, i, vocab) : from[i].x;
-        atomicAdd(&h[(key >> (kBits * pass)) & (kBins - 1)], 1u);
-    }
+    for (int64_t i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&h[key_of(ids, i, vocab) & (kBins - 1)], 1u);
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += blockDim.x) hist[int64_t(blockIdx.x) * kBins + i] = h[i];
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) {
+        hist[int64_t(blockIdx.x) * kBins + i] = h[i];
+        for (int p = 1; p < passes; ++p) hist[(int64_t(p) * blocks + blockIdx.x) * kBins + i] = 0;
+    }
 }
 
 // A block's tokens to their places: digits below, the same digit in blocks before, then within the block in order.
@@ -220,7 +221,8 @@ template <typename I>
 __global__ __launch_bounds__(kSortThreads) void scatter_kernel(const I *__restrict__ ids, const uint2 *__restrict__ from,
                                                               int64_t n, int64_t vocab, int pass, int blocks, int per,
                                                               const uint32_t *__restrict__ hist,
-                                                              uint2 *__restrict__ to, Fill fill) {
+                                                              uint32_t *__restrict__ next, uint2 *__restrict__ to,
+                                                              Fill fill) {
     if (int(blockIdx.x) >= blocks) {
         fill_share(fill, blockIdx.x - blocks, gridDim.x - blocks);
         return;
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(const I *__restri
     for (int i = threadIdx.x; i < WAVES * kBins; i += blockDim.x) (&cnt[0][0])[i] = 0;
     for (int bin = threadIdx.x; bin < kBins; bin += blockDim.x) {
         uint32_t before = 0, all = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int b = 0; b < blocks; ++b) {
             const uint32_t x = hist[int64_t(b) * kBins + bin];
             before += b < int(blockIdx.x) ? x : 0;
@@ -265,23 +267,35 @@ __global__ __launch_bounds__(kSortThreads) void scatter_kernel(const I *__restri
     auto item = [&](int64_t i) {
         return pass == 0 ? make_uint2(key_of(ids, i, vocab), uint32_t(i)) : from[i];
     };
-    for (int64_t i = lo + lane; i < hi; i += kWave) atomicAdd(&cnt[wave][(item(i).x >> (kBits * pass)) & (kBins - 1)], 1u);
+    // The first tokens of a lane stay in registers (all of them in blocks of 1024).
+    constexpr int KEEP = 1024 / kSortThreads;
+    uint2 kept[KEEP];
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) kept[j] = item(min(lo + j * kWave + lane, n - 1));
+    auto digit_of = [&](uint32_t key) { return (key >> (kBits * pass)) & (kBins - 1); };
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j)
+        if (lo + j * kWave + lane < hi) atomicAdd(&cnt[wave][digit_of(kept[j].x)], 1u);
+    for (int64_t i = lo + KEEP * kWave + lane; i < hi; i += kWave) atomicAdd(&cnt[wave][digit_of(item(i).x)], 1u);
     __syncthreads();
     place_bins<WAVES>(cnt, total, base);
-    for (int64_t i0 = lo; i0 < hi; i0 += kWave) {
-        const int64_t i = i0 + lane;
-        const uint2 x = item(min(i, n - 1));
-        const uint32_t digit = (x.x >> (kBits * pass)) & (kBins - 1);
-        const uint64_t m = same_digit(digit, __ballot(i < hi));
+    auto place = [&](const uint2 &x, bool live) __attribute__((always_inline)) {
+        const uint32_t digit = digit_of(x.x);
+        const uint64_t m = same_digit(digit, __ballot(live));
         uint32_t at = 0;
-        if (i < hi) at = cnt[wave][digit] + below(m, lane);
+        if (live) at = cnt[wave][digit] + below(m, lane);
         __builtin_amdgcn_wave_barrier();
-        if (i < hi) {
+        if (live) {
             to[at] = x;
             if ((m >> lane) == 1) cnt[wave][digit] = at + 1;
+            if (next != nullptr) atomicAdd(next + int64_t(at / uint32_t(per)) * kBins + ((x.x >> (kBits * (pass + 1))) & (kBins - 1)), 1u);
         }
         __builtin_amdgcn_wave_barrier();
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j)
+        if (lo + j * kWave < hi) place(kept[j], lo + j * kWave + lane < hi);
+    for (int64_t i0 = lo + KEEP * kWave; i0 < hi; i0 += kWave) place(item(min(i0 + lane, n - 1)), i0 + lane < hi);
 }
 
 // ---- sums ----
@@ -315,59 +329,71 @@ __device__ __forceinline__ void put_row(T *row, const Cols<T, VEC, STRIPS> &x, i
     }
 }
 
+// What is said of a chunk's end: no row goes on behind it, the row that goes on began in it, or it went on
+// into it as well.
+enum : uint32_t { kEnds = 0, kBegins, kThrough };
+
 // One wave per chunk of CH sorted tokens and slab.  edge[chunk] is the sum of the chunk's tokens whose row
 // began in an earlier chunk, edge[chunks + chunk] of those whose row goes on into the next one and began
-// in this.
+// in this.  (Letting a wave finish a row that ends within the next 48 tokens, to have fewer sums to join, made
+// chains of loads of it: 16384 tokens x 768 13 -> 33 us.)
 template <typename T, int VEC, int STRIPS, int CH>
 __global__ __launch_bounds__(256) void sum_kernel(const uint2 *__restrict__ sorted, const T *__restrict__ dout,
-                                                 T *__restrict__ dtable, acc_t<T> *__restrict__ edge, int64_t n,
-                                                 int64_t chunks, int64_t D, int slabs, int64_t vocab, acc_t<T> scale,
-                                                 int accumulate) {
+                                                 T *__restrict__ dtable, acc_t<T> *__restrict__ edge,
+                                                 uint2 *__restrict__ ends, int64_t n, int64_t chunks, int64_t D,
+                                                 int slabs, int64_t vocab, acc_t<T> scale, int accumulate) {
     using A = acc_t<T>;
     static_assert(CH <= kWave, "a lane per token");
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t w = int64_t(blockIdx.x) * (blockDim.x / kWave) + threadIdx.x / kWave;
     const int64_t chunk = w / slabs;
     if (chunk >= chunks) return;
-    const int64_t c0 = int64_t(w % slabs) * kWave * VEC * STRIPS + int64_t(lane) * VEC;
+    const int slab = int(w % slabs);
+    const int64_t c0 = int64_t(slab) * kWave * VEC * STRIPS + int64_t(lane) * VEC;
     const int64_t lo = chunk * CH;
     const int cnt = int(min(n - lo, int64_t(CH)));
     const uint2 mine = sorted[lo + min(lane, cnt - 1)];
     const uint32_t prev = lo > 0 ? sorted[lo - 1].x : 0xFFFFFFFFu;
     const uint32_t next = lo + cnt < n ? sorted[lo + cnt].x : 0xFFFFFFFFu;
+    auto key_at = [&](int i) __attribute__((always_inline)) { return uint32_t(__builtin_amdgcn_readlane(mine.x, i)); };
+    int64_t col[STRIPS];  // held inside the row: a guard on each load would make a chain of them
+#pragma unroll
+    for (int s = 0; s < STRIPS; ++s) col[s] = min(c0 + int64_t(s) * kWave * VEC, D - VEC);
     Cols<T, VEC, STRIPS> sum;
     sum.zero();
-    bool begun = true;  // the current row began in this chunk
-    begun = uint32_t(__builtin_amdgcn_readlane(mine.x, 0)) != prev;
-    constexpr int U = 8;  // rows in flight
+    bool begun = key_at(0) != prev;  // the current row began in this chunk
+    uint32_t row = 0, state = kEnds;
+    constexpr int U = sizeof(T) * VEC * STRIPS >= 16 ? 8 : 16;  // rows in flight
     for (int i0 = 0; i0 < cnt; i0 += U) {
         Pack<T, VEC> x[U][STRIPS];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = min(i0 + u, cnt - 1);
-            const int64_t pos = uint32_t(__builtin_amdgcn_readlane(mine.y, i));
+            const int64_t pos = uint32_t(__builtin_amdgcn_readlane(mine.y, min(i0 + u, cnt - 1)));
 #pragma unroll
-            for (int s = 0; s < STRIPS; ++s) {
-                const int64_t c = c0 + int64_t(s) * kWave * VEC;
-                if (c < D) x[u][s] = Pack<T, VEC>::load(dout + pos * D + c);
-            }
+            for (int s = 0; s < STRIPS; ++s) x[u][s] = Pack<T, VEC>::load(dout + pos * D + col[s]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u;
             if (i >= cnt) break;
-            const uint32_t key = __builtin_amdgcn_readlane(mine.x, i);
-            if (key >= uint32_t(vocab)) return;  // the rest belongs to no row
+            const uint32_t key = key_at(i);
+            if (key >= uint32_t(vocab)) {  // the rest belongs to no row
+                i0 = cnt;
+                break;
+            }
+            row = key;
 #pragma unroll
             for (int s = 0; s < STRIPS; ++s)
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) sum.a[s][e] += to_acc(x[u][s].v[e]);
-            const uint32_t after = i + 1 < cnt ? uint32_t(__builtin_amdgcn_readlane(mine.x, i + 1 < cnt ? i + 1 : i)) : next;
-            if (after == key && i + 1 < cnt) continue;
-            if (after != key && begun) {
+            const bool at_end = i + 1 >= cnt;
+            const bool goes_on = (at_end ? next : key_at(min(i + 1, cnt - 1))) == key;
+            if (goes_on && !at_end) continue;
+            if (!goes_on && begun) {
                 put_row<T, VEC, STRIPS>(dtable + int64_t(key) * D, sum, c0, D, scale, accumulate != 0);
             } else {
                 A *to = edge + (begun ? chunks + chunk : chunk) * D;
+                state = !goes_on ? kEnds : begun ? kBegins : kThrough;
 #pragma unroll
                 for (int s = 0; s < STRIPS; ++s)
 #pragma unroll
@@ -380,59 +406,66 @@ __global__ __launch_bounds__(256) void sum_kernel(const uint2 *__restrict__ sort
             begun = true;
         }
     }
+    if (slab == 0 && lane == 0) ends[chunk] = make_uint2(row, state);
 }
 
-// Rows across chunks: the workgroup of the chunk in which the row begins adds up its own edge and those
-// of the following chunks, wave w of 4 the w-th quarter of them, the waves' sums in order.
+// Rows across chunks: the workgroup of the chunk in which the row begins (and of a slab of columns) adds up its
+// own edge and those of the following chunks, wave w of 4 the w-th quarter of them, the waves' sums in order.  `ends`
+// tells in one load whether the chunk has such a row and how far it goes.  The pieces are loaded 8 at a time, their
+// columns held inside the row rather than guarded, so that a frequent row is not a chain of loads (16384 tokens x
+// 768: 13 us with guarded loads).
 constexpr int kJoinWaves = 4;
-template <typename T, int CH>
-__global__ __launch_bounds__(kJoinWaves *kWave) void join_kernel(const uint2 *__restrict__ sorted,
-                                                                T *__restrict__ dtable,
-                                                                const acc_t<T> *__restrict__ edge, int64_t n,
-                                                                int64_t chunks, int64_t D, int slabs, int64_t vocab,
-                                                                acc_t<T> scale, int accumulate) {
+constexpr int kJoinCols = 4;  // columns of a lane, 64 apart
+template <typename T>
+__global__ __launch_bounds__(kJoinWaves *kWave) void join_kernel(const uint2 *__restrict__ ends, T *__restrict__ dtable,
+                                                                const acc_t<T> *__restrict__ edge, int64_t chunks,
+                                                                int64_t D, int slabs, acc_t<T> scale, int accumulate) {
     using A = acc_t<T>;
-    constexpr int COLS = 4;  // columns of a lane, 64 apart
-    __shared__ A part[kJoinWaves][COLS * kWave];
+    __shared__ A part[kJoinWaves][kJoinCols * kWave];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int64_t chunk = blockIdx.x / slabs;
-    const int64_t c0 = int64_t(blockIdx.x % slabs) * COLS * kWave + lane;
-    const int64_t lo = chunk * CH, hi = lo + CH;
-    if (hi >= n) return;  // the last chunk's rows end in it
-    const uint32_t key = sorted[hi - 1].x;
-    if (key >= uint32_t(vocab) || sorted[hi].x != key) return;
-    if (lo > 0 && sorted[lo].x == key && sorted[lo - 1].x == key) return;  // began earlier
-    // Chunks hi / CH .. last: the last is the first whose last token is another row's (or none's).
-    int64_t last = chunk + 1;
+    const uint2 mine = ends[chunk];
+    int64_t last = chunk + 1;  // the row's last chunk: the first from here on that it does not go through
+    uint32_t other = ends[min(last + lane, chunks - 1)].y;
+    if (mine.y != kBegins) return;
     for (;;) {
-        const int64_t end = (last + lane + 1) * CH;  // behind chunk last + lane
-        const bool done = end >= n || sorted[min(end, n - 1)].x != key;
-        const uint64_t m = __ballot(done);
+        const uint64_t m = __ballot(last + lane >= chunks - 1 || other != kThrough);
         if (m != 0) {
             last += __ffsll((unsigned long long)m) - 1;
             break;
         }
         last += kWave;
+        other = ends[min(last + lane, chunks - 1)].y;
     }
+    const uint32_t key = mine.x;
     const int64_t parts = last - chunk + 1;  // this chunk's own edge first
     const int64_t per = (parts + kJoinWaves - 1) / kJoinWaves;
-    A s[COLS];
+    const int64_t c0 = int64_t(blockIdx.x % slabs) * kJoinCols * kWave + lane;
+    int64_t col[kJoinCols];
+    A s[kJoinCols];
 #pragma unroll
-    for (int k = 0; k < COLS; ++k) s[k] = 0;
+    for (int k = 0; k < kJoinCols; ++k) col[k] = min(c0 + k * kWave, D - 1), s[k] = 0;
     const int64_t p_end = min(parts, (wave + 1) * per);
-#pragma unroll 4
-    for (int64_t p = wave * per; p < p_end; ++p) {
-        const A *from = edge + (p == 0 ? chunks + chunk : chunk + p) * D;
+    constexpr int U = 8;
+    for (int64_t p = wave * per; p < p_end; p += U) {
+        A x[U][kJoinCols];
 #pragma unroll
-        for (int k = 0; k < COLS; ++k)
-            if (c0 + k * kWave < D) s[k] += from[c0 + k * kWave];
+        for (int u = 0; u < U; ++u) {
+            const int64_t q = min(p + u, p_end - 1);
+            const A *piece = edge + (q == 0 ? chunks + chunk : chunk + q) * D;
+#pragma unroll
+            for (int k = 0; k < kJoinCols; ++k) x[u][k] = piece[col[k]];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < kJoinCols; ++k) s[k] += p + u < p_end ? x[u][k] : A(0);
     }
 #pragma unroll
-    for (int k = 0; k < COLS; ++k) part[wave][k * kWave + lane] = s[k];
+    for (int k = 0; k < kJoinCols; ++k) part[wave][k * kWave + lane] = s[k];
     __syncthreads();
-    // Wave w writes column strip w.
-    static_assert(kJoinWaves == COLS, "a strip per wave");
-    const int64_t c = int64_t(blockIdx.x % slabs) * COLS * kWave + wave * kWave + lane;
+    static_assert(kJoinWaves == kJoinCols, "wave w writes strip w");
+    const int64_t c = c0 + wave * kWave;
     if (c < D) {
         A v = 0;
 #pragma unroll
@@ -444,12 +477,11 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void join_kernel(const uint2 *__
 }
 
 // ---- sizes ----
-constexpr int kChunk = 32;
-
 struct GradPlan {
     int passes, blocks, per;  // sort
+    int chunk;                // tokens of a piece: 16 or 32
     int64_t chunks;
-    int64_t off_a, off_b, off_hist, off_edge, bytes;
+    int64_t off_a, off_b, off_hist, off_ends, off_edge, bytes;
 };
 GradPlan grad_plan(int dtype, int64_t n, int64_t D, int64_t vocab) {
     GradPlan g{};
@@ -461,12 +493,15 @@ GradPlan grad_plan(int dtype, int64_t n, int64_t D, int64_t vocab) {
     while (per * 64 < n) per *= 2;
     g.per = int(per);
     g.blocks = int((n + per - 1) / per);
-    g.chunks = (n + kChunk - 1) / kChunk;
+    // Pieces of 32 tokens keep fewer sums across their ends; 16 make twice the waves.
+    g.chunk = n * D < (int64_t(1) << 25) ? 16 : 32;
+    g.chunks = (n + g.chunk - 1) / g.chunk;
     const int64_t pairs = capi::align_up(n * int64_t(sizeof(uint2)));
     g.off_a = 0;
     g.off_b = pairs;
     g.off_hist = 2 * pairs;
-    g.off_edge = g.off_hist + capi::align_up(int64_t(64) * kBins * 4);
+    g.off_ends = g.off_hist + capi::align_up(int64_t(64) * g.passes * kBins * 4);
+    g.off_edge = g.off_ends + capi::align_up(g.chunks * int64_t(sizeof(uint2)));
     g.bytes = g.off_edge + 2 * g.chunks * D * (dtype == CTATTN_F64 ? 8 : 4);
     return g;
 }
@@ -486,6 +521,36 @@ hipError_t lookup(const I *ids, const T *table, T *out, int64_t n, int64_t D, in
     return launch(lookup_kernel<T, I, 1>, 1);
 }
 
+template <typename T, int CH>
+hipError_t sums(const GradPlan &g, const uint2 *sorted, const T *dout, T *dtable, acc_t<T> *edge, uint2 *ends,
+                double scale,
+                bool accumulate, int64_t n, int64_t D, int64_t vocab, hipStream_t st) {
+    using A = acc_t<T>;
+    auto pieces = [&](auto kernel, int cols) {
+        const int64_t slabs = (D + kWave * cols - 1) / (kWave * cols);
+        const int64_t waves = g.chunks * slabs;
+        if (!grid_fits((waves + 3) / 4, 256)) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(kernel, dim3(unsigned((waves + 3) / 4)), dim3(256), 0, st, sorted, dout, dtable, edge, ends, n,
+                           g.chunks, D, int(slabs), vocab, A(scale), int(accumulate));
+        return hipGetLastError();
+    };
+    // 16 bytes a lane, or half of that where a row then fills its last slab better.
+    constexpr int V = 16 / int(sizeof(T)), H = sizeof(T) < 8 ? V / 2 : V;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dtable);
+    const auto lost = [&](int v) { return (D + kWave * v - 1) / (kWave * v) * (kWave * v) - D; };
+    hipError_t e;
+    if (D % V != 0 || at % 16 != 0) e = pieces(sum_kernel<T, 1, 4, CH>, 4);
+    else if (lost(H) < lost(V)) e = pieces(sum_kernel<T, H, 1, CH>, H);
+    else e = pieces(sum_kernel<T, V, 1, CH>, V);
+    if (e != hipSuccess) return e;
+    const int64_t slabs = (D + kJoinCols * kWave - 1) / (kJoinCols * kWave);
+    const int64_t groups = g.chunks * slabs;
+    if (!grid_fits(groups, kJoinWaves * kWave)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(join_kernel<T>, dim3(unsigned(groups)), dim3(kJoinWaves * kWave), 0, st, ends, dtable, edge,
+                       g.chunks, D, int(slabs), A(scale), int(accumulate));
+    return hipGetLastError();
+}
+
 template <typename T, typename I>
 hipError_t grad(int dtype, const I *ids, const T *dout, T *dtable, double scale, bool accumulate, char *ws, int64_t n,
                 int64_t D, int64_t vocab, hipStream_t st) {
@@ -494,6 +559,7 @@ hipError_t grad(int dtype, const I *ids, const T *dout, T *dtable, double scale,
     uint2 *a = reinterpret_cast<uint2 *>(ws + g.off_a), *b = reinterpret_cast<uint2 *>(ws + g.off_b);
     uint32_t *hist = reinterpret_cast<uint32_t *>(ws + g.off_hist);
     A *edge = reinterpret_cast<A *>(ws + g.off_edge);
+    uint2 *ends = reinterpret_cast<uint2 *>(ws + g.off_ends);
     const int64_t table_bytes = accumulate ? 0 : vocab * D * int64_t(sizeof(T));
     char *const table = reinterpret_cast<char *>(dtable);
     // Workgroups that write `bytes` of zeros: enough for every CU, 64 KiB each at least.
@@ -507,53 +573,32 @@ hipError_t grad(int dtype, const I *ids, const T *dout, T *dtable, double scale,
         if ((e = hipGetLastError()) != hipSuccess || n == 0) return e;
         sorted = a;
     } else {
-        const int launches = 2 * g.passes;
+        const int launches = 1 + g.passes;
         int step = 0;
         auto share = [&]() {
             const int64_t lo = table_bytes / launches / 256 * 256 * step;
             const int64_t hi = ++step == launches ? table_bytes : table_bytes / launches / 256 * 256 * step;
             return Fill{table + lo, hi - lo};
         };
+        Fill f = share();
+        hipLaunchKernelGGL(hist_kernel<I>, dim3(unsigned(g.blocks) + fillers(f.bytes)), dim3(kSortThreads), 0, st, ids,
+                           n, vocab, g.passes, g.blocks, g.per, hist, f);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
         const uint2 *from = nullptr;
         for (int pass = 0; pass < g.passes; ++pass) {
             uint2 *to = pass % 2 == 0 ? a : b;
-            Fill f = share();
-            hipLaunchKernelGGL(hist_kernel<I>, dim3(unsigned(g.blocks) + fillers(f.bytes)), dim3(kSortThreads), 0, st,
-                               ids, from, n, vocab, pass, g.blocks, g.per, hist, f);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
+            uint32_t *here = hist + int64_t(pass) * g.blocks * kBins;
             f = share();
             hipLaunchKernelGGL(scatter_kernel<I>, dim3(unsigned(g.blocks) + fillers(f.bytes)), dim3(kSortThreads), 0,
-                               st, ids, from, n, vocab, pass, g.blocks, g.per, hist, to, f);
+                               st, ids, from, n, vocab, pass, g.blocks, g.per, here,
+                               pass + 1 < g.passes ? here + int64_t(g.blocks) * kBins : nullptr, to, f);
             if ((e = hipGetLastError()) != hipSuccess) return e;
             from = to;
         }
         sorted = from;
     }
-    auto sums = [&](auto kernel, int cols) {
-        const int64_t slabs = (D + kWave * cols - 1) / (kWave * cols);
-        const int64_t waves = g.chunks * slabs;
-        if (!grid_fits((waves + 3) / 4, 256)) return hipErrorInvalidValue;
-        hipLaunchKernelGGL(kernel, dim3(unsigned((waves + 3) / 4)), dim3(256), 0, st, sorted, dout, dtable, edge, n,
-                           g.chunks, D, int(slabs), vocab, A(scale), int(accumulate));
-        return hipGetLastError();
-    };
-    // 16 bytes a lane, or half of that where a row then fills its last slab better.
-    constexpr int V = 16 / int(sizeof(T));
-    const uintptr_t at = reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dtable);
-    if (D % V == 0 && at % 16 == 0) {
-        constexpr int H = V / 2;
-        const auto lost = [&](int v) { return (D + kWave * v - 1) / (kWave * v) * (kWave * v) - D; };
-        if constexpr (H >= 1 && sizeof(T) < 8) e = lost(H) < lost(V) ? sums(sum_kernel<T, H, 1, kChunk>, H) : sums(sum_kernel<T, V, 1, kChunk>, V);
-        else e = sums(sum_kernel<T, V, 1, kChunk>, V);
-    } else {
-        e = sums(sum_kernel<T, 1, 4, kChunk>, 4);
-    }
-    if (e != hipSuccess) return e;
-    const int64_t slabs = (D + 4 * kWave - 1) / (4 * kWave);
-    if (!grid_fits(g.chunks * slabs, kJoinWaves * kWave)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((join_kernel<T, kChunk>), dim3(unsigned(g.chunks * slabs)), dim3(kJoinWaves * kWave), 0, st,
-                       sorted, dtable, edge, n, g.chunks, D, int(slabs), vocab, A(scale), int(accumulate));
-    return hipGetLastError();
+    return g.chunk == 16 ? sums<T, 16>(g, sorted, dout, dtable, edge, ends, scale, accumulate, n, D, vocab, st)
+                         : sums<T, 32>(g, sorted, dout, dtable, edge, ends, scale, accumulate, n, D, vocab, st);
 }
 
 template <typename Fn> hipError_t typed(int dtype, bool ids64, Fn fn) {
