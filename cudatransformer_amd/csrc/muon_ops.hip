@@ -17,8 +17,9 @@
 // Layout: a factor's 128 x 32 blocks lie one behind the other, each a run of 128 rows [32 hi | 32 lo] (128 bytes
 // a row, 16 KiB), so that one K step of a tile is one contiguous read.  A product's 32 x 32
 // block is then a run of 4 KiB as well.  Rows and columns are padded with zeros to 128 and no product checks a bound.
-// X is kept in both orders (X for A, X^T for B X): each product's operands then have the contraction
-// contiguous, and the writing product has the tile in registers in either order anyway.
+// X is kept transposed alone: X^T's rows are what B X contracts over, and A = X X^T, which contracts over
+// its columns, reads them through transposing LDS reads (ds_read_b64_tr_b16).  Keeping X as well made B X write
+// twice: 24 x 384 x 384 290 us, bf16 4096 x 1024 398, 2048 x 8192 1.96 ms for five steps.
 #include "attn_bf16_tiles.h"
 #include "attn_launch.h"
 #include "capi_util.h"
@@ -153,11 +154,11 @@ struct Shape {
     int tall;            // X = G^T
 };
 
-// X and X^T as factors: a wave per 32 x 32 block of G, whose rows it reads 4 elements a lane, 8 lanes a row.  The block
-// goes to the factor with G's order of rows as it is read, and through LDS to the other.
+// X^T as a factor: a wave per 32 x 32 block of G, whose rows it reads 4 elements a lane, 8 lanes a row.  Of a tall G
+// they are X^T's rows; of another they are transposed in LDS.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Shape s, double eps,
-                                                   const double *__restrict__ part, int blocks, char *__restrict__ x,
+                                                   const double *__restrict__ part, int blocks,
                                                    char *__restrict__ xt, int64_t bytes) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
     __shared__ float inv_s;
@@ -179,8 +180,7 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
     const int gcols = int(s.tall ? s.rp : s.cp);
     const int j0 = (int(blockIdx.x) * 4 + wave) * 32, i0 = int(blockIdx.y) * 32;
     if (j0 >= gcols) return;
-    char *same = (s.tall ? xt : x) + mat * bytes + factor_at(i0, j0, gcols / kGroup);
-    char *other = (s.tall ? x : xt) + mat * bytes + factor_at(j0, i0, int(s.tall ? s.cp : s.rp) / kGroup);
+    char *to = xt + mat * bytes + (s.tall ? factor_at(i0, j0, int(s.rp) / kGroup) : factor_at(j0, i0, int(s.rp) / kGroup));
     const uint32_t blk = lds_addr(smem) + uint32_t(wave * 4096);
     struct alignas(sizeof(T) * 4) Run {
         T v[4];
@@ -201,13 +201,16 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
         }
         v = v * inv;
         const Four f = split4(v);
-        *reinterpret_cast<u16x4 *>(same + line * kRowBytes + 2 * c) = f.hi;
-        *reinterpret_cast<u16x4 *>(same + line * kRowBytes + 2 * c + 64) = f.lo;
-        block_put4(blk, line, c, f);
+        if (s.tall) {
+            *reinterpret_cast<u16x4 *>(to + line * kRowBytes + 2 * c) = f.hi;
+            *reinterpret_cast<u16x4 *>(to + line * kRowBytes + 2 * c + 64) = f.lo;
+        } else {
+            block_put4(blk, line, c, f);
+        }
     }
-    __builtin_amdgcn_wave_barrier();
+    if (s.tall) return;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    block_transposed(blk, other, lane);
+    block_transposed(blk, to, lane);
 }
 
 // ---- products ----
@@ -220,9 +223,10 @@ struct Gemm {
     int tiles_m, tiles_n;        // kGram, kPoly: tiles_m (tiles_m + 1) / 2 lower tiles
     int mats, splits;
     float *part;                 // splits > 1: a tile's sums for each split
-    char *o, *ot;                // the product as a factor, and its transpose (kApply)
+    char *o;                     // the product as a factor (kApply: transposed)
     int64_t o_bytes;
-    int o_groups, ot_groups;     // their K steps a row
+    int o_groups;                // its K steps a row
+    int a_groups;                // kGram: of a row of X^T
     const char *gram;            // kPoly: A, for b A
     float pa, pb, pc;
     Mats out;                    // kLast
@@ -285,9 +289,9 @@ __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &ac
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
         // Four elements of row j0 + col of the transpose at a time, straight from the registers; the block as it is
-        // through LDS, where the transpose is transposed.
-        const int64_t at = factor_at(j0, i0, P == kApply ? g.ot_groups : g.o_groups) + mat * g.o_bytes + col * kRowBytes + 8 * half;
-        char *t = (P == kApply ? g.ot : g.o) + at;
+        // (symmetric products) through LDS, where the transpose is transposed.
+        const int64_t at = factor_at(j0, i0, g.o_groups) + mat * g.o_bytes + col * kRowBytes + 8 * half;
+        char *t = g.o + at;
         // a I on the diagonal of the rows that exist.
         const int diag = P == kPoly && i0 == j0 && i0 + col < g.s.r ? col - 4 * half : -1;
 #pragma unroll
@@ -308,11 +312,13 @@ __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &ac
                 *reinterpret_cast<u16x4 *>(t + 16 * q) = f.hi;
                 *reinterpret_cast<u16x4 *>(t + 16 * q + 64) = f.lo;
             }
-            block_put4(buf, col, 8 * q + 4 * half, f);
+            if (P != kApply) block_put4(buf, col, 8 * q + 4 * half, f);
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        block_transposed(buf, g.o + mat * g.o_bytes + factor_at(i0, j0, g.o_groups), lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next block's writes follow these reads
+        if constexpr (P != kApply) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            block_transposed(buf, g.o + mat * g.o_bytes + factor_at(i0, j0, g.o_groups), lane);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next block's writes follow these reads
+        }
     }
 }
 
@@ -349,14 +355,21 @@ void product_kernel(Gemm g) {
     const int steps_all = int(g.kp / kGroup);
     const int per = (steps_all + g.splits - 1) / g.splits;
     const int k0 = min(steps_all, split_i * per), k1 = min(steps_all, k0 + per);
-    const int64_t panel = int64_t(steps_all) * BLOCK;  // 128 rows
-    const char *ga = g.a + mat * g.a_bytes + int64_t(ti) * (C::BM / kPad) * panel;
-    const char *gb = g.b + mat * g.b_bytes + int64_t(tj) * (C::BM / kPad) * panel;
+    // A step's tile of an operand: BM rows of 128 bytes, or for kGram 32 rows of X^T in each of BM / 32 groups of
+    // columns, 4 KiB a group.
+    const int64_t panel = int64_t(P == kGram ? g.a_groups : steps_all) * BLOCK;  // 128 rows
+    const int64_t tile_bytes = P == kGram ? C::BM / kGroup * int64_t(BLOCK) : C::BM / kPad * panel;
+    const char *ga = g.a + mat * g.a_bytes + ti * tile_bytes;
+    const char *gb = g.b + mat * g.b_bytes + tj * tile_bytes;
+    auto step_at = [&](int k) __attribute__((always_inline)) {
+        return P == kGram ? int64_t(k / 4) * panel + (k % 4) * (32 * kRowBytes) : int64_t(k) * BLOCK;
+    };
     int64_t src[NL];  // this lane's 16-byte chunks of a step
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        const int p = (wave * NL + i) * kWave + lane;
-        src[i] = (p / 8 / kPad) * panel + (p / 8 % kPad) * kRowBytes + 16 * ((p % 8) ^ Tile<64>::swz(p / 8));
+        const int p = (wave * NL + i) * kWave + lane, row = p / 8;
+        src[i] = (P == kGram ? int64_t(row / 32) * BLOCK + (row % 32) * kRowBytes : (row / kPad) * panel + (row % kPad) * kRowBytes) +
+                 16 * ((p % 8) ^ Tile<64>::swz(row));
     }
     auto buffer = [&](int k) __attribute__((always_inline)) { return L + uint32_t((k - k0) % C::STAGES) * 2 * TB; };
     auto issue = [&](int k) __attribute__((always_inline)) {
@@ -364,7 +377,7 @@ void product_kernel(Gemm g) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const uint32_t dst = to + uint32_t((wave * NL + i) * kWave * 16);
-            const char *pa = ga + src[i] + int64_t(k) * BLOCK, *pb = gb + src[i] + int64_t(k) * BLOCK;
+            const char *pa = ga + src[i] + step_at(k), *pb = gb + src[i] + step_at(k);
             asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(pa),
                          "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
             asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(pb),
@@ -388,8 +401,24 @@ void product_kernel(Gemm g) {
     struct Half {
         f16x8 ah[MT], al[MT], bh[NT], bl[NT];
     };
+    const uint32_t cb0 = col_base<64>(0, 0, 0, lane), cb1 = col_base<64>(0, 0, 1, lane);
     auto read = [&](Half &x, int k, int s) __attribute__((always_inline)) {  // chunks 2 s + half of hi, 4 on of lo
         const uint32_t base = buffer(k);
+        if constexpr (P == kGram) {  // columns of 16 rows: the same order of the contraction in both operands
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t p = base + TB + uint32_t((NT * wn + n) * 32 * kRowBytes);
+                x.bh[n] = read_col<64, f16x8>(p + cb0, p + cb1, s, 0);
+                x.bl[n] = read_col<64, f16x8>(p + cb0, p + cb1, s, 1);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint32_t p = base + uint32_t((MT * wm + m) * 32 * kRowBytes);
+                x.ah[m] = read_col<64, f16x8>(p + cb0, p + cb1, s, 0);
+                x.al[m] = read_col<64, f16x8>(p + cb0, p + cb1, s, 1);
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t p = base + rb + uint32_t(32 * n * kRowBytes);
@@ -507,8 +536,8 @@ __global__ __launch_bounds__(256) void join_product_kernel(Gemm g) {
 // ---- sizes and launches ----
 struct Layout {
     Shape s;
-    int64_t x_bytes, a_bytes;  // one factor X (or X^T), one factor A
-    int64_t off_norm, off_x, off_xt[2], off_a, off_b, off_part, bytes;
+    int64_t x_bytes, a_bytes;  // one factor X^T, one factor A
+    int64_t off_norm, off_xt[2], off_a, off_b, off_part, bytes;
 };
 
 // How a product runs: the tile shape and the splits of K with the least estimated time, one workgroup a CU at a
@@ -559,7 +588,6 @@ Layout layout(int64_t mats, int64_t rows, int64_t cols) {
         return o;
     };
     l.off_norm = take(mats * kNormBlocks * 8);
-    l.off_x = take(mats * l.x_bytes);
     l.off_xt[0] = take(mats * l.x_bytes);
     l.off_xt[1] = take(mats * l.x_bytes);
     l.off_a = take(mats * l.a_bytes);
@@ -621,7 +649,7 @@ template <typename T> hipError_t orthogonalise(const Args &x, const Layout &l, c
     const int64_t gr = l.s.tall ? l.s.cp : l.s.rp, gc = l.s.tall ? l.s.rp : l.s.cp;  // G's padded shape
     const dim3 grid(unsigned(gc / 128), unsigned(gr / 32), unsigned(x.mats));
     auto split_g = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x.g, x.m, x.u, l.s, x.eps, norm, blocks, ws + l.off_x,
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, x.g, x.m, x.u, l.s, x.eps, norm, blocks,
                            ws + l.off_xt[0], l.x_bytes);
     };
     if (l.s.cols % 4 == 0 && at % 16 == 0) split_g(split_kernel<T, true>);
@@ -638,8 +666,9 @@ template <typename T> hipError_t orthogonalise(const Args &x, const Layout &l, c
     g.u = x.u;
     for (int i = 0; i < x.steps; ++i) {
         const char *xt = ws + l.off_xt[i % 2];
-        g.a = g.b = ws + l.off_x;
+        g.a = g.b = xt;
         g.a_bytes = g.b_bytes = l.x_bytes;
+        g.a_groups = int(l.s.rp / kGroup);
         g.kp = l.s.cp;
         g.o = ws + l.off_a;
         g.o_bytes = l.a_bytes;
@@ -653,11 +682,9 @@ template <typename T> hipError_t orthogonalise(const Args &x, const Layout &l, c
         g.a = ws + l.off_b;
         g.b = xt;
         g.b_bytes = l.x_bytes;
-        g.o = ws + l.off_x;
-        g.ot = ws + l.off_xt[(i + 1) % 2];
+        g.o = ws + l.off_xt[(i + 1) % 2];
         g.o_bytes = l.x_bytes;
-        g.o_groups = int(l.s.cp / kGroup);
-        g.ot_groups = int(l.s.rp / kGroup);
+        g.o_groups = int(l.s.rp / kGroup);
         e = i + 1 == x.steps ? product<T, kLast>(g, l.s.rp, l.s.cp, st) : product<T, kApply>(g, l.s.rp, l.s.cp, st);
         if (e != hipSuccess) return e;
     }
