@@ -82,9 +82,19 @@ __device__ __forceinline__ void block_put4(uint32_t blk, int row, int c, const F
     *(__attribute__((address_space(3))) u16x4 *)(uintptr_t)(blk + uint32_t(Tile<64>::off(row, c >> 3)) + in) = v.hi;
     *(__attribute__((address_space(3))) u16x4 *)(uintptr_t)(blk + uint32_t(Tile<64>::off(row, 4 + (c >> 3))) + in) = v.lo;
 }
-// Writes the block's transpose to `to` (the 4 KiB run of a factor's block): ds_read_b64_tr_b16 gives lane l of a
-// group of 16 column l of 4 rows, so two of them are 8 elements of one row of the transpose.
-__device__ __forceinline__ void block_transposed(uint32_t blk, char *to, int lane) {
+__device__ __forceinline__ void lds_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// The block to a factor's 4 KiB run, whole lines at a time (stores of 8 or 16 bytes a row, straight from registers, were
+// bound by their number: 24 x 384 x 384 19 us a product for 16).
+__device__ __forceinline__ void block_store(uint32_t blk, char *to, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + lane / 8, chunk = lane % 8;
+        *reinterpret_cast<u16x8 *>(to + row * kRowBytes + 16 * chunk) = lds_b128<u16x8>(blk + uint32_t(Tile<64>::off(row, chunk)));
+    }
+}
+// The block's transpose into another: ds_read_b64_tr_b16 gives lane l of a group of 16 column l of 4 rows, so
+// two of them are 8 elements of one row of the transpose.
+__device__ __forceinline__ void block_transpose(uint32_t blk, uint32_t into, int lane) {
     const int s = lane & 15, half = lane >> 5;
     const int chunk = 2 * ((lane >> 4) & 1) + ((s & 3) >> 1);
 #pragma unroll
@@ -99,7 +109,7 @@ __device__ __forceinline__ void block_transposed(uint32_t blk, char *to, int lan
                 x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)(uintptr_t)at);
             }
             const i16x8 y = {x[0][0], x[0][1], x[0][2], x[0][3], x[1][0], x[1][1], x[1][2], x[1][3]};
-            *reinterpret_cast<i16x8 *>(to + (lane & 31) * kRowBytes + 64 * part + 2 * (r0 + 8 * half)) = y;
+            *(__attribute__((address_space(3))) i16x8 *)(uintptr_t)(into + uint32_t(Tile<64>::off(lane & 31, 4 * part + r0 / 8 + half))) = y;
         }
 }
 // Byte offset of element (i, k)'s hi in a factor of `groups` K steps a row; lo is 64 bytes on.
@@ -160,7 +170,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Shape s, double eps,
                                                    const double *__restrict__ part, int blocks,
                                                    char *__restrict__ xt, int64_t bytes) {
-    __shared__ __attribute__((aligned(1024))) char smem[4 * 4096];
+    __shared__ __attribute__((aligned(1024))) char smem[4 * 8192];
     __shared__ float inv_s;
     __shared__ double sums[4];
     const int mat = blockIdx.z, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -181,7 +191,7 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
     const int j0 = (int(blockIdx.x) * 4 + wave) * 32, i0 = int(blockIdx.y) * 32;
     if (j0 >= gcols) return;
     char *to = xt + mat * bytes + (s.tall ? factor_at(i0, j0, int(s.rp) / kGroup) : factor_at(j0, i0, int(s.rp) / kGroup));
-    const uint32_t blk = lds_addr(smem) + uint32_t(wave * 4096);
+    const uint32_t blk = lds_addr(smem) + uint32_t(wave * 8192);
     struct alignas(sizeof(T) * 4) Run {
         T v[4];
     };
@@ -201,16 +211,14 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
         }
         v = v * inv;
         const Four f = split4(v);
-        if (s.tall) {
-            *reinterpret_cast<u16x4 *>(to + line * kRowBytes + 2 * c) = f.hi;
-            *reinterpret_cast<u16x4 *>(to + line * kRowBytes + 2 * c + 64) = f.lo;
-        } else {
-            block_put4(blk, line, c, f);
-        }
+        block_put4(blk, line, c, f);
     }
-    if (s.tall) return;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    block_transposed(blk, to, lane);
+    lds_done();
+    if (!s.tall) {
+        block_transpose(blk, blk + 4096, lane);
+        lds_done();
+    }
+    block_store(s.tall ? blk : blk + 4096, to, lane);
 }
 
 // ---- products ----
@@ -260,9 +268,9 @@ __device__ __forceinline__ void lower_tile(int t, int &ti, int &tj) {
 }
 
 // What a 32 x 32 block of sums becomes, by one wave: register r of lane (col, half) is row acc_row(r, half),
-// column col.  buf: LDS address of 4.25 KiB of the wave's own, on 1 KiB.  (i0, j0): the block's place in the
+// column col.  buf: LDS address of 8 KiB of the wave's own, on 1 KiB.  (i0, j0): the block's place in the
 // product, multiples of 32, so that the block of a factor is a run of 4 KiB, 128 bytes a row.
-constexpr int kBufBytes = 5120;
+constexpr int kBufBytes = 8192;
 template <typename T, int P>
 __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &acc, int i0, int j0, bool mirror,
                                       uint32_t buf, int lane) {
@@ -272,7 +280,7 @@ __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &ac
         lds_float *f = (lds_float *)(uintptr_t)buf;
 #pragma unroll
         for (int r = 0; r < 16; ++r) f[acc_row(r, half) * 33 + col] = acc[r] * (1.f / (kScale * kScale));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds_done();
         // Along the output's rows: X's row i0 + line, or for a tall matrix X's column j0 + line.
         const int64_t row0 = g.s.tall ? j0 : i0;
         const int64_t at = (g.s.tall ? i0 : j0) + col;
@@ -286,12 +294,13 @@ __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &ac
                 if (row0 + line < g.s.rows) *to = from_f32<T>(g.u.muon ? fmaf(-g.u.lr, v, g.u.keep * to_f32(*to)) : v);
             }
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds_done();
     } else {
-        // Four elements of row j0 + col of the transpose at a time, straight from the registers; the block as it is
-        // (symmetric products) through LDS, where the transpose is transposed.
-        const int64_t at = factor_at(j0, i0, g.o_groups) + mat * g.o_bytes + col * kRowBytes + 8 * half;
+        // The registers hold four elements of row j0 + col of the transpose at a time: that goes to LDS and out, and the
+        // block as it is (symmetric products) is its transpose.
+        const int64_t at = factor_at(j0, i0, g.o_groups) + mat * g.o_bytes;
         char *t = g.o + at;
+        const char *A0 = P == kPoly ? g.gram + at + col * kRowBytes + 8 * half : nullptr;
         // a I on the diagonal of the rows that exist.
         const int diag = P == kPoly && i0 == j0 && i0 + col < g.s.r ? col - 4 * half : -1;
 #pragma unroll
@@ -299,26 +308,23 @@ __device__ __forceinline__ void leave(const Gemm &g, int mat, const floatx16 &ac
             f32x4 v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
             v = v * (1.f / kScale);
             if constexpr (P == kPoly) {  // A is symmetric: its row j0 + col
-                const f32x4 A = join4(*reinterpret_cast<const u16x4 *>(g.gram + at + 16 * q),
-                                      *reinterpret_cast<const u16x4 *>(g.gram + at + 16 * q + 64));
+                const f32x4 A = join4(*reinterpret_cast<const u16x4 *>(A0 + 16 * q), *reinterpret_cast<const u16x4 *>(A0 + 16 * q + 64));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] = fmaf(g.pb, A[e], g.pc * v[e]);
                     if (8 * q + e == diag) v[e] += g.pa * kScale;
                 }
             }
-            const Four f = split4(v);
-            if (P == kApply || mirror) {
-                *reinterpret_cast<u16x4 *>(t + 16 * q) = f.hi;
-                *reinterpret_cast<u16x4 *>(t + 16 * q + 64) = f.lo;
-            }
-            if (P != kApply) block_put4(buf, col, 8 * q + 4 * half, f);
+            block_put4(buf, col, 8 * q + 4 * half, split4(v));
         }
+        lds_done();
+        if (P == kApply || mirror) block_store(buf, t, lane);
         if constexpr (P != kApply) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            block_transposed(buf, g.o + mat * g.o_bytes + factor_at(i0, j0, g.o_groups), lane);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next block's writes follow these reads
+            block_transpose(buf, buf + 4096, lane);
+            lds_done();
+            block_store(buf + 4096, g.o + mat * g.o_bytes + factor_at(i0, j0, g.o_groups), lane);
         }
+        lds_done();  // the next block's writes follow these reads
     }
 }
 
