@@ -50,6 +50,7 @@ class PackedPlan:
             self._dev = self._host.to(self.device, non_blocking=True)
             self._ready = torch.cuda.current_stream().record_event()
             self._stream = _stream_handle(None)
+        self._addresses = self._host.data_ptr(), self._dev.data_ptr()
 
     @property
     def cu_seqlens(self):
@@ -73,7 +74,7 @@ class PackedPlan:
             if not torch.cuda.is_current_stream_capturing():  # a capture begins with a device-wide wait
                 cur.wait_event(self._ready)
                 self._dev.record_stream(cur)
-        return self._host.data_ptr(), self._dev.data_ptr()
+        return self._addresses
 
 
 def packed_plan(seqlens, num_heads: int, num_kv_heads: int | None = None, device="cuda") -> PackedPlan:
@@ -87,26 +88,27 @@ def _check_packed(name, plan, q, k, v, *like_q):
         raise ValueError(f"{name}: plan must be a packed_plan on the GPU")
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{name}: tensors must be [tokens, heads, d], got {tuple(q.shape)} and {tuple(k.shape)}")
-    if q.dtype not in _DTYPE_CODE:
-        raise ValueError(f"{name}: dtype {q.dtype} unsupported (float32, bfloat16, float16, float64)")
-    rows, hq, d = q.shape
-    hkv = k.shape[1]
-    if tuple(k.shape) != (rows, hkv, d) or v.shape != k.shape:
-        raise ValueError(f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match")
+    dtype, device, shape = q.dtype, plan.device, q.shape
+    if dtype not in _DTYPE_CODE:
+        raise ValueError(f"{name}: dtype {dtype} unsupported (float32, bfloat16, float16, float64)")
+    rows, hq, d = shape
+    krows, hkv, kd = kshape = k.shape
+    if krows != rows or kd != d or v.shape != kshape:
+        raise ValueError(f"{name}: q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)} do not match")
     if hkv < 1 or hq != hkv * plan.group:
         raise ValueError(f"{name}: {hq} query heads on {hkv} key heads, the plan has {plan.group} to one")
     if rows < plan.tokens:
         raise ValueError(f"{name}: tensors of {rows} rows, the plan has {plan.tokens} tokens")
-    for t in (q, k, v) + like_q:
-        if t.device != plan.device:
-            raise ValueError(f"{name}: a tensor on {t.device}, the plan on {plan.device}")
-        if t.dtype != q.dtype:
-            raise ValueError(f"{name}: dtypes differ, {t.dtype} and {q.dtype}")
+    for t in (q, k, v, *like_q):
+        if t.device != device:
+            raise ValueError(f"{name}: a tensor on {t.device}, the plan on {device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name}: dtypes differ, {t.dtype} and {dtype}")
         if t.stride(2) != 1 and d > 1:
             raise ValueError(f"{name}: a head's elements must be contiguous")
     for t in like_q:
-        if t.shape != q.shape:
-            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(q.shape)}")
+        if t.shape != shape:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _check_lse(name, lse, q):
@@ -115,9 +117,7 @@ def _check_lse(name, lse, q):
         raise ValueError(f"{name}: lse must be contiguous {_stat_dtype(q.dtype)} {list(want)}")
 
 
-def _strides(*ts):
-    flat = [s for t in ts for s in (t.stride(0), t.stride(1))]
-    return (ctypes.c_int64 * len(flat))(*flat)
+_Strides4, _Strides8 = ctypes.c_int64 * 8, ctypes.c_int64 * 16  # (row, head) of 4 and of 8 tensors
 
 
 def flash_attn_packed_fwd(q, k, v, plan, causal: bool = False, out=None, lse=None, stream=None):
@@ -125,21 +125,33 @@ def flash_attn_packed_fwd(q, k, v, plan, causal: bool = False, out=None, lse=Non
     k and v [rows, Hkv, d], of any row and head strides.  Rows behind the last sequence are left as they
     are (zeros where the output is allocated here)."""
     name = "flash_attn_packed_fwd"
-    _check_packed(name, plan, q, k, v, *(() if out is None else (out,)))
-    rows, hq, d = q.shape
+    if out is None:
+        _check_packed(name, plan, q, k, v)
+    else:
+        _check_packed(name, plan, q, k, v, out)
+    if lse is not None:
+        _check_lse(name, lse, q)
+    if stream is None and plan.device.index == torch.cuda.current_device():
+        return _fwd(q, k, v, plan, causal, out, lse, None)
     with on_device(plan.device, stream):
-        make = q.new_empty if rows == plan.tokens else q.new_zeros
-        out = make((rows, hq, d)) if out is None else out
-        if lse is None:
-            lse = make((rows, hq), dtype=_stat_dtype(q.dtype))
-        else:
-            _check_lse(name, lse, q)
-        handle = _stream_handle(stream)
-        host, dev = plan._pointers(handle)
-        rc = load().ctattn_packed_fwd(_DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                      lse.data_ptr(), _strides(q, k, v, out), host, dev, rows, hq, k.shape[1], d,
-                                      int(bool(causal)), handle)
-    _check(rc, "ctattn_packed_fwd")
+        return _fwd(q, k, v, plan, causal, out, lse, stream)
+
+
+def _fwd(q, k, v, plan, causal, out, lse, stream):
+    rows, hq, d = q.shape
+    make = q.new_empty if rows == plan.tokens else q.new_zeros
+    if out is None:
+        out = make((rows, hq, d))
+    if lse is None:
+        lse = make((rows, hq), dtype=_stat_dtype(q.dtype))
+    handle = _stream_handle(stream)
+    host, dev = plan._pointers(handle)
+    strides = _Strides4(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0),
+                        out.stride(1))
+    rc = load().ctattn_packed_fwd(_DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                  lse.data_ptr(), strides, host, dev, rows, hq, k.shape[1], d, int(bool(causal)), handle)
+    if rc != 0:
+        _check(rc, "ctattn_packed_fwd")
     return out, lse
 
 
@@ -178,7 +190,7 @@ def flash_attn_packed_bwd(q, k, v, o, do, lse, plan, causal: bool = False, dq=No
         rc = load().ctattn_packed_bwd(_DTYPE_CODE[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
                                       do.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                       _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                      _strides(q, k, v, o, do, dq, dk, dv), host, dev, rows, hq, hkv, d,
+                                      _Strides8(*(n for t in (q, k, v, o, do, dq, dk, dv) for n in t.stride()[:2])), host, dev, rows, hq, hkv, d,
                                       int(bool(causal)), handle)
     _check(rc, "ctattn_packed_bwd")
     return dq, dk, dv
