@@ -11,6 +11,7 @@
 //   SGDOptimizer           SGDOptimizer.cu (over parameter / gradient maps)
 //   AdamOptimizer          AdamOptimizer.cu:21-140 (over parameter / gradient maps)
 //   AdamWOptimizer         AdamOptimizer.cu:142-233
+//   MuonOptimizer          no counterpart
 // Same conventions as the reference: weights start at zero (cudaMakeShared zero-fills,
 // LinearLayer.cu:28), LayerNorm at (1, 0); gradients accumulate across backward calls until
 // zeroGrad; backward(input, gradOutput) works for any `input`.  Differences: the reference
@@ -779,6 +780,59 @@ struct AdamWOptimizer : public AdamOptimizer<DType> {
     explicit AdamWOptimizer(std::map<std::string, Tensor<DType>> params, double lr = 1e-3, double b1 = 0.9,
                             double b2 = 0.999, double eps = 1e-8, double decay = 0.0)
         : AdamOptimizer<DType>(std::move(params), lr, b1, b2, eps, decay, true) {}
+};
+
+// Muon over a parameter map of matrices (no counterpart in the reference): step(grads) orthogonalises each matrix's
+// momentum and moves the matrix along it, matrices of one shape together (ctattn_muon_update_multi).  Parameters that
+// are not matrices, embeddings among them, belong to another optimizer.  fp32, bf16 and fp16; moments are fp32, zero
+// at construction; an update is scaled by sqrt(max(1, rows / cols)).
+template <typename DType = float>
+struct MuonOptimizer {
+    std::map<std::string, Tensor<DType>> parameters;
+    double learningRate, momentum, decay;
+    bool nesterov;
+    int steps;
+    std::map<std::string, std::shared_ptr<float[]>> moments;
+
+    explicit MuonOptimizer(std::map<std::string, Tensor<DType>> params, double lr = 0.02, double momentum = 0.95,
+                           double decay = 0.0, bool nesterov = true, int steps = 5)
+        : parameters(std::move(params)), learningRate(lr), momentum(momentum), decay(decay), nesterov(nesterov),
+          steps(steps) {
+        for (const auto &[name, p] : parameters) {
+            if (p.shape().size() != 2 || p.size() == 0)
+                throw std::invalid_argument("MuonOptimizer: parameter '" + name + "' is not a matrix.");
+            moments[name] = detail::zeros<float>(p.size());
+        }
+    }
+
+    void step(const std::map<std::string, Tensor<DType>> &grads) {
+        detail::checkGrads(parameters, grads);
+        struct Group {
+            std::vector<void *> p, m;
+            std::vector<const void *> g;
+        };
+        std::map<std::pair<int64_t, int64_t>, Group> groups;
+        for (const auto &[name, p] : parameters) {
+            Group &group = groups[{int64_t(p.shape()[0]), int64_t(p.shape()[1])}];
+            group.p.push_back(p.get());
+            group.g.push_back(grads.at(name).get());
+            group.m.push_back(moments.at(name).get());
+        }
+        for (auto &[shape, group] : groups) {
+            const int64_t rows = shape.first, cols = shape.second;
+            const int64_t bytes = ctattn_muon_update_workspace_bytes(DTypeCode<DType>::value, int64_t(group.p.size()), rows, cols);
+            if (bytes < 0) ctattnCheck(int(hipErrorInvalidValue), "ctattn_muon_update_workspace_bytes");
+            std::shared_ptr<uint8_t[]> workspace = deviceAlloc<uint8_t>(size_t(bytes));
+            ctattnCheck(ctattn_muon_update_multi(DTypeCode<DType>::value, int(group.p.size()), group.p.data(), group.g.data(),
+                                                 group.m.data(), workspace.get(), bytes, rows, cols, learningRate, momentum,
+                                                 nesterov ? 1 : 0, decay, std::sqrt(std::max(1.0, double(rows) / double(cols))),
+                                                 steps, 3.4445, -4.7750, 2.0315, 1e-7, Runtime::stream()),
+                        "ctattn_muon_update_multi");
+        }
+    }
+
+    double getLearningRate() const { return learningRate; }
+    void setLearningRate(double lr) { learningRate = lr; }
 };
 
 }  // namespace ct

@@ -23,7 +23,7 @@
 // <T>TransformerLayer and their factories (LayerNorm, Linear, Activation, ReLU, GELU, Sigmoid,
 // Tanh, MLP, Checkpoint, TransformerBlock, Transformer; with the <T> suffix, float without
 // one), <T>Softmax, <T>CrossEntropyLoss, <T>MSELoss, <T>TokenEmbedding, <T>PositionEmbedding,
-// <T>UnEmbedding, <T>NanoGPT, <T>SGDOptimizer, <T>AdamOptimizer, <T>AdamWOptimizer;
+// <T>UnEmbedding, <T>NanoGPT, <T>SGDOptimizer, <T>AdamOptimizer, <T>AdamWOptimizer, <T>MuonOptimizer (not Double);
 // IntTensor for ids; enums ActivationType and SamplingMode.  Id arguments accept an
 // IntTensor, a NumPy array or a list.  Half and Double tensors take float32 / float64 numpy
 // arrays.
@@ -577,6 +577,16 @@ void declareNanoGPT(py::module_ &m, const std::string &suffix) {
         .def(py::init<std::map<std::string, T>, double, double, double, double, double>(), py::arg("params"),
              py::arg("lr") = 0.001, py::arg("b1") = 0.9, py::arg("b2") = 0.999, py::arg("eps") = 1e-8,
              py::arg("decay") = 0.0);
+    if constexpr (!std::is_same_v<DType, double>) {
+        using MUON = MuonOptimizer<DType>;
+        py::class_<MUON>(m, name("MuonOptimizer").c_str(), "Muon over a map of matrices (orthogonalised momentum).")
+            .def(py::init<std::map<std::string, T>, double, double, double, bool, int>(), py::arg("params"),
+                 py::arg("lr") = 0.02, py::arg("momentum") = 0.95, py::arg("decay") = 0.0, py::arg("nesterov") = true,
+                 py::arg("steps") = 5)
+            .def("step", &MUON::step, py::arg("grads"), "One update of every matrix from `grads`.")
+            .def("getLearningRate", &MUON::getLearningRate)
+            .def("setLearningRate", &MUON::setLearningRate, py::arg("lr"));
+    }
 }
 
 }  // namespace
@@ -592,7 +602,7 @@ PYBIND11_MODULE(cuda_transformer, m) {
         "Checkpoint, TransformerBlock, Transformer, with a <T> suffix, float without one).\n"
         "Losses: <T>Softmax, <T>CrossEntropyLoss, <T>MSELoss.  Model: <T>TokenEmbedding,\n"
         "<T>PositionEmbedding, <T>UnEmbedding, <T>NanoGPT.  Optimizers: <T>SGDOptimizer,\n"
-        "<T>AdamOptimizer, <T>AdamWOptimizer.  Enums ActivationType, SamplingMode.";
+        "<T>AdamOptimizer, <T>AdamWOptimizer, <T>MuonOptimizer (not Double).  Enums ActivationType, SamplingMode.";
 
     py::enum_<ActivationType>(m, "ActivationType", "Activation of the MLP sub-layers.")
         .value("ReLU", ActivationType::ReLU)

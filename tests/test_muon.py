@@ -182,6 +182,32 @@ def test_muon_update(dtype, nesterov, count):
 
 
 @gpu
+@pytest.mark.parametrize("kind,dtype", [("Float", torch.float32), ("BFloat", torch.bfloat16), ("Half", torch.float16)])
+def test_native_optimizer(kind, dtype):
+    """The C++ host's optimizer moves its matrices as muon_update does: the same kernels in the same batches."""
+    from cudatransformer_amd import cuda_transformer as ctm
+
+    tensor = getattr(ctm, f"{kind}Tensor")
+    shapes = {"a": (40, 24), "b": (24, 40), "c": (40, 24)}
+    p = {n: _make(s, dtype, seed=i) for i, (n, s) in enumerate(shapes.items())}
+    g = {n: _make(s, dtype, seed=50 + i) for i, (n, s) in enumerate(shapes.items())}
+    to = lambda t: tensor.fromNumpy(t.double().cpu().numpy())  # noqa: E731
+    params, grads = {n: to(t) for n, t in p.items()}, {n: to(t) for n, t in g.items()}
+    opt = getattr(ctm, f"{kind}MuonOptimizer")(params, lr=0.03, momentum=0.9, decay=0.1)
+    moments = {n: torch.zeros(s, device="cuda") for n, s in shapes.items()}
+    for _ in range(2):
+        opt.step(grads)
+        ct.muon_update([p[n] for n in p], [g[n] for n in p], [moments[n] for n in p], lr=0.03, momentum=0.9, weight_decay=0.1)
+    for n in p:
+        assert torch.equal(torch.from_numpy(params[n].numpy()).double(), p[n].double().cpu()), n
+    with pytest.raises(ValueError):
+        opt.step({"a": grads["a"]})
+    with pytest.raises(ValueError):
+        getattr(ctm, f"{kind}MuonOptimizer")({"v": tensor.fromNumpy(torch.zeros(5).numpy())})
+    assert not hasattr(ctm, "DoubleMuonOptimizer")
+
+
+@gpu
 def test_binding_refusals():
     x = _make((8, 6), torch.float32)
     for f in (lambda: ct.newton_schulz(x.double()), lambda: ct.newton_schulz(x.t()), lambda: ct.newton_schulz(x.cpu()),
