@@ -626,6 +626,14 @@ int check(const char *fn, int dtype, int id_dtype, int64_t n, int64_t D, int64_t
     return 0;
 }
 
+// Whether [a, a + an) and [b, b + bn) share a byte.
+bool share(const void *a, int64_t an, const void *b, int64_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return an > 0 && bn > 0 && x < y + uintptr_t(bn) && y < x + uintptr_t(an);
+}
+int64_t elem_bytes(int dtype) { return dtype == CTATTN_F64 ? 8 : dtype == CTATTN_F32 ? 4 : 2; }
+int64_t id_bytes(int id_dtype) { return id_dtype == CTATTN_I64 ? 8 : 4; }
+
 }  // namespace
 }  // namespace ctattn
 
@@ -642,6 +650,9 @@ int ctattn_embedding_lookup(int dtype, int id_dtype, const void *ids, const void
     if (int rc = check(fn, dtype, id_dtype, n, D, vocab)) return rc;
     if (n == 0) return ok();
     if (!ids || !table || !out) return fail(hipErrorInvalidValue, "%s: null pointer", fn);
+    const int64_t es = elem_bytes(dtype);
+    if (share(out, n * D * es, table, vocab * D * es) || share(out, n * D * es, ids, n * id_bytes(id_dtype)))
+        return fail(hipErrorInvalidValue, "%s: out lies on an input's memory", fn);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const hipError_t e = typed(dtype, id_dtype == CTATTN_I64, [&](auto *t, auto *i) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -664,6 +675,9 @@ int ctattn_embedding_grad(int dtype, int id_dtype, const void *ids, const void *
     if (int rc = check(fn, dtype, id_dtype, n, D, vocab)) return rc;
     if (!dtable) return fail(hipErrorInvalidValue, "%s: null dtable pointer", fn);
     if (n > 0 && (!ids || !dout)) return fail(hipErrorInvalidValue, "%s: null ids/dout pointer", fn);
+    const int64_t es = elem_bytes(dtype);
+    if (share(dtable, vocab * D * es, dout, n * D * es) || share(dtable, vocab * D * es, ids, n * id_bytes(id_dtype)))
+        return fail(hipErrorInvalidValue, "%s: dtable lies on an input's memory", fn);
     const int64_t need = n == 0 ? 0 : grad_plan(dtype, n, D, vocab).bytes;
     if (need > 0 && (!workspace || workspace_bytes < need))
         return fail(hipErrorInvalidValue, "%s: workspace too small (%lld bytes, %lld needed)", fn,

@@ -26,7 +26,9 @@
 #include "ctattn.h"
 
 #include <algorithm>
+#include <exception>
 #include <type_traits>
+#include <vector>
 
 namespace ctattn {
 namespace {
@@ -741,6 +743,39 @@ int check_workspace(const char *fn, const void *ws, int64_t bytes, int64_t need)
     return 0;
 }
 
+// Refuses parameters or moments that share memory with any other tensor of the call.
+int check_separate(const char *fn, int count, void *const *param, const void *const *grad, void *const *moment, int64_t n,
+                   int64_t es) {
+    struct Range {
+        uintptr_t lo, hi;
+        bool written;
+    };
+    try {
+        std::vector<Range> all;
+        all.reserve(3 * size_t(count));
+        for (int i = 0; i < count; ++i) {
+            const auto add = [&](const void *p, int64_t bytes, bool written) {
+                const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+                all.push_back({at, at + uintptr_t(bytes), written});
+            };
+            add(param[i], n * es, true);
+            add(grad[i], n * es, false);
+            add(moment[i], n * 4, true);
+        }
+        std::sort(all.begin(), all.end(), [](const Range &a, const Range &b) { return a.lo < b.lo; });
+        uintptr_t any = 0, written = 0;  // how far the ranges so far reach
+        for (const Range &r : all) {
+            if (r.lo < written || (r.written && r.lo < any))
+                return fail(hipErrorInvalidValue, "%s: a parameter or moment shares memory with another tensor", fn);
+            any = std::max(any, r.hi);
+            if (r.written) written = std::max(written, r.hi);
+        }
+    } catch (const std::exception &) {
+        return fail(hipErrorOutOfMemory, "%s: out of host memory", fn);
+    }
+    return 0;
+}
+
 }  // namespace
 }  // namespace ctattn
 
@@ -792,6 +827,7 @@ int ctattn_muon_update_multi(int dtype, int count, void *const *param, const voi
     if (!param || !grad || !moment) return fail(hipErrorInvalidValue, "%s: null pointer table", fn);
     for (int i = 0; i < count; ++i)
         if (!param[i] || !grad[i] || !moment[i]) return fail(hipErrorInvalidValue, "%s: null pointer in matrix %d", fn, i);
+    if (int rc = check_separate(fn, count, param, grad, moment, rows * cols, dtype == CTATTN_F32 ? 4 : 2)) return rc;
     if (int rc = check_workspace(fn, workspace, workspace_bytes, batches_bytes(count, rows, cols))) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int i0 = 0; i0 < count; i0 += kMaxMats) {

@@ -125,6 +125,27 @@ int check_outputs(const char *fn, std::initializer_list<const PackedStride *> ou
     return 0;
 }
 
+// The bytes of a [rows, heads, d] tensor: `lo`, `hi` its first and last; within a row from `lo` on `span` of them
+// every `row`, unless heads lie further apart than rows.
+struct Bytes {
+    intptr_t lo, hi, row, span;
+};
+Bytes bytes_of(const void *p, const PackedStride &s, int64_t rows, int64_t heads, int64_t d, int64_t es) {
+    const intptr_t at = reinterpret_cast<intptr_t>(p);
+    const auto end = [&](int64_t n, int64_t step) { return n > 1 ? (n - 1) * step : 0; };
+    const int64_t up = std::max<int64_t>(0, end(rows, s.row)) + std::max<int64_t>(0, end(heads, s.head));
+    const int64_t down = std::min<int64_t>(0, end(rows, s.row)) + std::min<int64_t>(0, end(heads, s.head));
+    return {at + down * es, at + (up + d) * es, s.row * es, (end(heads, s.head) + d) * es};
+}
+// Whether two tensors may share a byte.  Slices of one row-major buffer (a projection's q, k, v) do not: their rows are
+// equally far apart and each lies in its own part of a row.
+bool may_overlap(const Bytes &a, const Bytes &b) {
+    if (a.hi <= b.lo || b.hi <= a.lo) return false;
+    if (a.row != b.row || a.row <= 0 || a.span <= 0 || b.span <= 0 || a.span > a.row || b.span > a.row) return true;
+    const intptr_t shift = ((b.lo - a.lo) % a.row + a.row) % a.row;
+    return !(a.span <= shift && shift + b.span <= a.row);
+}
+
 int64_t elem_bytes(int dtype) { return dtype == CTATTN_F64 ? 8 : dtype == CTATTN_F32 ? 4 : 2; }
 
 // The MFMA kernels move 16 bytes per access: pointers and strides on 16 bytes.
@@ -197,6 +218,11 @@ int ctattn_packed_fwd(int dtype, const void *q, const void *k, const void *v, vo
     if (c.tokens() == 0) return ok();
     if (int rc = check_outputs(fn, {&c.so}, {hq}, c.tokens(), d)) return rc;
     if (!q || !k || !v || !o) return fail(hipErrorInvalidValue, "%s: null q/k/v/o pointer", fn);
+    const int64_t es = elem_bytes(dtype);
+    const Bytes bo = bytes_of(o, c.so, c.tokens(), hq, d, es);
+    if (may_overlap(bo, bytes_of(q, c.sq, c.tokens(), hq, d, es)) || may_overlap(bo, bytes_of(k, c.sk, c.tokens(), hkv, d, es)) ||
+        may_overlap(bo, bytes_of(v, c.sv, c.tokens(), hkv, d, es)))
+        return fail(hipErrorInvalidValue, "%s: o lies on an input's memory", fn);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Sides all[] = {{q, &c.sq}, {k, &c.sk}, {v, &c.sv}, {o, &c.so}};
     const bool fast = mfma(c) && std::all_of(std::begin(all), std::end(all), [&](const Sides &x) { return on16(x, dtype); });
@@ -230,6 +256,16 @@ int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, co
     if (int rc = check_outputs(fn, {&c.sdq, &c.sdk, &c.sdv}, {hq, hkv, hkv}, c.tokens(), d)) return rc;
     if (!q || !k || !v || !o || !dout || !lse || !dq || !dk || !dv)
         return fail(hipErrorInvalidValue, "%s: null tensor pointer", fn);
+    const int64_t es = elem_bytes(dtype), n = c.tokens();
+    const Bytes in[] = {bytes_of(q, c.sq, n, hq, d, es),  bytes_of(k, c.sk, n, hkv, d, es), bytes_of(v, c.sv, n, hkv, d, es),
+                        bytes_of(o, c.so, n, hq, d, es),  bytes_of(dout, c.sdo, n, hq, d, es)};
+    const Bytes out[] = {bytes_of(dq, c.sdq, n, hq, d, es), bytes_of(dk, c.sdk, n, hkv, d, es), bytes_of(dv, c.sdv, n, hkv, d, es)};
+    for (int i = 0; i < 3; ++i) {
+        for (const Bytes &b : in)
+            if (may_overlap(out[i], b)) return fail(hipErrorInvalidValue, "%s: a gradient lies on an input's memory", fn);
+        for (int j = 0; j < i; ++j)
+            if (may_overlap(out[i], out[j])) return fail(hipErrorInvalidValue, "%s: two gradients share memory", fn);
+    }
     const int64_t need = scratch_bytes(c);
     if (!workspace || workspace_bytes < need)
         return fail(hipErrorInvalidValue, "%s: workspace too small (%lld bytes, %lld needed)", fn,

@@ -77,12 +77,8 @@ def muon_update(params, grads, moments, lr: float = 0.02, momentum: float = 0.95
     for i, (p, g, m) in enumerate(zip(params, grads, moments)):
         if p.dim() != 2 or p.shape != g.shape or p.shape != m.shape or m.dtype != torch.float32 or m.device != p.device:
             raise ValueError(f"{name}: matrix {i} needs a gradient and a float32 moment of its shape on its device")
-        if len({p.data_ptr(), g.data_ptr(), m.data_ptr()}) < 3 and p.numel() > 0:
-            raise ValueError(f"{name}: matrix {i} shares its memory with its gradient or moment")
         if p.numel() > 0:
             shapes.setdefault(tuple(p.shape), []).append(i)
-    if len({params[i].data_ptr() for s in shapes.values() for i in s}) < sum(len(s) for s in shapes.values()):
-        raise ValueError(f"{name}: a parameter is listed twice")
     a, b, c = (float(v) for v in coeffs)
     dev, code, lib = params[0].device, _DTYPE_CODE[params[0].dtype], load()
     needs = {}
@@ -116,6 +112,14 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.dim() != 2:
                     raise ValueError(f"Muon: parameters must be matrices, got {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # The base class gives a 16-bit parameter's state the parameter's type; moments stay float32.
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], saved["params"]):
+                if "moment" in state_dict["state"].get(key, {}):
+                    self.state[p]["moment"] = state_dict["state"][key]["moment"].to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):

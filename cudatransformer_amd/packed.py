@@ -44,6 +44,8 @@ class PackedPlan:
             return
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("packed_plan: a plan is made before a graph's capture, not in it")
         self._host = torch.empty(need, dtype=torch.uint8, pin_memory=True)
         _check(lib.ctattn_packed_plan(lens, n, self.group, self._host.data_ptr(), need), "ctattn_packed_plan")
         with on_device(self.device):

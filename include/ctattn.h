@@ -604,7 +604,8 @@ CTATTN_API int ctattn_packed_plan(const int64_t *seqlens, int64_t nseq, int64_t 
  * CTATTN_F64, else fp32; may be NULL).  q and o are [rows, Hq, d], k and v [rows, Hkv, d], rows >=
  * the plan's tokens; rows behind the last sequence are neither read nor written.  `strides` (HOST)
  * holds, in elements, the row and the head stride of q, k, v and o; the d elements of a head are
- * contiguous, and the outputs' elements must not overlap.
+ * contiguous.  No output may share memory with an input or another output (slices of one row-major buffer, a
+ * projection's q, k and v, do not; others are refused).
  *   - bf16, fp16 (d a multiple of 8) and fp32 (a multiple of 4) run on MFMA kernels for d <= 128 and
  *     Hq / Hkv <= 128 when pointers and strides are multiples of 16 bytes; other calls, f64, and every
  *     call under CTATTN_POLICY_GENERIC take generic kernels (same results, much slower).
@@ -639,7 +640,7 @@ CTATTN_API int ctattn_packed_bwd(int dtype, const void *q, const void *k, const 
  * out[i][:] = scale * table[ids[i]][:] for n ids (id_dtype CTATTN_I32 or CTATTN_I64), table [vocab][D], out
  * [n][D], both contiguous of type dtype (f32, bf16, f16, f64); an id outside [0, vocab) gives a row of
  * zeros.  Computed in fp32 (fp64 for f64) and rounded once.  No counterpart in the reference, whose
- * lookup has no scale (ctattn_embedding_fwd).
+ * lookup has no scale (ctattn_embedding_fwd).  out may not lie on table or ids (refused).
  */
 CTATTN_API int ctattn_embedding_lookup(int dtype, int id_dtype, const void *ids, const void *table, void *out,
                                        double scale, int64_t n, int64_t D, int64_t vocab, void *stream);
@@ -652,7 +653,7 @@ CTATTN_API int64_t ctattn_embedding_grad_workspace_bytes(int dtype, int64_t n, i
  * (rows without a token with zeros); accumulate != 0 adds to what dtable holds instead.  Ids outside
  * [0, vocab) add nothing.  Tokens are sorted by id and summed in the order of their positions, in fp32
  * (fp64 for f64), with one rounding per element: no atomics on values, the same inputs give the same
- * bits, any D and alignment.  ctattn_embedding_bwd, the reference's counterpart, adds into dtable with
+ * bits, any D and alignment; dtable may not lie on dout or ids (refused).  ctattn_embedding_bwd, the reference's counterpart, adds into dtable with
  * atomics.  The workspace (16-byte aligned) is scratch, free again when the stream has passed the call.
  */
 CTATTN_API int ctattn_embedding_grad(int dtype, int id_dtype, const void *ids, const void *dout, void *dtable,
@@ -680,7 +681,8 @@ CTATTN_API int ctattn_newton_schulz(int dtype, const void *x, void *out, void *w
  * One Muon step on `count` matrices [rows][cols] given by HOST tables of device pointers, in place:
  *   m <- momentum m + g;  u = nesterov ? g + momentum m : m
  *   p <- (1 - lr weight_decay) p - lr scale NewtonSchulz(u)
- * param and grad of type dtype, moment fp32 whatever the dtype; no tensor may overlap another.  The update of
+ * param and grad of type dtype, moment fp32 whatever the dtype; a param or moment may not share memory with any other
+ * tensor (refused).  The update of
  * p happens in the last product's epilogue.  64 matrices a batch, through one workspace.  Stands beside
  * ctattn_adam_update_multi; no counterpart in the reference.
  */

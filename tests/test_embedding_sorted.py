@@ -185,17 +185,25 @@ def test_binding_refusals():
               lambda: ct.embedding_grad(ids[::2], dout[::2], 20)):
         with pytest.raises(ValueError):
             f()
+    square = torch.zeros((20, 8), device="cuda")
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.embedding_lookup(torch.zeros(20, dtype=torch.int32, device="cuda"), square, out=square)
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.embedding_grad(torch.zeros(20, dtype=torch.int32, device="cuda"), square, 20, out=square)
     with pytest.raises(RuntimeError, match="workspace"):
         ct.embedding_grad(ids, dout, 20, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
 
 
 def test_c_entry_refusals():
     lib = _capi.load()
-    look = lambda dt=0, it=4, p=64, n=3, d=8, v=9: lib.ctattn_embedding_lookup(dt, it, p, p, p, 1.0, n, d, v, None)  # noqa: E731
+    look = lambda dt=0, it=4, p=1 << 20, n=3, d=8, v=9: lib.ctattn_embedding_lookup(dt, it, p, p, p, 1.0, n, d, v, None)  # noqa: E731
+    assert look() == 1 and "input's memory" in _capi.last_error()
     assert look(dt=4) == 1 and look(it=0) == 1 and look(p=None) == 1 and look(n=-1) == 1 and look(d=0) == 1 and look(v=0) == 1
     assert look(n=1 << 31) == 1 and look(v=(1 << 31) - 1) == 1 and look(d=1 << 30, n=1 << 30) == 1 and look(n=0, p=None) == 0
     need = lib.ctattn_embedding_grad_workspace_bytes(0, 3, 8, 9)
     assert need > 0 and lib.ctattn_embedding_grad_workspace_bytes(0, 3, 0, 9) == -1
-    grad = lambda ws=256, size=need, p=64, n=3: lib.ctattn_embedding_grad(0, 4, p, p, p, 1.0, 0, ws, size, n, 8, 9, None)  # noqa: E731
+    big = 1 << 20
+    grad = lambda ws=256, size=need, p=big, n=3: lib.ctattn_embedding_grad(0, 4, p, 2 * big if p else p, 3 * big if p else p, 1.0, 0, ws,  # noqa: E731
+                                                                           size, n, 8, 9, None)
     assert grad(ws=None) == 1 and grad(size=need - 1) == 1 and grad(ws=264) == 1 and grad(p=None) == 1
     assert ctypes.string_at(lib.ctattn_last_error()) != b""

@@ -208,6 +208,20 @@ def test_native_optimizer(kind, dtype):
 
 
 @gpu
+def test_state_of_16_bit_parameters_is_kept():
+    p = torch.nn.Parameter(_make((12, 9), torch.bfloat16))
+    p.grad = _make((12, 9), torch.bfloat16, seed=1)
+    opt = ct.Muon([p])
+    opt.step()
+    saved = opt.state_dict()
+    again = ct.Muon([p])
+    again.load_state_dict(saved)
+    got, want = again.state[p]["moment"], opt.state[p]["moment"]
+    assert got.dtype == torch.float32 and torch.equal(got, want) and got.data_ptr() != want.data_ptr()
+    again.step()
+
+
+@gpu
 def test_binding_refusals():
     x = _make((8, 6), torch.float32)
     for f in (lambda: ct.newton_schulz(x.double()), lambda: ct.newton_schulz(x.t()), lambda: ct.newton_schulz(x.cpu()),
@@ -238,11 +252,17 @@ def test_c_entry_refusals():
     need = lib.ctattn_muon_update_workspace_bytes(1, 100, 8, 6)
     # Batches of 64 and the rest.
     assert need == max(lib.ctattn_muon_update_workspace_bytes(1, n, 8, 6) for n in (64, 36)) > 0
-    one = (ctypes.c_void_p * 1)(64)
+    one, two, three = ((ctypes.c_void_p * 1)(i << 20) for i in (1, 2, 3))
     none = (ctypes.c_void_p * 1)(None)
 
-    def muon(p=one, g=one, m=one, count=1, size=1 << 40):
+    def muon(p=one, g=two, m=three, count=1, size=1 << 40):
         return lib.ctattn_muon_update_multi(1, count, p, g, m, 256, size, 8, 6, 0.1, 0.9, 1, 0.0, 1.0, 5, 1.0, 0.0, 0.0, 0.0, None)
 
     assert muon(p=None) == 1 and muon(g=none) == 1 and muon(m=none) == 1 and muon(size=64) == 1 and muon(count=-1) == 1
     assert muon(count=0, p=None) == 0
+    near = (ctypes.c_void_p * 1)((1 << 20) + 8 * 6 * 2 - 1)  # the last byte of p
+    for bad in (dict(g=one), dict(m=one), dict(m=two), dict(g=near), dict(m=near)):
+        assert muon(**bad) == 1 and "shares memory" in _capi.last_error()
+    twice = (ctypes.c_void_p * 2)(1 << 20, 1 << 20)
+    pair = lambda k: (ctypes.c_void_p * 2)(k << 20, (k + 1) << 20)  # noqa: E731
+    assert muon(p=twice, g=pair(4), m=pair(6), count=2) == 1 and "shares memory" in _capi.last_error()

@@ -97,13 +97,28 @@ def test_c_entry_refusals():
     for o_row, o_head in [(256, 32), (64, 64), (0, 64), (256, 0), (-256, 64)]:
         st = (ctypes.c_int64 * 8)(256, 64, 128, 64, 128, 64, o_row, o_head)
         assert fwd(strides=st) == 1 and "overlap" in _capi.last_error()
+    big = 1 << 20  # apart from each other
+    call = lambda q, k, v, o: lib.ctattn_packed_fwd(1, q, k, v, o, None, st8, host, None, 8, 4, 2, 64, 1, None)  # noqa: E731
+    assert call(big, 2 * big, 3 * big, 4 * big) == 1 and "device plan" in _capi.last_error()
     need = lib.ctattn_packed_bwd_workspace_bytes(1, host, 4, 2, 64)
     assert need > 0 and lib.ctattn_packed_bwd_workspace_bytes(1, host, 4, 4, 64) == -1
 
     def bwd(ws=256, size=need, p=64):
         return lib.ctattn_packed_bwd(1, p, p, p, p, p, p, p, p, p, ws, size, st8, host, 64, 8, 4, 2, 64, 1, None)
 
-    assert bwd(ws=None) == 1 and bwd(size=need - 1) == 1 and bwd(ws=8) == 1 and bwd(p=None) == 1
+    assert bwd(p=None) == 1
+
+    def grads(at, ws=256, size=need):
+        return lib.ctattn_packed_bwd(1, *[a * big for a in at], 9 * big, *[a * big for a in (6, 7, 8)], ws, size, st8, host, 64, 8, 4,
+                                     2, 64, 1, None)
+
+    assert grads((1, 2, 3, 4, 5), ws=None) == 1 and grads((1, 2, 3, 4, 5), size=need - 1) == 1 and grads((1, 2, 3, 4, 5), ws=8) == 1
+    for at in ((6, 2, 3, 4, 5), (1, 7, 3, 4, 5), (1, 2, 8, 4, 5), (1, 2, 3, 6, 5), (1, 2, 3, 4, 7)):
+        assert grads(at) == 1 and "input's memory" in _capi.last_error()
+    # Slices of one row-major buffer do not overlap, shifted ones do.
+    wide = lambda o: lib.ctattn_packed_fwd(1, big, 4 * big, 4 * big, big + o, None, (ctypes.c_int64 * 8)(512, 64, 128, 64, 128, 64, 512, 64),  # noqa: E731
+                                           host, 64, 8, 4, 2, 300, 1, None)
+    assert wide(512) == 801  # the head dim is refused first
     with pytest.raises(ValueError, match="on the GPU"):
         ct.flash_attn_packed_fwd(torch.zeros(8, 4, 64), torch.zeros(8, 2, 64), torch.zeros(8, 2, 64), plan)
 
@@ -458,3 +473,25 @@ def test_binding_refusals():
         ct.flash_attn_packed_bwd(q, k, v, o, do, lse, plan, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
     with pytest.raises(RuntimeError, match="overlap"):
         ct.flash_attn_packed_fwd(q, k, v, plan, out=q.new_empty(64).expand(12, 4, 64))
+    # Outputs on an input's memory, or on each other's.
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.flash_attn_packed_fwd(q, k, v, plan, out=q)
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.flash_attn_packed_bwd(q, k, v, o, do, lse, plan, dq=q)
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.flash_attn_packed_bwd(q, k, v, o, do, lse, plan, dv=v)
+    both = torch.empty_like(k)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ct.flash_attn_packed_bwd(q, k, v, o, do, lse, plan, dk=both, dv=both)
+    buf = q.new_empty((12, 8, 64))
+    buf[:, :4] = q
+    a, b = buf[:, :4], buf[:, 4:]  # apart within every row
+    assert torch.equal(ct.flash_attn_packed_fwd(a, k, v, plan, out=b)[0], o)
+    with pytest.raises(RuntimeError, match="input's memory"):
+        ct.flash_attn_packed_fwd(a, k, v, plan, out=buf[:, 3:7])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            ct.packed_plan([4], 4, 2)
+        q.mul_(1.0)  # a graph with nothing in it is not one
