@@ -639,15 +639,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
         }
     }
     nd += __shfl_xor(nd, 32, kWave);  // the row's other half
-    float nl = 0.f;
-    if (row < rows) {
-        nl = -a.lse[int64_t(it.start + token) * (a.hkv * a.group) + head] * kLog2e;
-        if (ks == 0 && half == 0) {
-            const int64_t at = (int64_t(kvh) * a.tokens + it.start) * a.group + row;
-            a.ndelta[at] = nd;
-            a.nl2[at] = nl;
-        }
-    }
+    const float nl = row < rows ? -a.lse[int64_t(it.start + token) * (a.hkv * a.group) + head] * kLog2e : 0.f;
     floatx16 dq[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) dq[dt] = zero16();
@@ -663,12 +655,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
         load_rows<C::RB, C::BN, C::NW, PAD>(t, kb0 + j0 * a.k.row, a.k.row, a.width, it.len - j0, wave, lane);
         load_rows<C::RB, C::BN, C::NW, PAD>(t + C::KB, vb0 + j0 * a.v.row, a.v.row, a.width, it.len - j0, wave, lane);
     };
-    auto block = [&](auto mask, int kb) __attribute__((always_inline)) {
-        constexpr bool MASK = decltype(mask)::value;
+    // ALONE: the block holds every key that the wave's rows see, so that delta = sum_j P dP is there before dS needs it.
+    // rowsum(dO O) is off by O's rounding, which for rows of few keys (O as large as V, dS small or 0) is as much as the
+    // other roundings of dQ and dK: 26 documents of 1 to 3011 tokens, bf16, dQ off by 2.6e-3 of its norm with it
+    // everywhere, by 2.4e-3 this way.
+    auto block = [&](auto mask, auto alone, int kb) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask)::value, ALONE = decltype(alone)::value;
         const uint32_t kt = L + uint32_t((kb % C::NBUF) * 2 * C::KB) + uint32_t(koff * C::RB);
         floatx16 s = zero16(), dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = nd;
+        for (int r = 0; r < 16; ++r) dp[r] = ALONE ? 0.f : nd;
         V k[2], v[2];
         const uint32_t ak = kt + rk;
         k[0] = lds_b128<V>(ak);
@@ -686,14 +682,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
             dp = F::mma(v[cur], gb[st], dp);
         }
         typename F::pvec db[2];
+        if constexpr (ALONE) {
+            float delta = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float ds = fast_exp2(fmaf(s[r], a.c, nl)) * dp[r];
-            if (MASK) {
+            for (int r = 0; r < 16; ++r) {
                 const int key = kb * C::BN + koff + acc_row(r, half);
-                ds = (key >= it.len || (a.causal && key > token)) ? 0.f : ds;
+                const bool hidden = key >= it.len || (a.causal && key > token);
+                s[r] = hidden ? 0.f : fast_exp2(fmaf(s[r], a.c, nl));
+                dp[r] = hidden ? 0.f : dp[r];
+                delta = fmaf(s[r], dp[r], delta);
             }
-            F::put(db[r / 8], r % 8, ds);
+            delta += __shfl_xor(delta, 32, kWave);
+            nd = row < rows ? -delta : 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) F::put(db[r / 8], r % 8, s[r] * (dp[r] - delta));
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float ds = fast_exp2(fmaf(s[r], a.c, nl)) * dp[r];
+                if (MASK) {
+                    const int key = kb * C::BN + koff + acc_row(r, half);
+                    ds = (key >= it.len || (a.causal && key > token)) ? 0.f : ds;
+                }
+                F::put(db[r / 8], r % 8, ds);
+            }
         }
         constexpr int NS = 2 * C::DT;
         typename F::cols x[2];
@@ -722,15 +734,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
     const int jp = min(jw, kwhole >= koff + 32 ? (kwhole - koff - 32) / C::BN + 1 : 0);
     issue(0);
     int kb = 0;
+    if (jw == 1 && ksome <= 32) {
+        step(0);
+        block(std::true_type{}, std::true_type{}, 0);
+        kb = 1;
+    }
     for (; kb < jp; ++kb) {
         step(kb);
-        block(std::false_type{}, kb);
+        block(std::false_type{}, std::false_type{}, kb);
     }
     for (; kb < jw; ++kb) {
         step(kb);
-        block(std::true_type{}, kb);
+        block(std::true_type{}, std::false_type{}, kb);
     }
     for (; kb < nkb; ++kb) step(kb);
+    if (row < rows && ks == 0 && half == 0) {
+        const int64_t at = (int64_t(kvh) * a.tokens + it.start) * a.group + row;
+        a.ndelta[at] = nd;
+        a.nl2[at] = nl;
+    }
     if constexpr (C::KS > 1) {
         // The key slices' sums join through LDS, the upper half of them added to the lower.
         static_assert(C::KS / 2 * C::RS * C::DT * 16 * kWave * 4 <= C::LDS, "join buffer");
