@@ -490,15 +490,18 @@ packed_dkdv_kernel(BwdArgs a) {
         }
     };
 
+    // Rows from the last to the first that sees the keys: the workgroups of a sequence and key head begin with the
+    // same blocks, which they find in L2 (bf16 d 128, 16.4k tokens, 32/8 heads: 1574 us from the diagonal down, 1515
+    // from the end up).
     auto step = [&](int qb) __attribute__((always_inline)) {
-        const int buf = C::NBUF == 2 ? (qb - qb_first) & 1 : 0;
+        const int buf = C::NBUF == 2 ? (nqb - 1 - qb) & 1 : 0;
         if (C::NBUF == 1) {
             lds_barrier();  // every wave is done with the last block
             issue(qb, 0);
         }
         wait_loads();
         lds_barrier();
-        if (C::NBUF == 2 && qb + 1 < nqb) issue(qb + 1, buf ^ 1);
+        if (C::NBUF == 2 && qb > qb_first) issue(qb - 1, buf ^ 1);
         return buf;
     };
     // This wave's blocks, in loops without branches inside (one loop over both variants makes the
@@ -517,22 +520,22 @@ packed_dkdv_kernel(BwdArgs a) {
         qp = min(max(qp, qa), qn);
         qe = min(max(qe, qp), qn);
     }
-    if (C::NBUF == 2) issue(qb_first, 0);  // the tile's first key is in the sequence: qb_first < nqb
-    int qb = qb_first;
-    for (; qb < qa; ++qb) step(qb);
-    for (; qb < qp; ++qb) {
+    if (C::NBUF == 2) issue(nqb - 1, 0);  // the tile's first key is in the sequence: qb_first < nqb
+    int qb = nqb - 1;
+    for (; qb >= qn; --qb) step(qb);
+    for (; qb >= qe; --qb) {
         const int buf = step(qb);
         block(std::true_type{}, qb * C::BM + 32 * rs, buf);
     }
-    for (; qb < qe; ++qb) {
+    for (; qb >= qp; --qb) {
         const int buf = step(qb);
         block(std::false_type{}, qb * C::BM + 32 * rs, buf);
     }
-    for (; qb < qn; ++qb) {
+    for (; qb >= qa; --qb) {
         const int buf = step(qb);
         block(std::true_type{}, qb * C::BM + 32 * rs, buf);
     }
-    for (; qb < nqb; ++qb) step(qb);
+    for (; qb >= qb_first; --qb) step(qb);
 
     // The row slices' sums join through LDS, the upper half of them added to the lower.
     float *red = reinterpret_cast<float *>(smem);
