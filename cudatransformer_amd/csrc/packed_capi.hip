@@ -75,7 +75,6 @@ struct Sides {
     const PackedStride *s;
 };
 
-// Strides as the caller gives them: (row, head) pairs.  Kernels form 64-bit offsets from them.
 int check_call(const char *fn, int dtype, const void *plan_host, const void *plan, int64_t rows, int64_t hq,
                int64_t hkv, int64_t d, const int64_t *strides, PackedCall &c) {
     if (dtype != CTATTN_F32 && dtype != CTATTN_BF16 && dtype != CTATTN_F16 && dtype != CTATTN_F64)
@@ -148,6 +147,16 @@ bool may_overlap(const Bytes &a, const Bytes &b) {
 
 int64_t elem_bytes(int dtype) { return dtype == CTATTN_F64 ? 8 : dtype == CTATTN_F32 ? 4 : 2; }
 
+// A stride that is never stepped along (one head, one token) may hold anything: 0, so that it decides nothing.
+void settle(PackedCall &c) {
+    const int64_t heads[] = {c.hq, c.hkv, c.hkv, c.hq, c.hq, c.hq, c.hkv, c.hkv};
+    PackedStride *const all[] = {&c.sq, &c.sk, &c.sv, &c.so, &c.sdo, &c.sdq, &c.sdk, &c.sdv};
+    for (int i = 0; i < 8; ++i) {
+        if (heads[i] == 1) all[i]->head = 0;
+        if (c.tokens() <= 1) all[i]->row = 0;
+    }
+}
+
 // The MFMA kernels move 16 bytes per access: pointers and strides on 16 bytes.
 bool on16(const Sides &x, int dtype) {
     const int64_t e = elem_bytes(dtype);
@@ -215,6 +224,7 @@ int ctattn_packed_fwd(int dtype, const void *q, const void *k, const void *v, vo
     c.sk = {strides[2], strides[3]};
     c.sv = {strides[4], strides[5]};
     c.so = {strides[6], strides[7]};
+    settle(c);
     if (c.tokens() == 0) return ok();
     if (int rc = check_outputs(fn, {&c.so}, {hq}, c.tokens(), d)) return rc;
     if (!q || !k || !v || !o) return fail(hipErrorInvalidValue, "%s: null q/k/v/o pointer", fn);
@@ -234,11 +244,8 @@ int ctattn_packed_fwd(int dtype, const void *q, const void *k, const void *v, vo
 
 int64_t ctattn_packed_bwd_workspace_bytes(int dtype, const void *plan_host, int64_t hq, int64_t hkv, int64_t d) {
     PackedCall c{};
-    const int64_t none[16] = {};
-    const int64_t dummy = 0;
-    const PackedHeader *h = static_cast<const PackedHeader *>(plan_host);
-    if (check_call("ctattn_packed_bwd_workspace_bytes", dtype, plan_host, &dummy, h ? h->tokens : 0, hq, hkv, d, none, c) != 0)
-        return -1;
+    const int64_t any[16] = {};  // strides and rows play no part
+    if (check_call("ctattn_packed_bwd_workspace_bytes", dtype, plan_host, any, kMaxRows, hq, hkv, d, any, c) != 0) return -1;
     return scratch_bytes(c);
 }
 
@@ -252,6 +259,7 @@ int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, co
     c.causal = causal != 0;
     PackedStride *const to[] = {&c.sq, &c.sk, &c.sv, &c.so, &c.sdo, &c.sdq, &c.sdk, &c.sdv};
     for (int i = 0; i < 8; ++i) *to[i] = {strides[2 * i], strides[2 * i + 1]};
+    settle(c);
     if (c.tokens() == 0) return ok();
     if (int rc = check_outputs(fn, {&c.sdq, &c.sdk, &c.sdv}, {hq, hkv, hkv}, c.tokens(), d)) return rc;
     if (!q || !k || !v || !o || !dout || !lse || !dq || !dk || !dv)

@@ -201,7 +201,8 @@ def flash_attn_packed_bwd(q, k, v, o, do, lse, plan, causal: bool = False, dq=No
 def _ready(t):
     """`t`, or a copy of it where a head is not contiguous or rows lie off the 16 bytes of the fast kernels."""
     e = t.element_size()
-    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and t.stride(0) * e % 16 == 0 and t.stride(1) * e % 16 == 0:
+    on16 = all(n <= 1 or step * e % 16 == 0 for n, step in zip(t.shape[:2], t.stride()[:2]))
+    if t.stride(2) == 1 and t.data_ptr() % 16 == 0 and on16:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

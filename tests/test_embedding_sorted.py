@@ -163,6 +163,33 @@ def test_graph():
 
 
 @gpu
+def test_offsets_past_32_bits():
+    """A table of 2.3e9 elements."""
+    vocab, d = 70000, 33000
+    ids = torch.tensor([69999, 3, 69999, 66000], dtype=torch.int32, device="cuda")
+    dout = torch.randn((4, d), generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    grad = ct.embedding_grad(ids, dout, vocab)
+    rows = torch.tensor([69999, 3, 66000], device="cuda")
+    assert torch.equal(grad[rows[1:]], dout[[1, 3]])
+    assert torch.equal(grad[69999], (dout[0].float() + dout[2].float()).bfloat16())
+    assert torch.equal(ct.embedding_lookup(ids, grad), grad[ids.long()])
+    grad[rows] = 0
+    assert not any(bool(part.any()) for part in grad.split(7000))
+
+
+@gpu
+def test_two_streams_at_once():
+    cases = [_case(n, 700, 64, torch.bfloat16, seed=n, spread=3) for n in (3000, 9000)]
+    want = [ct.embedding_grad(i, x, 700) for i, x in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = [ct.embedding_grad(i, x, 700, stream=st) for (i, x), st in zip(cases, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@gpu
 def test_autograd():
     ids = torch.randint(0, 9, (4, 6), device="cuda")
     table = torch.randn((9, 5), dtype=torch.float64, device="cuda", requires_grad=True)

@@ -153,6 +153,25 @@ def test_same_bits_streams_and_graph():
 
 
 @gpu
+def test_two_streams_at_once():
+    xs = [_make((3, 130, 200), torch.float32, seed=1), _make((700, 260), torch.float32, seed=2)]
+    want = [ct.newton_schulz(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        got = [ct.newton_schulz(x, stream=st) for x, st in zip(xs, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1024, 1024), (1100, 1300), (2, 1024, 2048)])
+def test_large_tiles(shape):
+    x = _make(shape, torch.float32, seed=shape[-1])
+    _check_steps(ct.newton_schulz(x), x)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("count", [1, 5, 70])

@@ -446,6 +446,63 @@ def test_streams_and_graph():
 
 
 @gpu
+def test_strides_of_single_heads_and_rows():
+    """One head, or one token: that dimension's stride may be anything."""
+    lens, d = [70, 5], 64
+    x = _inputs(lens, 2, 1, d, torch.bfloat16)
+    plan = ct.packed_plan(lens, 2, 1)
+    want = _run(*x, plan, True)
+    k, v = (t[:, 0].as_strided((75, 1, d), (d, 3, 1)) for t in x[1:3])
+    got = _run(x[0], k, v, x[3], plan, True)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    one = ct.packed_plan([1], 2, 1)
+    y = [t[:1] for t in x]
+    odd = [t.as_strided(t.shape, (7, t.stride(1), 1)) for t in y]
+    a, b = _run(*y, one, True), _run(*odd, one, True)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """Rows 2 MiB apart: the later ones of 4200 lie past 2^32 bytes and 2^32 elements."""
+    lens, hq, hkv, d = [4100, 100], 2, 1, 64
+    n = sum(lens)
+    x = _inputs(lens, hq, hkv, d, torch.bfloat16)
+    plan = ct.packed_plan(lens, hq, hkv)
+    want = _run(*x, plan, True)
+    buf = torch.empty((n, 1 << 20), dtype=torch.bfloat16, device="cuda")
+    parts, at = [], 0
+    for heads in (hq, hkv, hkv, hq, hq, hq, hkv, hkv):  # q k v do o dq dk dv
+        parts.append(buf[:, at:at + heads * d].view(n, heads, d))
+        at += heads * d
+    for t, y in zip(parts, x):
+        t.copy_(y)
+    q, k, v, do, o, dq, dk, dv = parts
+    _, lse = ct.flash_attn_packed_fwd(q, k, v, plan, causal=True, out=o)
+    ct.flash_attn_packed_bwd(q, k, v, o, do, lse, plan, causal=True, dq=dq, dk=dk, dv=dv)
+    got = dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv)
+    assert all(torch.equal(got[name], want[name]) for name in want)
+
+
+@gpu
+def test_two_streams_at_once():
+    lens = [400, 130, 64]
+    plan = ct.packed_plan(lens, 8, 2)
+    xs = [_inputs(lens, 8, 2, 64, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [_run(*x, plan, True) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        got = []
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                got.append(_run(*x, plan, True))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(g[n], w[n]) for n in w)
+
+
+@gpu
 def test_binding_refusals():
     lens = [8, 4]
     plan = ct.packed_plan(lens, 4, 2)
