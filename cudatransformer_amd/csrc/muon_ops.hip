@@ -10,9 +10,9 @@
 // is the sum of two fp16 numbers, hi = fp16(256 x) and lo = fp16(256 x - hi), 22 significant bits, and a
 // product is hi hi + hi lo + lo hi in one fp32 accumulator: three 16-bit MFMAs, what is left out
 // (lo lo) is 2^-22 of the product, below the fp32 sums' own rounding.  fp16's range is enough because X is
-// normalised: |X|, |A| and |B| stay below 255.9, and 256 x keeps lo a normal number down to x of 2^-7
-// of an entry's usual 1 / sqrt(c).  One fp16 term alone would not do: five steps amplify a
-// direction by up to a^5 = 485, and its rounding with it.
+// normalised: |X|, |A| and |B| stay below 255.9, and lo is a normal number down to x = 2^-10 (an entry of X is
+// about 1 / sqrt(c)); below that a factor is off by 2^-33 at most, whatever x.  One fp16 term alone would not
+// do: five steps amplify a direction by up to a^5 = 485, and its rounding with it.
 //
 // Layout: a factor's 128 x 32 blocks lie one behind the other, each a run of 128 rows [32 hi | 32 lo] (128 bytes
 // a row, 16 KiB), so that one K step of a tile is one contiguous read.  A product's 32 x 32
