@@ -76,9 +76,10 @@ class EmbeddingLookupFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, ids, table, scale=1.0):
+        ids = ids.contiguous()
         ctx.save_for_backward(ids)
         ctx.vocab, ctx.scale = table.shape[0], scale
-        return embedding_lookup(ids, table, scale)
+        return embedding_lookup(ids, table.contiguous(), scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable

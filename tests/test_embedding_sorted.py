@@ -200,6 +200,17 @@ def test_autograd():
 
 
 @gpu
+def test_autograd_takes_ids_and_a_table_of_any_order():
+    ids = torch.randint(0, 9, (4, 6), device="cuda").t()
+    leaf = torch.randn((5, 9), dtype=torch.float64, device="cuda", requires_grad=True)
+    dout = torch.randn((5, 6, 4), dtype=torch.float64, device="cuda").permute(1, 2, 0)
+    out = ct.embedding(ids, leaf.t(), 0.5)
+    assert torch.equal(out, 0.5 * leaf.detach().t()[ids])  # a product by a power of two is exact
+    out.backward(dout)
+    _check(leaf.grad.t(), _expected(ids.reshape(-1), dout.reshape(24, 5), 9, 0.5))
+
+
+@gpu
 def test_binding_refusals():
     ids, dout = _case(10, 20, 8, torch.float32)
     table = torch.zeros((20, 8), device="cuda")
