@@ -304,11 +304,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
 
 // ---- backward ----
 
+// fp16 (F::RANGE): P enters dV's product as 2^kPExp P, and dS as es dS with es a power of two of the lane's own row or
+// key, from kDsStart down.  Finite inputs keep |es dS| below 2^(10 + 39 + 50) at the start, inside fp32.
+constexpr int kPExp = 10;
+constexpr float kDsStart = 1125899906842624.f;  // 2^50
+constexpr float kDsLimit = 32768.f;  // a lane's sum of |dS| es over 16 rows or keys below which none passes fp16's range
+
+// The lane's 16 values es dS: where their sum passes the limit, and for every lane of the wave that holds a value from
+// kDsLimit / 16 on, a smaller es, so that the largest of the row or key (lane and lane ^ 32) lies in [2^7, 2^8).  Returns
+// the power of two by which es changes, and with it the values and the sums.
+__device__ __forceinline__ float fit_range(float (&w)[16]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += fabsf(w[r]);
+    if (!__any(!(sum <= kDsLimit))) return 1.f;
+    float top = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(w[r]));
+    top = max_xor32(top);
+    float f = 1.f;
+    // 2^(7 - exponent) from the exponent bits; an infinity or NaN stays what it is.
+    if (top >= kDsLimit / 16 && top < INFINITY) f = __uint_as_float(uint32_t(127 + 7 + 127 - int(__float_as_uint(top) >> 23)) << 23);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] *= f;
+    return f;
+}
+
 struct BwdArgs {
     View q, k, v, o, dout, dq, dk, dv;
     const float *lse;
-    // -delta = -rowsum(dO O) and -L log2(e) of every (token, head), rows (token, head of the group) behind each
-    // other for each key head, as the dK / dV kernel walks them.  The dQ kernel, which has dO's rows in
+    // -delta = -rowsum(dO O) and -L log2(e) (fp16: + kPExp) of every (token, head), rows (token, head of the group) behind
+    // each other for each key head, as the dK / dV kernel walks them.  The dQ kernel, which has dO's rows in
     // registers, runs first and writes them.
     float *ndelta, *nl2;
     const PackedItem *items;
@@ -384,6 +410,7 @@ packed_dkdv_kernel(BwdArgs a) {
     floatx16 dk[C::DT], dv[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
+    float es = kDsStart;  // of the lane's key (fp16)
 
     const uint32_t rq = uint32_t(Tile<C::RB / 2>::off(32 * rs + col, half));
     const uint32_t ak = L + C::K_OFF + uint32_t(Tile<C::RB / 2>::off(32 * ks + col, half));
@@ -461,6 +488,7 @@ packed_dkdv_kernel(BwdArgs a) {
             }
         }
         typename F::pvec pb[2], db[2];
+        [[maybe_unused]] float w[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const floatx4 n4 = lds_f4(anl + 32 * g);
@@ -477,8 +505,19 @@ packed_dkdv_kernel(BwdArgs a) {
                     ds = hidden ? 0.f : ds;
                 }
                 F::put(pb[r / 8], r % 8, p);
-                F::put(db[r / 8], r % 8, ds);
+                if constexpr (F::RANGE) w[r] = ds * es;
+                else F::put(db[r / 8], r % 8, ds);
             }
+        }
+        if constexpr (F::RANGE) {
+            const float f = fit_range(w);
+            if (__any(f != 1.f)) {
+                es *= f;
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt) dk[dt] *= f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) F::put(db[r / 8], r % 8, w[r]);
         }
         constexpr int NS = 2 * C::DT;
         typename F::cols go[2], gq[2];
@@ -545,6 +584,11 @@ packed_dkdv_kernel(BwdArgs a) {
     }
     for (; qb >= qb_first; --qb) step(qb);
 
+    if constexpr (F::RANGE) {
+        const float back = 1.f / (es * float(1 << kPExp));
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt) dk[dt] *= back, dv[dt] *= 1.f / float(1 << kPExp);
+    }
     // The row slices' sums join through LDS, the upper half of them added to the lower.
     float *red = reinterpret_cast<float *>(smem);
 #pragma unroll
@@ -654,6 +698,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
     floatx16 dq[C::DT];
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt) dq[dt] = zero16();
+    // fp16: dS's scale of the lane's row, which P's exponent takes along.
+    float es = F::RANGE ? kDsStart : 1.f;
+    float nls = F::RANGE ? nl + log2f(kDsStart) : nl;
 
     const uint32_t rk = uint32_t(Tile<C::RB / 2>::off(col, half));
     const uint32_t ck0 = F::template col0<C::RB>(lane), ck1 = F::template col1<C::RB>(lane);
@@ -693,6 +740,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
             dp = F::mma(v[cur], gb[st], dp);
         }
         typename F::pvec db[2];
+        [[maybe_unused]] float w[16];
         if constexpr (ALONE) {
             float delta = 0.f;
 #pragma unroll
@@ -706,17 +754,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
             delta += __shfl_xor(delta, 32, kWave);
             nd = row < rows ? -delta : 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) F::put(db[r / 8], r % 8, s[r] * (dp[r] - delta));
+            for (int r = 0; r < 16; ++r) {
+                const float ds = s[r] * (dp[r] - delta);
+                if constexpr (F::RANGE) w[r] = ds * es;
+                else F::put(db[r / 8], r % 8, ds);
+            }
         } else {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float ds = fast_exp2(fmaf(s[r], a.c, nl)) * dp[r];
+                float ds = fast_exp2(fmaf(s[r], a.c, nls)) * dp[r];
                 if (MASK) {
                     const int key = kb * C::BN + koff + acc_row(r, half);
                     ds = (key >= it.len || (a.causal && key > token)) ? 0.f : ds;
                 }
-                F::put(db[r / 8], r % 8, ds);
+                if constexpr (F::RANGE) w[r] = ds;
+                else F::put(db[r / 8], r % 8, ds);
             }
+        }
+        if constexpr (F::RANGE) {
+            const float f = fit_range(w);
+            if (__any(f != 1.f)) {
+                es *= f;
+                nls = nl + log2f(es);
+#pragma unroll
+                for (int dt = 0; dt < C::DT; ++dt) dq[dt] *= f;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) F::put(db[r / 8], r % 8, w[r]);
         }
         constexpr int NS = 2 * C::DT;
         typename F::cols x[2];
@@ -762,7 +826,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
     if (row < rows && ks == 0 && half == 0) {
         const int64_t at = (int64_t(kvh) * a.tokens + it.start) * a.group + row;
         a.ndelta[at] = nd;
-        a.nl2[at] = nl;
+        a.nl2[at] = F::RANGE ? nl + float(kPExp) : nl;
+    }
+    if constexpr (F::RANGE) {
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt) dq[dt] *= 1.f / es;
     }
     if constexpr (C::KS > 1) {
         // The key slices' sums join through LDS, the upper half of them added to the lower.

@@ -12,6 +12,8 @@
 
 #include "attn_bf16_tiles.h"
 
+#include <type_traits>
+
 namespace ctattn {
 namespace packedtile {
 
@@ -22,6 +24,7 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 template <typename H> struct Fmt16 : H {
     static constexpr int ES = 2;
+    static constexpr bool RANGE = std::is_same_v<H, F16Fmt>;  // narrower in exponent than fp32
     using vec = typename H::vec;  // a 16-byte chunk
     using pvec = vec;             // 8 values as a B operand
     using store = uint16_t;
@@ -43,6 +46,7 @@ using PF16 = Fmt16<F16Fmt>;
 
 struct PF32 {
     static constexpr int ES = 4;
+    static constexpr bool RANGE = false;
     using vec = floatx4;
     using pvec = f32x8;
     using store = float;
