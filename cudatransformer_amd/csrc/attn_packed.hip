@@ -7,8 +7,8 @@
 // two buffers); or 32 rows, of whose keys each wave walks a quarter.  Scores are computed
 // transposed, S^T = K Q^T, so that a lane holds one row: the running maximum and sum of the
 // softmax need one exchange with lane ^ 32, and the accumulator registers are, as they stand, the B
-// operand of O^T += V^T P^T.  The maximum is raised only when a block exceeds it by 2^8 (P stays
-// below 2^8, exact to scale in fp32 sums).  P is rounded to 16 bits for the second product (the
+// operand of O^T += V^T P^T.  The maximum is raised only when a block exceeds it by 2^8 (fp16: 2^15; P stays
+// below that, exact to scale in fp32 sums).  P is rounded to 16 bits for the second product (the
 // MFMA's operand type); the sum adds the unrounded values.
 //
 // Backward: P = exp(S - L), dV = P^T dO, dS = P (dO V^T - delta), dQ = dS K, dK = dS^T Q, in two
@@ -36,9 +36,15 @@ namespace {
 
 using namespace packedtile;
 
-constexpr float kRaise = 8.0f;       // raise the running maximum when a block exceeds it by 2^8
 constexpr float kLowest = -3.402823466e38f;  // the running maximum before any score (finite: m - m is 0, not NaN)
-constexpr float kPsumLimit = 256.f;  // a lane's share of a block's P below which no P exceeds 2^8
+// m, the running maximum, is raised when a block exceeds it by 2^8, to the row's maximum.  fp16 (F::RANGE): to 2^7 below
+// it, when a block exceeds it by 2^15, so that P fills the format: its smallest step, 2^-24, is 2^-31 of the row's largest
+// P then, where 2^-24 of it would be lost for every one of a long row's keys.
+template <typename F> struct Rise {
+    static constexpr float UNDER = F::RANGE ? 7.f : 0.f;
+    static constexpr float BY = F::RANGE ? 15.f : 8.f;
+    static constexpr float PSUM = F::RANGE ? 32768.f : 256.f;  // a lane's share of a block's P below which no P exceeds 2^BY
+};
 
 // Byte strides and pointers of one [tokens, heads, d] tensor.
 struct View {
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
             }
         };
         expo();
-        if (__any(!(psum <= kPsumLimit))) {
+        if (__any(!(psum <= Rise<F>::PSUM))) {
             float top = -INFINITY;
 #pragma unroll
             for (int kt = 0; kt < C::KT; ++kt) {
@@ -183,9 +189,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(FwdCfg<F, D
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[kt][r]);
             }
             top = max_xor32(top) * a.c;
-            if (__any(top > m_run + kRaise)) {
+            if (__any(top > m_run + Rise<F>::BY)) {
                 // A row that sees none of the wave's keys yet keeps m at the lowest: P = 2^(-inf) = 0.
-                const float m_new = fmaxf(m_run, top);
+                const float m_new = fmaxf(m_run, top - Rise<F>::UNDER);
                 const float resc = fast_exp2(m_run - m_new);
                 m_run = m_new;
                 l_run *= resc;

@@ -141,3 +141,22 @@ def test_an_infinity_in_one_row_of_do_stays_in_its_row_of_dq():
     dq = ct.flash_attn_packed_bwd(*x[:3], o, x[3], lse, plan, causal=True)[0]
     assert not bool(torch.isfinite(dq[~keep]).any())
     _check(dict(dq=dq[keep]), dict(dq=tuple(t[keep] for t in want["dq"])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,hq,hkv", [([8192], 1, 1), ([4096, 1000], 16, 4), ([700, 33], 4, 2)])
+@pytest.mark.parametrize("gap", [12.0, 16.0, 17.05, 17.6])
+def test_one_key_above_many(gap, lens, hq, hkv, causal):
+    """One key's score lies e^gap above every other's: each of those has a P near or below a subnormal step of fp16, and all
+    of them together make the output."""
+    d, n = 64, sum(lens)
+    q, k, v, _ = _random(lens, hq, hkv, d, seed=5)
+    q, k, v = 0 * q, 0 * k, 1 + 0.1 * v
+    q[:, :, 0] = 8
+    for first in [sum(lens[:i]) for i in range(len(lens))]:
+        k[first, :, 0], v[first] = gap, 0
+    x = [t.to(F16).cuda() for t in (q, k, v)]
+    o, _ = ct.flash_attn_packed_fwd(*x, ct.packed_plan(lens, hq, hkv), causal=causal)
+    # P's rounding in the forward: 2^-32, half a subnormal step where the row's largest P is held at 2^7 or above.
+    _check(dict(o=o), _reference(*x, torch.zeros_like(x[0]), lens, causal, eta_o=2.0 ** -32))
