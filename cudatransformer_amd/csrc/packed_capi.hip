@@ -145,6 +145,12 @@ bool may_overlap(const Bytes &a, const Bytes &b) {
     return !(a.span <= shift && shift + b.span <= a.row);
 }
 
+// `n` bytes from p on, whole.
+Bytes run_of(const void *p, int64_t n) {
+    const intptr_t at = reinterpret_cast<intptr_t>(p);
+    return {at, at + n, 0, 0};
+}
+
 int64_t elem_bytes(int dtype) { return dtype == CTATTN_F64 ? 8 : dtype == CTATTN_F32 ? 4 : 2; }
 
 // A stride that is never stepped along (one head, one token) may hold anything: 0, so that it decides nothing.
@@ -161,6 +167,10 @@ void settle(PackedCall &c) {
 bool on16(const Sides &x, int dtype) {
     const int64_t e = elem_bytes(dtype);
     return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.s->row * e) % 16 == 0 && (x.s->head * e) % 16 == 0;
+}
+
+Bytes lse_bytes(const void *lse, const PackedCall &c) {
+    return run_of(lse, c.tokens() * c.hq * (c.dtype == CTATTN_F64 ? 8 : 4));
 }
 
 bool mfma(const PackedCall &c) {
@@ -238,9 +248,13 @@ int ctattn_packed_fwd(int dtype, const void *q, const void *k, const void *v, vo
     if (!q || !k || !v || !o) return fail(hipErrorInvalidValue, "%s: null q/k/v/o pointer", fn);
     const int64_t es = elem_bytes(dtype);
     const Bytes bo = bytes_of(o, c.so, c.tokens(), hq, d, es);
-    if (may_overlap(bo, bytes_of(q, c.sq, c.tokens(), hq, d, es)) || may_overlap(bo, bytes_of(k, c.sk, c.tokens(), hkv, d, es)) ||
-        may_overlap(bo, bytes_of(v, c.sv, c.tokens(), hkv, d, es)))
-        return fail(hipErrorInvalidValue, "%s: o lies on an input's memory", fn);
+    const Bytes in[] = {bytes_of(q, c.sq, c.tokens(), hq, d, es), bytes_of(k, c.sk, c.tokens(), hkv, d, es),
+                        bytes_of(v, c.sv, c.tokens(), hkv, d, es)};
+    for (const Bytes &b : in) {
+        if (may_overlap(bo, b)) return fail(hipErrorInvalidValue, "%s: o lies on an input's memory", fn);
+        if (lse && may_overlap(lse_bytes(lse, c), b)) return fail(hipErrorInvalidValue, "%s: lse lies on an input's memory", fn);
+    }
+    if (lse && may_overlap(lse_bytes(lse, c), bo)) return fail(hipErrorInvalidValue, "%s: lse lies on o's memory", fn);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Sides all[] = {{q, &c.sq}, {k, &c.sk}, {v, &c.sv}, {o, &c.so}};
     const bool fast = mfma(c) && std::all_of(std::begin(all), std::end(all), [&](const Sides &x) { return on16(x, dtype); });
@@ -274,7 +288,7 @@ int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, co
         return fail(hipErrorInvalidValue, "%s: null tensor pointer", fn);
     const int64_t es = elem_bytes(dtype), n = c.tokens();
     const Bytes in[] = {bytes_of(q, c.sq, n, hq, d, es),  bytes_of(k, c.sk, n, hkv, d, es), bytes_of(v, c.sv, n, hkv, d, es),
-                        bytes_of(o, c.so, n, hq, d, es),  bytes_of(dout, c.sdo, n, hq, d, es)};
+                        bytes_of(o, c.so, n, hq, d, es),  bytes_of(dout, c.sdo, n, hq, d, es), lse_bytes(lse, c)};
     const Bytes out[] = {bytes_of(dq, c.sdq, n, hq, d, es), bytes_of(dk, c.sdk, n, hkv, d, es), bytes_of(dv, c.sdv, n, hkv, d, es)};
     for (int i = 0; i < 3; ++i) {
         for (const Bytes &b : in)
@@ -288,6 +302,10 @@ int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, co
                     (long long)workspace_bytes, (long long)need);
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return fail(hipErrorInvalidValue, "%s: workspace must be 16-byte aligned", fn);
+    const Bytes ws = run_of(workspace, need);
+    const auto on_ws = [&](const Bytes &b) { return may_overlap(ws, b); };
+    if (std::any_of(std::begin(in), std::end(in), on_ws) || std::any_of(std::begin(out), std::end(out), on_ws))
+        return fail(hipErrorInvalidValue, "%s: workspace lies on a tensor's memory", fn);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Sides all[] = {{q, &c.sq}, {k, &c.sk}, {v, &c.sv}, {o, &c.so}, {dout, &c.sdo}, {dq, &c.sdq}, {dk, &c.sdk}, {dv, &c.sdv}};
     const bool fast = mfma(c) && std::all_of(std::begin(all), std::end(all), [&](const Sides &x) { return on16(x, dtype); });

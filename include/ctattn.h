@@ -604,8 +604,8 @@ CTATTN_API int ctattn_packed_plan(const int64_t *seqlens, int64_t nseq, int64_t 
  * CTATTN_F64, else fp32; may be NULL).  q and o are [rows, Hq, d], k and v [rows, Hkv, d], rows >=
  * the plan's tokens; rows behind the last sequence are neither read nor written.  `strides` (HOST)
  * holds, in elements, the row and the head stride of q, k, v and o; the d elements of a head are
- * contiguous.  No output may share memory with an input or another output (slices of one row-major buffer, a
- * projection's q, k and v, do not; others are refused).
+ * contiguous.  No output, lse among them, may share memory with an input or another output (slices of one row-major
+ * buffer, a projection's q, k and v, do not; others are refused).
  *   - bf16, fp16 (d a multiple of 8) and fp32 (a multiple of 4) run on MFMA kernels for d <= 128 and
  *     Hq / Hkv <= 128 when pointers and strides are multiples of 16 bytes; other calls, f64, and every
  *     call under CTATTN_POLICY_GENERIC take generic kernels (same results, much slower).
@@ -626,7 +626,8 @@ CTATTN_API int64_t ctattn_packed_bwd_workspace_bytes(int dtype, const void *plan
  * over the query heads that share a key head.  They are overwritten in rows 0 .. tokens - 1 and left
  * alone behind them.  `strides` holds the row and head strides of q, k, v, o, dout, dq, dk, dv.  No
  * atomics: the same inputs give the same bits.  The workspace (16-byte aligned) is scratch, free
- * again when the stream has passed the call.
+ * again when the stream has passed the call.  No gradient may share memory with an input or another gradient, nor the
+ * workspace with any tensor (refused as in the forward).
  */
 CTATTN_API int ctattn_packed_bwd(int dtype, const void *q, const void *k, const void *v, const void *o,
                                  const void *dout, const void *lse, void *dq, void *dk, void *dv, void *workspace,
