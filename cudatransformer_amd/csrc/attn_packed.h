@@ -71,6 +71,7 @@ hipError_t launch_packed_generic_bwd(const PackedCall &c, const void *q, const v
 
 // ---- MFMA kernels: fp32, bf16, fp16; d whole 16-byte chunks up to 128; base pointers and row and head
 // strides of q, k, v, o, dout on 16 bytes, of dq, dk, dv on 16 bytes too.  lse may be NULL in the forward. ----
+constexpr int64_t kMfmaMaxGroup = 128;
 bool packed_mfma_supported(int dtype, int64_t d, int64_t group);
 int64_t packed_bwd_scratch_bytes(const PackedCall &c);
 hipError_t launch_packed_fwd(const PackedCall &c, const void *q, const void *k, const void *v, void *o, float *lse,

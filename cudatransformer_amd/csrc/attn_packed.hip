@@ -346,7 +346,9 @@ struct BwdArgs {
     const PackedItem *items;
     int64_t tokens;
     int hkv, group, causal, width;
-    uint32_t magic;  // ceil(65536 / group): x / group = x magic >> 16 for x < 64 + group, group <= 128
+    // ceil(65536 / group): x / group = x magic >> 16 while x (group - 1) < 65536, as magic group exceeds 65536 by less than
+    // group (KvCfg asserts it of every tile and group).
+    uint32_t magic;
     float c, inv_sqrt_d;
 };
 
@@ -371,6 +373,7 @@ template <typename F, int D, typename W> struct KvCfg : W {
     static constexpr int S_OFF = V_OFF + (KREG ? 0 : KB);  // buffer b: nl2[BM], ndelta[BM]
     static constexpr int LDS = S_OFF + W::NBUF * 2 * BM * 4;
     static_assert(LDS <= 160 * 1024, "LDS");
+    static_assert((BM + kMfmaMaxGroup - 2) * (kMfmaMaxGroup - 1) < 65536, "rows of a tile by BwdArgs::magic");
     static constexpr int WPE = NW >= 8 || LDS <= 80 * 1024 ? 2 : 1;
     static_assert(W::KS * W::RS / 2 * DT * 2 * 16 * kWave * 4 <= LDS, "reduction buffer");
 };
@@ -991,7 +994,7 @@ struct BwdCall {
 
 bool packed_mfma_supported(int dtype, int64_t d, int64_t group) {
     if (dtype != 0 && dtype != 1 && dtype != 2) return false;
-    return d >= 1 && d <= 128 && d % (dtype == 0 ? 4 : 8) == 0 && group <= 128;
+    return d >= 1 && d <= 128 && d % (dtype == 0 ? 4 : 8) == 0 && group <= kMfmaMaxGroup;
 }
 
 int64_t packed_bwd_scratch_bytes(const PackedCall &c) { return c.tokens() * c.hq * 2 * int64_t(sizeof(float)); }
