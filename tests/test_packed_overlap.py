@@ -62,3 +62,19 @@ def test_gradients_lie_on_no_lse_and_the_workspace_on_nothing(dtype):
         for ws in (apart[i], apart[i] + (size - 1) // 16 * 16, apart[i] + 16 - (need + 15) // 16 * 16):
             rc, said, _ = _bwd(plan, apart, dtype, ws=ws)
             assert rc == 1 and "workspace lies on" in said, (i, ws)
+
+
+def test_slices_of_one_buffer():
+    """q and o as slices of one row-major buffer are refused where they are shifted onto each other within the rows."""
+    lib, plan = _capi.load(), _plan()
+    host, es, row = plan._host.data_ptr(), 2, 2 * HQ * D
+
+    def call(o_at):
+        st = (ctypes.c_int64 * 8)(row, D, HKV * D, D, HKV * D, D, row, D)
+        rc = lib.ctattn_packed_fwd(1, BIG, 4 * BIG, 5 * BIG, BIG + es * o_at, None, st, host, 64, ROWS, HQ, HKV, D, 1, None)
+        return rc, _capi.last_error()
+
+    # One element into q's part of a row, at either end, and half of the part.
+    for o_at in (0, 1, HQ * D - 1, HQ * D // 2, HQ * D + 1, row - 1, -1, 1 - HQ * D):
+        rc, said = call(o_at)
+        assert rc == 1 and "input's memory" in said, o_at
