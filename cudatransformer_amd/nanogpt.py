@@ -67,14 +67,17 @@ class Attention(nn.Module):
     def forward_packed(self, x, plan):
         """x [tokens, d_model], documents behind each other; each attends to itself."""
         n = x.shape[0]
-        q, k, v = (f(x).view(n, -1, self.head_dim) for f in (self.q, self.k, self.v))
+        q = self.q(x).view(n, self.n_heads, self.head_dim)
+        k, v = (f(x).view(n, self.n_kv_heads, self.head_dim) for f in (self.k, self.v))
         if self.attention == "ctattn":
             o = flash_attention_packed(q, k, v, plan, self.causal)
         else:
             group = self.n_heads // self.n_kv_heads
             k, v = (y.repeat_interleave(group, dim=1) for y in (k, v))
-            parts = zip(*(y.transpose(0, 1).split(plan.seqlens, dim=1) for y in (q, k, v)))
-            o = torch.cat([F.scaled_dot_product_attention(*p, is_causal=self.causal) for p in parts], dim=1).transpose(0, 1)
+            q, k, v = (y.transpose(0, 1) for y in (q, k, v))
+            parts = zip(*(y.split(plan.seqlens, dim=1) for y in (q, k, v)))
+            o = [F.scaled_dot_product_attention(*p, is_causal=self.causal) for p in parts if p[0].shape[1] > 0]
+            o = torch.cat([q[:, :0], *o], dim=1).transpose(0, 1)
         return self.o(o.reshape(n, self.n_heads * self.head_dim))
 
     def forward(self, x, plan=None):
@@ -82,8 +85,8 @@ class Attention(nn.Module):
             return self.forward_packed(x, plan)
         b, t, _ = x.shape
         # [B, T, H*d] -> [B, H, T, d]: the layout attention_qkv_kernels.cu:112-120 writes.
-        split = lambda y: y.view(b, t, -1, self.head_dim).transpose(1, 2).contiguous()  # noqa: E731
-        q, k, v = split(self.q(x)), split(self.k(x)), split(self.v(x))
+        split = lambda y, heads: y.view(b, t, heads, self.head_dim).transpose(1, 2).contiguous()  # noqa: E731
+        q, k, v = split(self.q(x), self.n_heads), split(self.k(x), self.n_kv_heads), split(self.v(x), self.n_kv_heads)
         if self.n_kv_heads != self.n_heads:
             k, v = (y.repeat_interleave(self.n_heads // self.n_kv_heads, dim=1) for y in (k, v))
         if self.attention == "ctattn":
@@ -231,7 +234,8 @@ def make_packed_batch(seqlens, vocab, seed: int):
     token predicts one more."""
     g = torch.Generator().manual_seed(seed)
     docs = [torch.randint(0, vocab, (n + 1,), generator=g) for n in seqlens]
-    return torch.cat([d[:-1] for d in docs]), torch.cat([d[1:] for d in docs])
+    none = torch.empty(0, dtype=torch.int64)  # a batch without documents is one
+    return torch.cat([none] + [d[:-1] for d in docs]), torch.cat([none] + [d[1:] for d in docs])
 
 
 def muon_parameters(model):
