@@ -115,6 +115,14 @@ class Block(nn.Module):
         return self.fc2(self.act(self.fc1(self.ln2(x))))
 
 
+class TokenTable(nn.Embedding):
+    """nn.Embedding; with a scale the lookup and its gradient run on the ctattn kernels (embedding.embedding), where an
+    id outside the table gives zeros and no gradient."""
+
+    def forward(self, ids, scale=None):
+        return super().forward(ids) if scale is None else embedding(ids, self.weight, scale)
+
+
 class NanoGPT(nn.Module):
     def __init__(self, vocab, max_seq_len, d_model, n_heads, head_dim, mlp_dim, n_layers,
                  causal=True, attention="ctattn", activation="gelu", n_kv_heads=None, embedding_scale=1.0, **_):
@@ -129,7 +137,7 @@ class NanoGPT(nn.Module):
         if embedding_scale != 1.0:
             self.config["embedding_scale"] = embedding_scale
         self.attention, self.embedding_scale = attention, embedding_scale
-        self.tok = nn.Embedding(vocab, d_model)
+        self.tok = TokenTable(vocab, d_model)
         self.pos = nn.Embedding(max_seq_len, d_model)
         self.blocks = nn.ModuleList(
             Block(d_model, n_heads, head_dim, mlp_dim, causal, attention, activation, n_kv_heads) for _ in range(n_layers))
@@ -151,7 +159,8 @@ class NanoGPT(nn.Module):
 
     def forward(self, ids, plan=None):
         """Logits of ids [B, T], or with a plan (packed.packed_plan) of ids [tokens], whole documents behind
-        each other: positions restart with each and none attends to another."""
+        each other: positions restart with each and none attends to another.  An id outside the vocabulary is an error of
+        the dense path; the packed one on the ctattn kernels embeds it as zeros, as a padding id."""
         if plan is None:
             positions = torch.arange(ids.shape[1], device=ids.device)
         else:
@@ -161,7 +170,7 @@ class NanoGPT(nn.Module):
                 raise ValueError(f"a document of {max(plan.seqlens)} tokens, {self.config['max_seq_len']} at most")
             positions = plan.positions(ids.device)
         if plan is not None and self.attention == "ctattn":
-            x = embedding(ids, self.tok.weight, self.embedding_scale)
+            x = self.tok(ids, self.embedding_scale)
         else:
             x = self.tok(ids)
             if self.embedding_scale != 1.0:
