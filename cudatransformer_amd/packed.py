@@ -63,12 +63,21 @@ class PackedPlan:
         return out
 
     def positions(self, device=None):
-        """int64 [tokens]: each token's position in its sequence (made on first use for a device, then kept)."""
+        """int64 [tokens]: each token's position in its sequence (made on first use for a device, then kept; before a
+        graph's capture, not in it)."""
         device = self.device if device is None else torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
         if device not in self._positions:
+            if capturing:
+                raise RuntimeError("PackedPlan.positions: made before a graph's capture, not in it")
             p = torch.cat([torch.arange(n) for n in self.seqlens]) if self.seqlens else torch.empty(0, dtype=torch.int64)
             self._positions[device] = p.to(device)
-        return self._positions[device]
+        p = self._positions[device]
+        if p.is_cuda and not capturing:  # the memory goes back when this stream, too, has passed what reads it
+            p.record_stream(torch.cuda.current_stream(device))
+        return p
 
     def _pointers(self, handle: int):
         if handle != self._stream:
