@@ -7,6 +7,7 @@ batch's plan from its lengths, once for all layers and both directions.
 from __future__ import annotations
 
 import ctypes
+import operator
 
 import torch
 
@@ -26,7 +27,10 @@ class PackedPlan:
             if seqlens.dim() != 1 or seqlens.is_floating_point() or seqlens.dtype == torch.bool:
                 raise ValueError("packed_plan: seqlens must be a list or a 1-D integer tensor")
             seqlens = seqlens.tolist()
-        self.seqlens = tuple(int(n) for n in seqlens)
+        try:
+            self.seqlens = tuple(operator.index(n) for n in seqlens)
+        except TypeError:
+            raise ValueError("packed_plan: seqlens must be whole numbers") from None
         self.tokens = sum(self.seqlens)
         self.group = num_heads // num_kv_heads
         lib = load()
