@@ -177,7 +177,9 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
                                                    const double *__restrict__ part, int blocks,
                                                    char *__restrict__ xt, int64_t bytes) {
     __shared__ __attribute__((aligned(1024))) char smem[4 * 8192];
+    // 256 / (|G| + eps) = inv_s 2^exp_s: by itself it may lie outside fp32 where every 256 X is inside.
     __shared__ float inv_s;
+    __shared__ int exp_s;
     __shared__ double sums[4];
     const int mat = blockIdx.z, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     {
@@ -186,10 +188,16 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
         ss = wave_sum(ss);
         if (lane == 0) sums[wave] = ss;
         __syncthreads();
-        if (threadIdx.x == 0) inv_s = float(double(kScale) / (sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + eps));
+        if (threadIdx.x == 0) {
+            const double x = double(kScale) / (sqrt((sums[0] + sums[1]) + (sums[2] + sums[3])) + eps);
+            int e = 0;
+            inv_s = x < double(INFINITY) ? float(frexp(x, &e)) : float(x);  // G = 0 without an eps: 0 times an infinity
+            exp_s = e;
+        }
     }
     __syncthreads();
     const float inv = inv_s;
+    const int inv_e = exp_s;
     const T *gp = g.at<const T>(mat);
     const float *mp = u.muon ? m.at<const float>(mat) : nullptr;
     // G's padded shape; its row blocks in y, four column blocks a workgroup in x.
@@ -215,7 +223,8 @@ __global__ __launch_bounds__(256) void split_kernel(Mats g, Mats m, Update u, Sh
             for (int e = 0; e < 4; ++e)
                 if (j + e < s.cols) v[e] = update_value(u, gp, mp, at + e);
         }
-        v = v * inv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ldexpf(v[e], inv_e) * inv;
         const Four f = split4(v);
         block_put4(blk, line, c, f);
     }
