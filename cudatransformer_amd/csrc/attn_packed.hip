@@ -18,11 +18,12 @@
 // alternative, dQ by atomics, is bound by their rate and not reproducible.  dS is rounded to 16
 // bits as an operand, as P is.
 //
-// Measured (causal): bf16 d 128, 16.4k tokens in 5 sequences, 32/8 heads: forward 786 us (955
-// TFLOP/s), dQ 1075, dK / dV 1510, matrix cores 50 to 55 % busy beside the exponentials.  bf16 d 64,
-// 13.8k tokens in 26, 16/4 heads: 79, 108, 172 us, 26 to 29 % busy, vector work for half as many
-// products.  fp32 d 64, 4.1k tokens in 13, 6/6 heads: 36, 51, 68 us, waves waiting half of the time on
-// a grid of one or two workgroups a CU.
+// Measured (causal; two cards where they differ): bf16 d 128, 16.4k tokens in 5 sequences, 32/8 heads: forward 738 to
+// 827 us (1017 to 907 TFLOP/s), dQ 1017 to 1138, dK / dV 1406 to 1576, matrix cores 49 to 55 % busy beside the
+// exponentials.  bf16 d 64, 14.7k tokens in 26, 16/4 heads: 77 to 82, 105 to 113, 161 to 176 us, 26 to 30 % busy, vector
+// work for half as many products.  fp32 d 64, 4.1k tokens in 13, 6/6 heads: 36, 50, 67 us, waves waiting half of the
+// time on a grid of one or two workgroups a CU.  fp16's scales of dS: 3.4 % of forward and backward (the bf16 cases in
+// fp16 without / with them 317 / 328 us and 3401 / 3514).
 #include "attn_launch.h"
 #include "attn_packed.h"
 #include "attn_packed_tiles.h"
@@ -886,7 +887,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(QCfg<F, D, 
 // batch's pairs make fewer than a quarter of as many blocks of `pairs_of_block` for each of the `slots` workgroups that
 // the chip holds at once.  Then smaller tiles, whose waves share the walk, win; else larger ones, which load less for a
 // pair.  Measured, us, causal, larger / smaller tiles, with the ratio:
-//   forward  bf16 d 64: 26 documents of 13.8k tokens, 16/4 heads (1.1) 78 / 155; 8 x 512 16/4 (2) 14 / 25; 4096 4/2 (8)
+//   forward  bf16 d 64: 26 documents of 14.7k tokens, 16/4 heads (1.1) 78 / 155; 8 x 512 16/4 (2) 14 / 25; 4096 4/2 (8)
 //            55 / 28.  d 128: 8192 8/2 (2) 200 / 254; 2048 8/2 (8) 44 / 29.  fp32 d 64: 13 documents of 4k tokens, 6/6 (9)
 //            76 / 36; 16 x 512 12/12 (1.3) 83 / 108.  fp32 d 128: 4 x 1024 8/2 (4) 153 / 104
 //   dK, dV   (whole backward) bf16 d 64: the 26 documents (4.5) 328 / 275; 8 x 512 16/4 (8) 68 / 49; 4096 4/2 (16) 211 /

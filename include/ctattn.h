@@ -158,6 +158,9 @@ CTATTN_API int64_t ctattn_bwd_workspace_bytes_max(int dtype, int64_t B, int64_t 
  * dS tiles (the error message names the minimum).  With a workspace that holds the dS tiles
  * dQ = dS K reads them back; else bf16 / fp16 dQ recomputes S and dP (the same results up to
  * bf16 rounding of dS) and fp32 takes the policy's other dQ scheme.
+ * fp16 at d <= 128 holds P and dS = P (dO V^T - delta) as fp16 numbers as they are: a |dS| above 65504 becomes infinite,
+ * P and dS below 2^-14 have fewer bits and below 2^-25 none (dO of 4e-6 on rows of 2048 keys: dQ and dK off by 5 %), so
+ * dout should be scaled to its largest values near one or above.  (ctattn_packed_bwd and d above 128 scale dS themselves.)
  * Reproducibility depends on the policy (see enum ctattn_policy).
  */
 CTATTN_API int ctattn_bwd(int dtype, const void *q, const void *k, const void *v, const void *o,
@@ -608,7 +611,11 @@ CTATTN_API int ctattn_packed_plan(const int64_t *seqlens, int64_t nseq, int64_t 
  * buffer, a projection's q, k and v, do not; others are refused).
  *   - bf16, fp16 (d a multiple of 8) and fp32 (a multiple of 4) run on MFMA kernels for d <= 128 and
  *     Hq / Hkv <= 128 when pointers and strides are multiples of 16 bytes; other calls, f64, and every
- *     call under CTATTN_POLICY_GENERIC take generic kernels (same results, much slower).
+ *     call under CTATTN_POLICY_GENERIC take generic kernels, much slower.  The MFMA kernels of the 16-bit types
+ *     round P to the type as an operand of P V (and P and dS in the backward), which the generic ones keep in fp32: in
+ *     bf16 O, dQ, dK and dV are off by 2.0e-3 to 2.4e-3 of their norm where the outputs' rounding alone makes
+ *     1.6e-3 to 1.7e-3.  fp16 scales P and dS by powers of two: its smallest step is at most 2^-31 of the largest P
+ *     or dS of the row or key.  Sums and LSE are fp32 in both.
  *   - a NaN or an infinity in a sequence's keys or values may reach any row of that sequence and head
  *     group, and no other sequence.
  */
@@ -668,7 +675,10 @@ CTATTN_API int ctattn_embedding_grad(int dtype, int id_dtype, const void *ids, c
  * x): X = G / (|G|_F + eps), then `steps` (1 .. 100) times X <- a X + (b X X^T + c (X X^T)^2) X, products on
  * the shorter side.  With a = 3.4445, b = -4.7750, c = 2.0315 five steps bring every singular value that is
  * not tiny near one.  dtype f32, bf16 or f16 (storage; f64 is refused); the iteration itself runs in
- * fp32 precision whatever the storage (factors of 22 significant bits, fp32 sums) and is rounded once.
+ * fp32 precision whatever the storage (factors of 22 significant bits, fp32 sums) and is rounded once.  Factors'
+ * elements below 2^-10 (of X, whose norm starts at one) have an absolute error of up to 2^-33 instead: nothing to the norm
+ * of the result, but a row of G 1e-5 as large as the strongest comes out off by about 5e-4 of its own norm, where
+ * fp32 products give 4e-5.
  * Coefficients up to 64 in absolute value; an iteration whose values pass 255 ends in infinities or NaN, as
  * do a NaN or an infinity in G for its matrix.  No atomics: the same inputs give the same bits.  The workspace
  * (256-byte aligned) is scratch.  No counterpart in the reference.
