@@ -5,6 +5,8 @@ Layers of this package
   * ``cuda_transformer`` -- C++ host module (pybind11) mirroring the reference's
     ``Tensor`` / ``FlashAttentionLayer`` API on top of that C-ABI.
   * ``packed``         -- attention on packed sequences of different lengths.
+  * ``paged``          -- a paged key / value cache and attention of requests that share a prompt.
+  * ``sampling``       -- next tokens by temperature, top-k, top-p and min-p.
   * ``embedding``      -- scaled token lookup with a reproducible gradient.
   * ``muon``           -- Newton-Schulz orthogonalisation and the Muon step.
   * ``_capi``          -- ctypes binding of the same C-ABI over torch device tensors
@@ -51,6 +53,15 @@ from .packed import (  # noqa: E402
     packed_bwd_workspace_bytes,
     packed_plan,
 )
+from .paged import (  # noqa: E402
+    cache_write,
+    flash_attn_shared_prefix,
+    page_pool,
+    page_release,
+    page_reserve,
+    shared_prefix_workspace_bytes,
+)
+from .sampling import sample_tokens, sample_workspace_bytes  # noqa: E402
 
 __all__ = [
     "BF16",
@@ -64,6 +75,7 @@ __all__ = [
     "PackedAttentionFunction",
     "PackedPlan",
     "bwd_workspace_bytes",
+    "cache_write",
     "embedding",
     "embedding_grad",
     "embedding_grad_workspace_bytes",
@@ -74,11 +86,18 @@ __all__ = [
     "flash_attn_fwd",
     "flash_attn_packed_bwd",
     "flash_attn_packed_fwd",
+    "flash_attn_shared_prefix",
     "muon_update",
     "newton_schulz",
     "newton_schulz_workspace_bytes",
     "packed_bwd_workspace_bytes",
     "packed_plan",
+    "page_pool",
+    "page_release",
+    "page_reserve",
+    "sample_tokens",
+    "sample_workspace_bytes",
+    "shared_prefix_workspace_bytes",
     "out_proj_bwd",
     "out_proj_fwd",
     "qkv_proj_bwd",

@@ -135,6 +135,13 @@ def load() -> ctypes.CDLL:
         "ctattn_muon_update_workspace_bytes": ([c_int] + [i64] * 3, i64),
         "ctattn_muon_update_multi": ([c_int, c_int] + [vp] * 4 + [i64] * 3 + [f64] * 2 + [c_int] + [f64] * 2 + [c_int]
                                      + [f64] * 4 + [vp], c_int),
+        "ctattn_page_reserve": ([vp] * 11 + [i64] * 6 + [vp], c_int),
+        "ctattn_page_release": ([vp] * 7 + [i64] * 5 + [vp], c_int),
+        "ctattn_cache_write": ([c_int] + [vp] * 6 + [i64] * 5 + [vp], c_int),
+        "ctattn_shared_prefix_workspace_bytes": ([c_int] + [i64] * 9, i64),
+        "ctattn_shared_prefix_fwd": ([c_int] + [vp] * 12 + [i64, vp] + [i64] * 10 + [c_int, vp], c_int),
+        "ctattn_sample_workspace_bytes": ([i64] * 2, i64),
+        "ctattn_sample": ([c_int] + [vp] * 6 + [f64, i64, f64, f64] + [vp] * 3 + [i64] * 4 + [vp], c_int),
         "ctattn_tensor_matmul": ([c_int, vp, vp, vp] + [i64] * 5 + [vp], c_int),
     }
     for name, (args, res) in sigs.items():

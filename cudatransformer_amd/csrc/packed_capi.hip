@@ -2,6 +2,7 @@
 // checks of arguments and the choice between the MFMA and the generic kernels.
 #include "attn_launch.h"
 #include "attn_packed.h"
+#include "capi_bytes.h"
 #include "capi_util.h"
 #include "ctattn.h"
 
@@ -12,9 +13,12 @@
 #include <vector>
 
 using namespace ctattn;
+using ctattn::capi::Bytes;
 using ctattn::capi::fail;
 using ctattn::capi::finish;
+using ctattn::capi::may_overlap;
 using ctattn::capi::ok;
+using ctattn::capi::run_of;
 
 namespace {
 
@@ -124,11 +128,6 @@ int check_outputs(const char *fn, std::initializer_list<const PackedStride *> ou
     return 0;
 }
 
-// The bytes of a [rows, heads, d] tensor: `lo`, `hi` its first and last; within a row from `lo` on `span` of them
-// every `row`, unless heads lie further apart than rows.
-struct Bytes {
-    intptr_t lo, hi, row, span;
-};
 Bytes bytes_of(const void *p, const PackedStride &s, int64_t rows, int64_t heads, int64_t d, int64_t es) {
     const intptr_t at = reinterpret_cast<intptr_t>(p);
     const auto end = [&](int64_t n, int64_t step) { return n > 1 ? (n - 1) * step : 0; };
@@ -136,21 +135,6 @@ Bytes bytes_of(const void *p, const PackedStride &s, int64_t rows, int64_t heads
     const int64_t down = std::min<int64_t>(0, end(rows, s.row)) + std::min<int64_t>(0, end(heads, s.head));
     return {at + down * es, at + (up + d) * es, s.row * es, (end(heads, s.head) + d) * es};
 }
-// Whether two tensors may share a byte.  Slices of one row-major buffer (a projection's q, k, v) do not: their rows are
-// equally far apart and each lies in its own part of a row.
-bool may_overlap(const Bytes &a, const Bytes &b) {
-    if (a.hi <= b.lo || b.hi <= a.lo) return false;
-    if (a.row != b.row || a.row <= 0 || a.span <= 0 || b.span <= 0 || a.span > a.row || b.span > a.row) return true;
-    const intptr_t shift = ((b.lo - a.lo) % a.row + a.row) % a.row;
-    return !(a.span <= shift && shift + b.span <= a.row);
-}
-
-// `n` bytes from p on, whole.
-Bytes run_of(const void *p, int64_t n) {
-    const intptr_t at = reinterpret_cast<intptr_t>(p);
-    return {at, at + n, 0, 0};
-}
-
 int64_t elem_bytes(int dtype) { return dtype == CTATTN_F64 ? 8 : dtype == CTATTN_F32 ? 4 : 2; }
 
 // A stride that is never stepped along (one head, one token) may hold anything: 0, so that it decides nothing.

@@ -1,0 +1,75 @@
+"""Next tokens from logits and given random numbers over torch device tensors (ctattn_sample of include/ctattn.h)."""
+from __future__ import annotations
+
+import operator
+
+import torch
+
+from ._capi import _DTYPE_CODE, _check, _ptr, _stream_handle, last_error, load, on_device
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of the workspace of sample_tokens."""
+    need = load().ctattn_sample_workspace_bytes(rows, vocab)
+    if need < 0:
+        raise ValueError(last_error())
+    return need
+
+
+def sample_tokens(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, logprobs=None, workspace=None,
+                  stream=None):
+    """(tokens, logprobs) [rows]: a token (int64) of each row of logits [rows, vocab] (float32, bfloat16 or float16; rows any
+    distance apart) from random numbers u [rows] (float32 in [0, 1)), and its log-probability (float32) among all tokens at
+    the row's temperature.
+
+    Tokens are ranked by logit, equal ones by the lower id.  Kept are the first top_k (0: all), of these the ranks
+    before which less than top_p of their probability lies (1: all), of these the ones at least min_p times as
+    probable as the first; always the first.  A token is drawn in the order of ids.  temperature <= 0 takes the first
+    rank.  Each parameter is a number or a tensor [rows] (float32; top_k int32).  Logits of -inf or NaN are
+    never taken; a row of nothing else gives token -1."""
+    name = "sample_tokens"
+    if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError(f"{name}: logits must be [rows, vocab] with contiguous rows on the GPU, got {list(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"{name}: dtype {logits.dtype} unsupported (float32, bfloat16, float16)")
+    (rows, vocab), device = logits.shape, logits.device
+
+    def each(what, x, dtype, number):
+        if not isinstance(x, torch.Tensor):
+            return None, number(x)
+        if x.dtype != dtype or tuple(x.shape) != (rows,) or x.device != device or not x.is_contiguous():
+            raise ValueError(f"{name}: {what} must be a number or contiguous {dtype} [{rows}] on {device}, got {x.dtype} {list(x.shape)} "
+                             f"on {x.device}")
+        return x, number(0)
+
+    t, t_all = each("temperature", temperature, torch.float32, float)
+    k, k_all = each("top_k", top_k, torch.int32, operator.index)
+    p, p_all = each("top_p", top_p, torch.float32, float)
+    m, m_all = each("min_p", min_p, torch.float32, float)
+    if u is None:
+        if t is not None or t_all > 0:
+            raise ValueError(f"{name}: random numbers may be left out for temperature 0 alone")
+    else:
+        each("u", u, torch.float32, float)
+        if not isinstance(u, torch.Tensor):
+            raise ValueError(f"{name}: u must be a tensor")
+    for what, x, dtype in (("tokens", tokens, torch.int64), ("logprobs", logprobs, torch.float32)):
+        if x is not None:
+            each(what, x, dtype, float)
+    if workspace is not None and (not workspace.is_contiguous() or workspace.device != device):
+        raise ValueError(f"{name}: workspace must be contiguous on {device}")
+    need = sample_workspace_bytes(rows, vocab)
+    with on_device(device, stream):
+        tokens = logits.new_empty(rows, dtype=torch.int64) if tokens is None else tokens
+        logprobs = logits.new_empty(rows, dtype=torch.float32) if logprobs is None else logprobs
+        if workspace is None and need > 0:
+            workspace = logits.new_empty(need, dtype=torch.uint8)
+        rc = load().ctattn_sample(_DTYPE_CODE[logits.dtype], _ptr(logits), _ptr(u), _ptr(t), _ptr(k), _ptr(p), _ptr(m), t_all, k_all,
+                                  p_all, m_all, _ptr(tokens), _ptr(logprobs), _ptr(workspace),
+                                  0 if workspace is None else workspace.numel() * workspace.element_size(), rows, vocab,
+                                  logits.stride(0), _stream_handle(stream))
+    _check(rc, "ctattn_sample")
+    return tokens, logprobs
+
+
+__all__ = ["sample_tokens", "sample_workspace_bytes"]

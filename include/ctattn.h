@@ -704,6 +704,122 @@ CTATTN_API int ctattn_muon_update_multi(int dtype, int count, void *const *param
                                         double scale, int steps, double a, double b, double c, double eps,
                                         void *stream);
 
+/* ---- generating: a paged key / value cache, attention of requests that share a prompt, sampling ----
+ *
+ * A cache is `pages` pages of page_size (a power of two) tokens, each [heads, d], of any page, token and head strides.
+ * A request's own tokens lie, in order, in the pages of its row of a table, table[i][0 .. ceil(len / page_size) - 1].
+ * Lengths, tables and counters are device memory that no call reads on the host: a captured step replays on what they hold
+ * then.  What they hold is brought into range where it is read, so that a wrong length or table gives wrong
+ * results and no wrong access.  No counterpart in the reference, whose generate() computes the whole context for every token
+ * (NanoGPT.cu:266-280).
+ *
+ * Free pages are a ring of free_places entries; counters[0] pages have been taken from it and counters[1] given to it,
+ * and free_pages[j mod free_places], counters[0] <= j < counters[1], are the free ones (a new pool: all pages, {0, pages}).
+ */
+
+/*
+ * Pages for new_lens[i] new tokens of each request, that holds lens[i] (numbers below 0 count as 0), and where each goes.
+ * Requests are served in order; one whose tokens do not all find room (in the table's width, in max_tokens rows, among
+ * the free pages) gets none, and those behind it that need no fresh page or fit in what is left are served.
+ *   table        [requests][table_row]: entries of the fresh pages are written, no others
+ *   starts       [requests + 1]: the first row of each request's new tokens, served or not; at the end their number
+ *   slots        [max_tokens]: page * page_size + place of each row, -1 for rows of unserved requests and behind the last
+ *   positions    [max_tokens]: a row's number in its request, plus offsets[i] if offsets is not NULL; 0 where slots is -1
+ *   lens_out     [requests]: lens + new_lens, or lens of unserved requests
+ *   counters_out [2]
+ * Up to 2^24 requests.  Outputs are apart from inputs and from each other (refused otherwise), so that a call can be
+ * repeated: it writes the same again.
+ */
+CTATTN_API int ctattn_page_reserve(const int32_t *lens, const int32_t *new_lens, const int32_t *offsets, int32_t *table,
+                                   const int32_t *free_pages, const int64_t *counters, int64_t *slots,
+                                   int64_t *positions, int32_t *starts, int32_t *lens_out, int64_t *counters_out,
+                                   int64_t requests, int64_t table_row, int64_t table_width, int64_t free_places,
+                                   int64_t page_size, int64_t max_tokens, void *stream);
+
+/*
+ * Gives the pages of the requests with done[i] != 0 (bytes) back to the ring, in order; their lens_out is 0, the others'
+ * lens.  A request whose pages the ring has no room for (they are in it already) keeps them.  The table is left as it is.
+ */
+CTATTN_API int ctattn_page_release(const void *done, const int32_t *lens, const int32_t *table, int32_t *free_pages,
+                                   const int64_t *counters, int32_t *lens_out, int64_t *counters_out, int64_t requests,
+                                   int64_t table_row, int64_t table_width, int64_t free_places, int64_t page_size,
+                                   void *stream);
+
+/*
+ * Copies row n of k and of v [rows, hkv, d] to place slots[n] of the caches; rows whose slot is outside the cache
+ * are skipped.  Any of the four floating dtypes.  `strides` (HOST) holds, in elements, the row and head strides of k and v, then
+ * the page, token and head strides of k_cache and v_cache; the d elements of a head are contiguous.  The caches may be
+ * slices of one buffer; neither may lie on k, v or slots (refused).  Of two rows with one slot either may
+ * remain, element by element.
+ */
+CTATTN_API int ctattn_cache_write(int dtype, const void *k, const void *v, void *k_cache, void *v_cache,
+                                  const int64_t *slots, const int64_t *strides, int64_t rows, int64_t hkv, int64_t d,
+                                  int64_t pages, int64_t page_size, void *stream);
+
+/* Bytes of device workspace ctattn_shared_prefix_fwd needs, or -1 on invalid arguments. */
+CTATTN_API int64_t ctattn_shared_prefix_workspace_bytes(int dtype, int64_t rows, int64_t requests, int64_t groups,
+                                                        int64_t hq, int64_t hkv, int64_t d, int64_t page_size,
+                                                        int64_t table_width, int64_t prefix_width);
+
+/*
+ * Attention of requests in groups that share a prompt: O = softmax(q K^T / sqrt(d)) V, and lse [rows, hq] (fp64 for
+ * CTATTN_F64, else fp32; may be NULL), over the prompt of the request's group, prefix_lens[g] tokens in the pages of
+ * prefix_table[g], and its own tokens, lens[i] in the pages of table[i].  Prompts are read once for all requests
+ * of a group (in blocks of 128 rows of token and head).
+ *   - starts [requests + 1] says which rows of q and o [rows, hq, d] are request i's: its last starts[i + 1] - starts[i]
+ *     own tokens, in order, whose keys are in the cache already; each sees the prompt and the own tokens up to itself.  NULL: one
+ *     row a request.  Rows before the first and behind the last request's are left as they are, or with fill != 0
+ *     written with zeros (lse -inf), as is a row that sees no key.
+ *   - group_starts [groups + 1] says which requests are group g's; NULL: equal groups.  Requests outside every group, and
+ *     all with groups = 0, have no prompt.
+ *   - an entry of a table that is no page of the cache is read as page 0; lengths are cut to the tables' widths.
+ *   - `strides` (HOST), in elements: row and head of q and of o, page, token and head of k_cache and of v_cache, rows of
+ *     table and of prefix_table.
+ *   - kernels: bf16, fp16 (d a multiple of 8) and fp32 (a multiple of 4) run on MFMA for d <= 128 and hq / hkv <= 128 when
+ *     pointers and strides are multiples of 16 bytes; other calls, f64, and every call under CTATTN_POLICY_GENERIC take a
+ *     generic kernel, much slower (and need no workspace).  The MFMA kernels round P to the 16-bit type as an operand of
+ *     P V, as ctattn_packed_fwd does; sums, maxima and the partial O of the splits are fp32.
+ *   - a NaN or an infinity in a prompt's or a request's tokens may reach any row that the prompt or the request belongs to; what
+ *     lies behind the last token of a page reaches none.
+ *   - no atomics: the same inputs give the same bits.  o, lse and the workspace (16-byte aligned, scratch) may lie on no
+ *     other tensor (refused).
+ */
+CTATTN_API int ctattn_shared_prefix_fwd(int dtype, const void *q, const void *k_cache, const void *v_cache,
+                                        const int32_t *table, const int32_t *lens, const int32_t *prefix_table,
+                                        const int32_t *prefix_lens, const int32_t *group_starts, const int32_t *starts,
+                                        void *o, void *lse, void *workspace, int64_t workspace_bytes,
+                                        const int64_t *strides, int64_t rows, int64_t requests, int64_t groups,
+                                        int64_t hq, int64_t hkv, int64_t d, int64_t pages, int64_t page_size,
+                                        int64_t table_width, int64_t prefix_width, int fill, void *stream);
+
+/* Bytes of device workspace ctattn_sample needs, or -1 on invalid arguments. */
+CTATTN_API int64_t ctattn_sample_workspace_bytes(int64_t rows, int64_t vocab);
+
+/*
+ * A token of each row of logits [rows][vocab] (f32, bf16, f16; rows `stride` elements apart; f64 is refused) from a given
+ * random number u[row] in [0, 1).  With M the row's largest logit and w_i = exp((x_i - M) / T), tokens are ranked by
+ * logit, equal ones by the lower id, and kept are
+ *   top-k  the first k ranks (k < 1: all),
+ *   top-p  of these, the ranks before which less than top_p of their sum of w lies (top_p >= 1: all),
+ *   min-p  of these, w >= min_p (min_p <= 0: all),
+ * and always the first.  The token is the first id, in the order of ids, at which the sum of kept w exceeds u times the sum
+ * of all kept w.  T <= 0 takes the first rank (u may then be NULL if T is not an array).  tokens int64; logprobs fp32: the
+ * token's log-probability among all tokens at temperature T (at 1 where T <= 0).
+ *   - temperature, top_k, top_p and min_p are device arrays of one number a row, or NULL: the number `_all`
+ *     then.  NaN counts as 0 for T and min_p, as 1 for top_p.
+ *   - a logit of -inf or NaN is never taken; a row of nothing else gives token -1 and log-probability -inf.  Logits of
+ *     +inf share the whole mass.
+ *   - w and its sums are held in 64 bits: only u within about 1e-13 of a border of two tokens can fall on
+ *     the other side of it.  The same inputs give the same tokens.
+ * Up to 65535 rows of up to 524288 logits.  tokens, logprobs and the workspace (16-byte aligned, scratch) may lie on no
+ * other tensor (refused).  Stands beside NanoGPT's predict() of the host, which copies the probabilities there.
+ */
+CTATTN_API int ctattn_sample(int dtype, const void *logits, const float *u, const float *temperature,
+                             const int32_t *top_k, const float *top_p, const float *min_p, double temperature_all,
+                             int64_t top_k_all, double top_p_all, double min_p_all, int64_t *tokens, float *logprobs,
+                             void *workspace, int64_t workspace_bytes, int64_t rows, int64_t vocab, int64_t stride,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif
