@@ -62,31 +62,40 @@ struct Args {
     int dp;      // d in whole tiles of 32
     int width;   // bytes of d elements
     int fill;
-    int one_page;  // a load instruction's rows lie in one page, both caches at equal token strides
+    int one_page;  // a load instruction's rows lie in one page, and lane offsets in 32 bits
     int ptiles, psplits, otiles, osplits;
-    float c;     // log2(e) / sqrt(d)
+    int pper, oper;  // tiles of each group or request where all have as many, or 0
+    int omost;       // keys of a request's own that a workgroup takes, or 0: equal stretches
+    float c;         // log2(e) / sqrt(d)
 };
 
-// How a workgroup's 4 waves share its work: RS slices of 32 rows x KS slices of 32 KT keys of every block.
-template <int RS_, int KS_, int KT_> struct Waves {
-    static constexpr int RS = RS_, KS = KS_, KT = KT_;
-    static_assert(RS * KS == 4, "4 waves");
-};
-template <typename F, int D, typename W> struct Cfg : W {
+// Rows of a tile: 128, of which each of the 4 waves takes 32 and all walk the same keys (tall), or 32, of whose keys every
+// wave walks a quarter.
+template <typename F, int D> struct Base {
     static constexpr int NW = 4;
-    static constexpr int BM = 32 * W::RS;
-    static constexpr int BN = 32 * W::KT * W::KS;
     static constexpr int DT = D / 32;
     static constexpr int RB = D * F::ES;
     static constexpr int STEPS = RB / 32;
-    static constexpr int KB = BN * RB;
-    // Two buffers, or with shared keys one where that lets a second workgroup onto the CU.
-    static constexpr int NBUF = W::KS > 1 && 4 * KB > 80 * 1024 ? 1 : 2;
-    static constexpr int LDS = NBUF * 2 * KB;  // buffer b: K at 2 b KB, V behind it
     using L = Tile<RB / 2>;
-    static constexpr int RPL = kWave / L::CH;        // rows of one load instruction
-    static constexpr int NL = BN / (NW * RPL);       // load instructions of a wave a tile
-    static_assert(kWave % L::CH == 0 && BN % (NW * RPL) == 0, "tile loads");
+    static constexpr int RPL = kWave / L::CH;  // rows of one load instruction
+    static_assert(kWave % L::CH == 0, "tile loads");
+};
+template <typename F, int D> struct Tall : Base<F, D> {
+    using B = Base<F, D>;
+    static constexpr int BM = 128;
+    static constexpr int KT = 2;
+    static constexpr int BN = 32 * KT;
+    static constexpr int KB = BN * B::RB;
+    static constexpr int LDS = 4 * KB;  // two buffers of K with V behind it
+    static constexpr int NL = BN / (B::NW * B::RPL);  // load instructions of a wave a tile
+};
+template <typename F, int D> struct Flat : Base<F, D> {
+    using B = Base<F, D>;
+    static constexpr int BM = 32;
+    static constexpr int BN = 32 * B::NW;  // of the workgroup; 32 keys a wave
+    static constexpr int KB = 32 * B::RB;
+    static constexpr int LDS = B::NW * 2 * KB;  // a wave's K with V behind it
+    static constexpr int NL = 32 / B::RPL;
 };
 
 // What a workgroup works on: rows (token, head of the group) r0 .. of `tokens` tokens from row `first` on, keys
@@ -98,51 +107,60 @@ struct Item {
     int split;
 };
 
-__device__ __forceinline__ void stretch(Item &it, int part, int parts, int block) {
-    const int each = ((it.len + parts - 1) / parts + block - 1) / block * block;
+// Part `part` of its keys, in whole blocks: `most` keys each, or if that is 0 in `parts` equal stretches.
+__device__ __forceinline__ void stretch(Item &it, int part, int parts, int most, int block) {
+    const int each = most > 0 ? most : ((it.len + parts - 1) / parts + block - 1) / block * block;
     const int64_t k0 = int64_t(part) * each;
     it.k0 = k0 < it.len ? int(k0) : it.len;
     it.k1 = it.len - it.k0 > each ? it.k0 + each : it.len;
 }
 
-// Tiles of a list of row ranges [row(i), row(i + 1)) have places of their own without a scan: range i's begin at
-// floor(row(i) G / BM) + i, and up to the next range's there are at least as many as it has tiles.
-template <typename Row> __device__ __forceinline__ int range_of(int n, int slot, int group, int bm, Row row) {
+// Tiles of a list of row ranges [row(i), row(i + 1)).  Equal ranges of one row a request have as many tiles each
+// (`per`).  Others have places of their own without a scan: range i's begin at floor(row(i) G / BM) + i, and up to
+// the next range's there are at least as many as it has tiles.
+template <typename Row> __device__ __forceinline__ int range_of(int n, int slot, int per, int group, int bm, Row row, int &tile) {
+    if (per > 0) {
+        tile = slot % per;
+        return slot / per;
+    }
     int lo = 0;
     for (int hi = n - 1; lo < hi;) {
         const int mid = (lo + hi + 1) / 2;
         if (row(mid) * group / bm + mid <= slot) lo = mid;
         else hi = mid - 1;
     }
+    tile = slot - (row(lo) * group / bm + lo);
     return lo;
 }
 template <int BM, int BN> __device__ __forceinline__ bool prefix_item(const Args &a, int slot, int part, Item &it) {
     const SharedLayout &y = a.lay;
     const auto row = [&](int g) { return y.group_row(g); };
-    const int g = range_of(y.groups, slot, y.group, BM, row);
+    int tile;
+    const int g = range_of(y.groups, slot, a.pper, y.group, BM, row, tile);
     it.first = row(g);
     it.tokens = row(g + 1) - it.first;
-    it.r0 = (slot - (it.first * y.group / BM + g)) * BM;
+    it.r0 = tile * BM;
     it.len = y.prefix_len(g);
     it.off = it.len;
     it.pages = y.prefix_table + g * y.prefix_row;
     it.split = part;
-    stretch(it, part, a.psplits, BN);
-    return it.r0 >= 0 && it.r0 < it.tokens * y.group;
+    stretch(it, part, a.psplits, 0, BN);
+    return tile >= 0 && it.r0 < it.tokens * y.group;
 }
 template <int BM, int BN> __device__ __forceinline__ bool own_item(const Args &a, int slot, int part, Item &it) {
     const SharedLayout &y = a.lay;
     const auto row = [&](int i) { return y.first_row(i); };
-    const int i = range_of(y.requests, slot, y.group, BM, row);
+    int tile;
+    const int i = range_of(y.requests, slot, a.oper, y.group, BM, row, tile);
     it.first = row(i);
     it.tokens = row(i + 1) - it.first;
-    it.r0 = (slot - (it.first * y.group / BM + i)) * BM;
+    it.r0 = tile * BM;
     it.len = y.own_len(i);
     it.off = it.len - it.tokens;
     it.pages = y.table + i * y.table_row;
     it.split = a.psplits + part;
-    stretch(it, part, a.osplits, BN);
-    return it.r0 >= 0 && it.r0 < it.tokens * y.group;
+    stretch(it, part, a.osplits, a.omost, BN);
+    return tile >= 0 && it.r0 < it.tokens * y.group;
 }
 
 __device__ __forceinline__ void load_chunk_saddr(uint32_t off, uint64_t base, uint32_t dst) {
@@ -154,132 +172,49 @@ __device__ __forceinline__ void load_chunk_saddr(uint32_t off, uint64_t base, ui
                  : "memory", "m0");
 }
 
-template <typename F, int D, bool PAD, typename W>
-__device__ __forceinline__ void walk(const Args &a, const Item &it, const int kvh, char *smem) {
-    using C = Cfg<F, D, W>;
-    using T = typename C::L;
-    using V = typename F::vec;
-    const uint32_t L = lds_addr(smem);
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int col = lane & 31, half = lane >> 5;
-    const int group = a.lay.group;
-    const int rows = it.tokens * group;
-    const int rs = wave % C::RS, ks = wave / C::RS;
-    const int r0w = it.r0 + 32 * rs;
-    const int row = r0w + col;
-    const int token = row / group, head = kvh * group + row % group;
-    const int koff = 32 * C::KT * ks;
-    // Keys from k0 on that a token sees.
-    const auto seen = [&](int t) { return max(min(it.k1, it.off >= it.len ? it.len : it.off + t + 1) - it.k0, 0); };
-    const int row_end = seen(token);
-    const int whole = seen(r0w / group);  // every row of the wave
-    const int some = seen(min((r0w + 31) / group, it.tokens - 1));  // any of them
-    const int kend = seen((min(it.r0 + C::BM, rows) - 1) / group);  // any of the workgroup
-    const int nkb = (kend + C::BN - 1) / C::BN;
+// A wave's 32 rows: query operands, O^T, and the running maximum and sum.
+template <typename F, int D> struct WaveState {
+    using B = Base<F, D>;
+    typename F::vec qb[B::STEPS];
+    floatx16 o[B::DT];
+    float m = kLowest, l = 0.f;
 
-    V qb[C::STEPS];
-    {
-        const char *p = a.q.at(it.first + token, head);
+    template <bool PAD> __device__ __forceinline__ void init(const char *p, bool there, int width, int half) {
 #pragma unroll
-        for (int s = 0; s < C::STEPS; ++s) {
+        for (int s = 0; s < B::STEPS; ++s) {
             floatx4 x = {0.f, 0.f, 0.f, 0.f};
-            if (row < rows && (!PAD || 32 * s + 16 * half < a.width))
-                x = *reinterpret_cast<const floatx4 *>(p + 32 * s + 16 * half);
-            qb[s] = __builtin_bit_cast(V, x);
+            if (there && (!PAD || 32 * s + 16 * half < width)) x = *reinterpret_cast<const floatx4 *>(p + 32 * s + 16 * half);
+            qb[s] = __builtin_bit_cast(typename F::vec, x);
         }
+#pragma unroll
+        for (int dt = 0; dt < B::DT; ++dt) o[dt] = zero16();
     }
-    floatx16 oacc[C::DT];
+    // S^T of the 32 keys whose tile's row operands begin at ka.
+    __device__ __forceinline__ floatx16 scores(uint32_t ka) const {
+        using V = typename F::vec;
+        floatx16 c = zero16();
+        V x[2];
+        x[0] = lds_b128<V>(ka);
 #pragma unroll
-    for (int dt = 0; dt < C::DT; ++dt) oacc[dt] = zero16();
-    float m_run = kLowest, l_run = 0.f;
-
-    const uint32_t rk = uint32_t(T::off(col, half));
-    const uint32_t cv0 = F::template col0<C::RB>(lane), cv1 = F::template col1<C::RB>(lane);
-
-    // Loads.  Instruction i of a wave fills rows RPL (wave NL + i) .. of the tile; a lane its chunk of one of them.
-    const int lr = lane / T::CH;
-    const int shift = a.lay.shift, in_page = (1 << shift) - 1;
-    const char *kbase = a.k.p + kvh * a.k.head, *vbase = a.v.p + kvh * a.v.head;
-    const auto chunk = [&](int i) { return 16 * ((lane % T::CH) ^ T::swz(C::RPL * (wave * C::NL + i) + lr)); };
-    int page[C::NL];
-    const auto look_up = [&](int kb) __attribute__((always_inline)) {
-        // Past the end the last key's page: no place of the table is read that its length does not cover.
-        if (!a.one_page) return;
-#pragma unroll
-        for (int i = 0; i < C::NL; ++i) {
-            const int key = min(it.k0 + kb * C::BN + C::RPL * (wave * C::NL + i), it.k0 + kend - 1);
-            page[i] = a.lay.page_at(it.pages, key);
+        for (int s = 0; s < B::STEPS; ++s) {
+            if (s + 1 < B::STEPS) x[(s + 1) & 1] = lds_b128<V>(ka ^ uint32_t((s + 1) << 5));
+            read_fence();
+            c = F::mma(x[s & 1], qb[s], c);
         }
-    };
-    const auto issue = [&](int kb) __attribute__((always_inline)) {
-        const uint32_t t = L + uint32_t((kb % C::NBUF) * 2 * C::KB);
-        const int j0 = kb * C::BN;
-        if (a.one_page && j0 + C::BN <= kend) {
-#pragma unroll
-            for (int i = 0; i < C::NL; ++i) {
-                const int first = C::RPL * (wave * C::NL + i);
-                const int64_t in = (it.k0 + j0 + first) & in_page;
-                const uint32_t dst = t + uint32_t(first * C::RB);
-                const uint32_t off = uint32_t(lr * int(a.k.token) + chunk(i));
-                if (!PAD || chunk(i) < a.width) {
-                    load_chunk_saddr(off, uint64_t(kbase) + uint64_t(int64_t(page[i]) * a.k.page + in * a.k.token), dst);
-                    load_chunk_saddr(off, uint64_t(vbase) + uint64_t(int64_t(page[i]) * a.v.page + in * a.v.token), dst + C::KB);
-                }
-            }
-        } else {
-            // Rows past the last key re-read it (their results are masked).
-#pragma unroll
-            for (int i = 0; i < C::NL; ++i) {
-                const int first = C::RPL * (wave * C::NL + i);
-                const int key = it.k0 + min(j0 + first + lr, kend - 1);
-                const int64_t pg = a.lay.page_at(it.pages, key), in = key & in_page;
-                const uint32_t dst = t + uint32_t(first * C::RB);
-                if (!PAD || chunk(i) < a.width) {
-                    load_chunk_dma(kbase + pg * a.k.page + in * a.k.token + chunk(i), dst);
-                    load_chunk_dma(vbase + pg * a.v.page + in * a.v.token + chunk(i), dst + C::KB);
-                }
-            }
-        }
-    };
-    // This wave's keys of a block.  MASK: some rows of the wave do not see some of them.
-    auto block = [&](auto mask, int kb) __attribute__((always_inline)) {
-        constexpr bool MASK = decltype(mask)::value;
-        const int j0 = kb * C::BN + koff;
-        const uint32_t kt0 = L + uint32_t((kb % C::NBUF) * 2 * C::KB) + uint32_t(koff * C::RB);
-        bool active[C::KT];
-        floatx16 sacc[C::KT];
-#pragma unroll
-        for (int kt = 0; kt < C::KT; ++kt) {
-            const int t0 = j0 + 32 * kt;
-            active[kt] = !MASK || t0 < some;
-            sacc[kt] = zero16();
-            if (!active[kt]) continue;
-            const uint32_t ka = kt0 + rk + uint32_t(32 * kt * C::RB);
-            V x[2];
-            x[0] = lds_b128<V>(ka);
-#pragma unroll
-            for (int s = 0; s < C::STEPS; ++s) {
-                if (s + 1 < C::STEPS) x[(s + 1) & 1] = lds_b128<V>(ka ^ uint32_t((s + 1) << 5));
-                read_fence();
-                sacc[kt] = F::mma(x[s & 1], qb[s], sacc[kt]);
-            }
-            if (MASK) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t0 + acc_row(r, half) >= row_end) sacc[kt][r] = -INFINITY;
-            }
-        }
-        typename F::pvec pb[C::KT][2];
+        return c;
+    }
+    // P of KT tiles' scores, with the maximum raised where they pass it by far.
+    template <int KT>
+    __device__ __forceinline__ void softmax(const floatx16 (&c)[KT], const bool (&active)[KT], typename F::pvec (&pb)[KT][2], float scale) {
         float psum;
         auto expo = [&]() __attribute__((always_inline)) {
             psum = 0.f;
 #pragma unroll
-            for (int kt = 0; kt < C::KT; ++kt) {
+            for (int kt = 0; kt < KT; ++kt) {
                 if (!active[kt]) continue;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float p = fast_exp2(fmaf(sacc[kt][r], a.c, -m_run));
+                    const float p = fast_exp2(fmaf(c[kt][r], scale, -m));
                     psum += p;
                     F::put(pb[kt][r / 8], r % 8, p);
                 }
@@ -289,69 +224,196 @@ __device__ __forceinline__ void walk(const Args &a, const Item &it, const int kv
         if (__any(!(psum <= Rise<F>::PSUM))) {
             float top = -INFINITY;
 #pragma unroll
-            for (int kt = 0; kt < C::KT; ++kt) {
+            for (int kt = 0; kt < KT; ++kt) {
                 if (!active[kt]) continue;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, sacc[kt][r]);
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, c[kt][r]);
             }
-            top = max_xor32(top) * a.c;
-            if (__any(top > m_run + Rise<F>::BY)) {
-                const float m_new = fmaxf(m_run, top - Rise<F>::UNDER);
-                const float resc = fast_exp2(m_run - m_new);
-                m_run = m_new;
-                l_run *= resc;
+            top = max_xor32(top) * scale;
+            if (__any(top > m + Rise<F>::BY)) {
+                const float m_new = fmaxf(m, top - Rise<F>::UNDER);
+                const float resc = fast_exp2(m - m_new);
+                m = m_new;
+                l *= resc;
 #pragma unroll
-                for (int dt = 0; dt < C::DT; ++dt) oacc[dt] *= resc;
+                for (int dt = 0; dt < B::DT; ++dt) o[dt] *= resc;
             }
             expo();
         }
-        l_run += psum;
-        const uint32_t v0 = kt0 + uint32_t(C::KB) + cv0, v1 = kt0 + uint32_t(C::KB) + cv1;
+        l += psum;
+    }
+    // O^T += V^T P^T of 32 keys whose column operands begin at v0, v1.
+    __device__ __forceinline__ void add(uint32_t v0, uint32_t v1, const typename F::pvec (&pb)[2]) {
+        constexpr int NS = 2 * B::DT;
+        typename F::cols x[2];
+        x[0] = F::template read_cols<B::RB>(v0, v1, 0, 0);
 #pragma unroll
-        for (int kt = 0; kt < C::KT; ++kt) {
-            if (!active[kt]) continue;
-            constexpr int NS = 2 * C::DT;
-            typename F::cols x[2];
-            x[0] = F::template read_cols<C::RB>(v0 + 32 * kt * C::RB, v1 + 32 * kt * C::RB, 0, 0);
+        for (int i = 0; i < NS; ++i) {
+            if (i + 1 < NS) x[(i + 1) & 1] = F::template read_cols<B::RB>(v0, v1, (i + 1) / B::DT, (i + 1) % B::DT);
+            read_fence();
+            o[i % B::DT] = F::col_mma(x[i & 1], pb[i / B::DT], o[i % B::DT]);
+        }
+    }
+    // The row's part of the item's split: m and l, and O where a key was seen.
+    template <bool PAD>
+    __device__ __forceinline__ void leave(const Args &a, const Item &it, int token, int head, int half, bool saw) const {
+        const float sum = l + __shfl_xor(l, 32, kWave);
+        const int64_t at = (int64_t(it.split) * a.lay.rows + it.first + token) * (a.lay.hkv * a.lay.group) + head;
+        if (half == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{m, sum};
+        if (!saw) return;
+        float *po = a.po + at * a.dp;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                if (i + 1 < NS)
-                    x[(i + 1) & 1] = F::template read_cols<C::RB>(v0 + 32 * kt * C::RB, v1 + 32 * kt * C::RB,
-                                                                  (i + 1) / C::DT, (i + 1) % C::DT);
-                read_fence();
-                oacc[i % C::DT] = F::col_mma(x[i & 1], pb[kt][i / C::DT], oacc[i % C::DT]);
+        for (int dt = 0; dt < B::DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (!PAD || (32 * dt + 8 * g + 4 * half) * F::ES < a.width)
+                    *reinterpret_cast<floatx4 *>(po + 32 * dt + 8 * g + 4 * half) =
+                        floatx4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+    }
+};
+
+// Loads of NL instructions of RPL rows each, rows base(i) .. of a stretch of keys from k0 on; PAD: chunks past `width`
+// bytes are left as they are (zeros).
+template <typename B, int NL, bool PAD> struct PagedLoads {
+    const Args &a;
+    const Item &it;
+    const char *k, *v;
+    int row0, lane;  // the first instruction's first row in a block
+    int page[NL];    // of the next block's rows, or the block's own lanes' pages at the end
+
+    __device__ __forceinline__ PagedLoads(const Args &a_, const Item &it_, int kvh, int row0_, int lane_)
+        : a(a_), it(it_), k(a_.k.p + kvh * a_.k.head), v(a_.v.p + kvh * a_.v.head), row0(row0_), lane(lane_) {}
+    __device__ __forceinline__ int chunk(int i) const {
+        return 16 * ((lane % B::L::CH) ^ B::L::swz(row0 + B::RPL * i + lane / B::L::CH));
+    }
+    __device__ __forceinline__ bool fast(int j0, int block, int end) const { return a.one_page && j0 + block <= end; }
+    // The pages of the rows of a block at j0 (keys from k0 on, `end` of them); past the end the last key's: no place of
+    // the table is read that its length does not cover.  Through the constant address space: scalar loads.
+    __device__ __forceinline__ void look_up(int j0, int end) {
+        if (!a.one_page) return;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int key = __builtin_amdgcn_readfirstlane(it.k0 + min(j0 + row0 + B::RPL * i, end - 1));
+            const auto *t = (const __attribute__((address_space(4))) int32_t *)(it.pages + (key >> a.lay.shift));
+            const int p = *t;
+            page[i] = uint32_t(p) < uint32_t(a.lay.pages) ? p : 0;
+        }
+    }
+    // Every lane's row of the block at j0; rows past the last key are that key's (their results are masked).
+    __device__ __forceinline__ int last_key(int j0, int end, int i) const {
+        return it.k0 + min(j0 + row0 + B::RPL * i + lane / B::L::CH, end - 1);
+    }
+    __device__ __forceinline__ void look_up_lanes(int j0, int end) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) page[i] = a.lay.page_at(it.pages, last_key(j0, end, i));
+    }
+    __device__ __forceinline__ void load(const char *cache, const CacheView &c, uint32_t tile, int j0, int end, bool whole) const {
+        const int in_page = (1 << a.lay.shift) - 1;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const uint32_t dst = tile + uint32_t(B::RPL * i * B::RB);
+            if (whole) {
+                const int64_t in = (it.k0 + j0 + row0 + B::RPL * i) & in_page;
+                if (!PAD || chunk(i) < a.width)
+                    load_chunk_saddr(uint32_t((lane / B::L::CH) * int(c.token) + chunk(i)),
+                                     uint64_t(cache) + uint64_t(int64_t(page[i]) * c.page + in * c.token), dst);
+            } else {
+                const int64_t in = last_key(j0, end, i) & in_page;
+                if (!PAD || chunk(i) < a.width) load_chunk_dma(cache + int64_t(page[i]) * c.page + in * c.token + chunk(i), dst);
             }
         }
-    };
-    auto step = [&](int kb) __attribute__((always_inline)) {
-        if (C::NBUF == 1 && kb > 0) {
-            lds_barrier();  // every wave is done with the last block
-            issue(kb);
-            if (kb + 1 < nkb) look_up(kb + 1);
+    }
+};
+
+template <bool PAD, int BYTES> __device__ __forceinline__ void clear_padding(char *smem) {
+    // Chunks past the head dim are zeros that no load overwrites.
+    if (!PAD) return;
+    for (uint32_t x = threadIdx.x * 16; x < uint32_t(BYTES); x += 256 * 16)
+        *reinterpret_cast<floatx4 *>(smem + x) = floatx4{0.f, 0.f, 0.f, 0.f};
+    lds_barrier();
+}
+
+// 128 rows, whose waves walk the same keys in blocks of 64, two buffers.
+template <typename F, int D, bool PAD>
+__device__ __forceinline__ void walk_tall(const Args &a, const Item &it, const int kvh, char *smem) {
+    using C = Tall<F, D>;
+    const uint32_t L = lds_addr(smem);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 31, half = lane >> 5;
+    const int group = a.lay.group, rows = it.tokens * group;
+    const int r0w = it.r0 + 32 * wave, row = r0w + col;
+    const int token = row / group, head = kvh * group + row % group;
+    // Keys from k0 on that a token sees.
+    const auto seen = [&](int t) { return max(min(it.k1, it.off >= it.len ? it.len : it.off + t + 1) - it.k0, 0); };
+    const int row_end = seen(token);
+    const int whole = seen(r0w / group);  // every row of the wave
+    const int some = r0w < rows ? seen(min((r0w + 31) / group, it.tokens - 1)) : 0;  // any of them
+    const int end = seen((min(it.r0 + C::BM, rows) - 1) / group);  // any of the workgroup
+    const int nkb = (end + C::BN - 1) / C::BN;
+    WaveState<F, D> w;
+    w.template init<PAD>(a.q.at(it.first + token, head), row < rows, a.width, half);
+    const uint32_t rk = uint32_t(C::L::off(col, half));
+    const uint32_t cv0 = F::template col0<C::RB>(lane), cv1 = F::template col1<C::RB>(lane);
+    PagedLoads<Base<F, D>, C::NL, PAD> loads(a, it, kvh, C::RPL * C::NL * wave, lane);
+
+    const auto issue = [&](int kb) __attribute__((always_inline)) {
+        const uint32_t t = L + uint32_t((kb & 1) * 2 * C::KB + C::RPL * C::NL * wave * C::RB);
+        const int j0 = kb * C::BN;
+        const bool fast = loads.fast(j0, C::BN, end);
+        if (fast) {
+            loads.load(loads.k, a.k, t, j0, end, true);
+            loads.load(loads.v, a.v, t + C::KB, j0, end, true);
+        } else {
+            loads.look_up_lanes(j0, end);
+            loads.load(loads.k, a.k, t, j0, end, false);
+            loads.load(loads.v, a.v, t + C::KB, j0, end, false);
         }
-        // This wave's loads of the block have landed; after the barrier every wave's have, and
-        // (two buffers) every wave is done reading the other one.
+    };
+    // MASK: some rows of the wave do not see some keys of the block.
+    const auto block = [&](auto mask, int kb) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask)::value;
+        const uint32_t kt0 = L + uint32_t((kb & 1) * 2 * C::KB);
+        bool active[C::KT];
+        floatx16 c[C::KT];
+#pragma unroll
+        for (int kt = 0; kt < C::KT; ++kt) {
+            const int t0 = kb * C::BN + 32 * kt;
+            active[kt] = !MASK || t0 < some;
+            if (!active[kt]) continue;
+            c[kt] = w.scores(kt0 + rk + uint32_t(32 * kt * C::RB));
+            if (MASK) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t0 + acc_row(r, half) >= row_end) c[kt][r] = -INFINITY;
+            }
+        }
+        typename F::pvec pb[C::KT][2];
+        w.template softmax<C::KT>(c, active, pb, a.c);
+        const uint32_t vt = kt0 + uint32_t(C::KB);
+#pragma unroll
+        for (int kt = 0; kt < C::KT; ++kt)
+            if (active[kt]) w.add(vt + cv0 + 32 * kt * C::RB, vt + cv1 + 32 * kt * C::RB, pb[kt]);
+    };
+    const auto step = [&](int kb) __attribute__((always_inline)) {
+        // This wave's loads of the block have landed; after the barrier every wave's have, and every wave is done reading
+        // the other buffer.
         wait_loads();
         lds_barrier();
-        if (C::NBUF == 2 && kb + 1 < nkb) {
+        if (kb + 1 < nkb) {
             issue(kb + 1);
-            if (kb + 2 < nkb) look_up(kb + 2);
+            if (kb + 2 < nkb) loads.look_up((kb + 2) * C::BN, end);
         }
     };
-    if (PAD) {
-        // Chunks past the head dim are zeros that no load overwrites.
-        for (uint32_t x = threadIdx.x * 16; x < uint32_t(C::LDS); x += 256 * 16)
-            *reinterpret_cast<floatx4 *>(smem + x) = floatx4{0.f, 0.f, 0.f, 0.f};
-        lds_barrier();
-    }
+    clear_padding<PAD, C::LDS>(smem);
     if (nkb > 0) {
-        look_up(0);
+        loads.look_up(0, end);
         issue(0);
-        if (nkb > 1) look_up(1);
+        if (nkb > 1) loads.look_up(C::BN, end);
     }
     // This wave's blocks, in loops without branches inside: [0, jp) whole, [jp, jw) masked, [jw, nkb) none of its pairs.
-    const int jw = r0w < rows && some > koff ? (some - koff + C::BN - 1) / C::BN : 0;
-    const int jp = min(jw, whole >= koff + 32 * C::KT ? (whole - koff - 32 * C::KT) / C::BN + 1 : 0);
+    const int jw = (some + C::BN - 1) / C::BN;
+    const int jp = min(jw, whole / C::BN);
     int kb = 0;
     for (; kb < jp; ++kb) {
         step(kb);
@@ -362,88 +424,149 @@ __device__ __forceinline__ void walk(const Args &a, const Item &it, const int kv
         block(std::true_type{}, kb);
     }
     for (; kb < nkb; ++kb) step(kb);
+    if (row < rows) w.template leave<PAD>(a, it, token, head, half, row_end > 0);
+}
 
-    if constexpr (C::KS > 1) {
-        // The key slices of a row slice join: m = max, O and l weighted by 2^(their m - m).  A slice that
-        // saw no key has the lowest m and l = 0.
-        constexpr int NR = C::DT * 16 + 2;
-        static_assert((C::KS - 1) * C::RS * NR * kWave * 4 <= C::LDS, "join buffer");
-        float *jb = reinterpret_cast<float *>(smem);
-        lds_barrier();  // every wave is done with the tiles
-        if (ks > 0) {
-            float *to = jb + ((ks - 1) * C::RS + rs) * NR * kWave + lane;
-#pragma unroll
-            for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) to[(dt * 16 + r) * kWave] = oacc[dt][r];
-            to[(NR - 2) * kWave] = m_run;
-            to[(NR - 1) * kWave] = l_run;
+template <int N> __device__ __forceinline__ void wait_loads_but() {
+    static_assert(N < 64, "vmcnt");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// 32 rows, whose keys the waves walk apart, 32 of every block of 128 each, through LDS of their own: no barriers, and a
+// wave's next K is on its way while it adds V, its next V while it computes scores.
+template <typename F, int D, bool PAD>
+__device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const int kvh, char *smem) {
+    using C = Flat<F, D>;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane & 31, half = lane >> 5;
+    const int group = a.lay.group, rows = it.tokens * group;
+    const int row = it.r0 + col;
+    const int token = row / group, head = kvh * group + row % group;
+    const auto seen = [&](int t) { return max(min(it.k1, it.off >= it.len ? it.len : it.off + t + 1) - it.k0, 0); };
+    const int row_end = seen(token);
+    const int whole = seen(it.r0 / group);
+    const int end = seen((min(it.r0 + C::BM, rows) - 1) / group);
+    WaveState<F, D> w;
+    w.template init<PAD>(a.q.at(it.first + token, head), row < rows, a.width, half);
+    const uint32_t kt = lds_addr(smem) + uint32_t(wave * 2 * C::KB), vt = kt + uint32_t(C::KB);
+    const uint32_t rk = kt + uint32_t(C::L::off(col, half));
+    const uint32_t cv0 = vt + F::template col0<C::RB>(lane), cv1 = vt + F::template col1<C::RB>(lane);
+    PagedLoads<Base<F, D>, C::NL, PAD> loads(a, it, kvh, 0, lane);
+    clear_padding<PAD, C::LDS>(smem);
+
+    // This wave's blocks begin at keys 32 wave + 128 n.
+    int j0 = 32 * wave;
+    bool fast = false;
+    const auto load_k = [&](int j) __attribute__((always_inline)) {
+        fast = loads.fast(j, 32, end);
+        if (fast) {
+            loads.load(loads.k, a.k, kt, j, end, true);
+        } else {
+            loads.look_up_lanes(j, end);
+            loads.load(loads.k, a.k, kt, j, end, false);
         }
-        lds_barrier();
-        if (ks > 0) return;
-        const float *from = jb + rs * NR * kWave + lane;
-        float m = m_run, w[C::KS - 1];
+    };
+    const auto load_v = [&](int j) __attribute__((always_inline)) {
+        if (fast) loads.load(loads.v, a.v, vt, j, end, true);
+        else loads.load(loads.v, a.v, vt, j, end, false);
+    };
+    if (j0 < end) {
+        loads.look_up(j0, end);
+        load_k(j0);
+        load_v(j0);
+        while (true) {
+            const int next = j0 + C::BN;
+            const bool more = next < end;
+            floatx16 c[1];
+            const bool active[1] = {true};
+            typename F::pvec pb[1][2];
+            wait_loads_but<C::NL>();  // K is there, V may be on its way
+            c[0] = w.scores(rk);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+            if (more) {
+                loads.look_up(next, end);
+                load_k(next);
+            }
+            if (j0 + 32 > whole) {
 #pragma unroll
-        for (int i = 0; i < C::KS - 1; ++i) m = fmaxf(m, from[i * C::RS * NR * kWave + (NR - 2) * kWave]);
-        const float w0 = fast_exp2(m_run - m);
-        l_run *= w0;
-#pragma unroll
-        for (int i = 0; i < C::KS - 1; ++i) {
-            w[i] = fast_exp2(from[i * C::RS * NR * kWave + (NR - 2) * kWave] - m);
-            l_run += from[i * C::RS * NR * kWave + (NR - 1) * kWave] * w[i];
+                for (int r = 0; r < 16; ++r)
+                    if (j0 + acc_row(r, half) >= row_end) c[0][r] = -INFINITY;
+            }
+            w.template softmax<1>(c, active, pb, a.c);
+            if (more) wait_loads_but<C::NL>();  // V is there
+            else wait_loads_but<0>();
+            w.add(cv0, cv1, pb[0]);
+            if (!more) break;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
+            load_v(next);
+            j0 = next;
         }
+    }
+
+    // The waves join: m = max, O and l weighted by 2^(their m - m).  A wave that saw no key has the lowest m and l = 0.
+    constexpr int KS = C::NW, NR = C::DT * 16 + 2;
+    static_assert((KS - 1) * NR * kWave * 4 <= C::LDS, "join buffer");
+    float *jb = reinterpret_cast<float *>(smem);
+    lds_barrier();  // every wave is done with its tiles
+    if (wave > 0) {
+        float *to = jb + (wave - 1) * NR * kWave + lane;
 #pragma unroll
         for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float x = oacc[dt][r] * w0;
-#pragma unroll
-                for (int i = 0; i < C::KS - 1; ++i) x += from[i * C::RS * NR * kWave + (dt * 16 + r) * kWave] * w[i];
-                oacc[dt][r] = x;
-            }
-        m_run = m;
+            for (int r = 0; r < 16; ++r) to[(dt * 16 + r) * kWave] = w.o[dt][r];
+        to[(NR - 2) * kWave] = w.m;
+        to[(NR - 1) * kWave] = w.l;
     }
-    const float l_tot = l_run + __shfl_xor(l_run, 32, kWave);
-    if (row >= rows) return;
-    const int64_t at = (int64_t(it.split) * a.lay.rows + it.first + token) * (a.lay.hkv * group) + head;
-    if (half == 0) *reinterpret_cast<float2 *>(a.ml + 2 * at) = float2{m_run, l_tot};
-    if (row_end == 0) return;  // l = 0: nothing to join
-    float *po = a.po + at * a.dp;
+    lds_barrier();
+    if (wave > 0) return;
+    // One after the other: all at once take more registers than there are.
+#pragma unroll 1
+    for (int i = 0; i < KS - 1; ++i) {
+        const float *from = jb + i * NR * kWave + lane;
+        const float mi = from[(NR - 2) * kWave], m = fmaxf(w.m, mi);
+        const float x = fast_exp2(w.m - m), y = fast_exp2(mi - m);
+        w.m = m;
+        w.l = w.l * x + from[(NR - 1) * kWave] * y;
 #pragma unroll
-    for (int dt = 0; dt < C::DT; ++dt)
+        for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-            if (!PAD || (32 * dt + 8 * g + 4 * half) * F::ES < a.width)
-                *reinterpret_cast<floatx4 *>(po + 32 * dt + 8 * g + 4 * half) =
-                    floatx4{oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
+            for (int r = 0; r < 16; ++r) w.o[dt][r] = w.o[dt][r] * x + from[(dt * 16 + r) * kWave] * y;
+    }
+    if (row < rows) w.template leave<PAD>(a, it, token, head, half, row_end > 0);
 }
 
-template <typename F, int D, typename WP, typename WO> struct Both {
-    static constexpr int LDS = Cfg<F, D, WP>::LDS > Cfg<F, D, WO>::LDS ? Cfg<F, D, WP>::LDS : Cfg<F, D, WO>::LDS;
-    static constexpr int WPE = Cfg<F, D, WP>::RB > 256 || LDS > 80 * 1024 ? 1 : 2;
-};
-
 // Workgroups of the prompts' keys first, then those of the requests' own.
-template <typename F, int D, bool PAD, typename WP, typename WO>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Both<F, D, WP, WO>::WPE, 2))) void shared_kernel(
-    Args a) {
-    __shared__ __attribute__((aligned(1024))) char smem[Both<F, D, WP, WO>::LDS];
+template <typename F, int D, bool TP, bool TO> struct Both {
+    static constexpr int TALL = TP || TO ? Tall<F, D>::LDS : 0, FLAT = TP && TO ? 0 : Flat<F, D>::LDS;
+    static constexpr int LDS = TALL > FLAT ? TALL : FLAT;
+    static constexpr int WPE = Base<F, D>::RB > 256 || LDS > 80 * 1024 ? 1 : 2;
+};
+template <typename F, int D, bool PAD, bool TP, bool TO>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Both<F, D, TP, TO>::WPE, 2))) void shared_kernel(Args a) {
+    __shared__ __attribute__((aligned(1024))) char smem[Both<F, D, TP, TO>::LDS];
     const int hkv = a.lay.hkv;
     const int kvh = blockIdx.x % hkv;
     int slot = blockIdx.x / hkv;
     Item it;
+    const auto walk = [&](auto tall) __attribute__((always_inline)) {
+        if constexpr (decltype(tall)::value) walk_tall<F, D, PAD>(a, it, kvh, smem);
+        else walk_flat<F, D, PAD>(a, it, kvh, smem);
+    };
+    using P = std::conditional_t<TP, Tall<F, D>, Flat<F, D>>;
+    using O = std::conditional_t<TO, Tall<F, D>, Flat<F, D>>;
     if (slot < a.ptiles * a.psplits) {
-        if (!prefix_item<Cfg<F, D, WP>::BM, Cfg<F, D, WP>::BN>(a, slot % a.ptiles, slot / a.ptiles, it)) return;
-        walk<F, D, PAD, WP>(a, it, kvh, smem);
+        if (!prefix_item<P::BM, P::BN>(a, slot % a.ptiles, slot / a.ptiles, it)) return;
+        walk(std::bool_constant<TP>{});
     } else {
         slot -= a.ptiles * a.psplits;
-        if (!own_item<Cfg<F, D, WO>::BM, Cfg<F, D, WO>::BN>(a, slot % a.otiles, slot / a.otiles, it)) return;
-        walk<F, D, PAD, WO>(a, it, kvh, smem);
+        if (!own_item<O::BM, O::BN>(a, slot % a.otiles, slot / a.otiles, it)) return;
+        walk(std::bool_constant<TO>{});
     }
 }
 
 // O = sum of 2^(m_s - m) O_s / sum of 2^(m_s - m) l_s over the splits s that saw a key.  A thread joins 4 elements of a row's
-// head.
+// head, 8 splits' loads at a time.
 template <typename F> __global__ __launch_bounds__(256) void shared_join_kernel(Args a, int d) {
     using S = typename F::store;
     const SharedLayout &y = a.lay;
@@ -458,19 +581,31 @@ template <typename F> __global__ __launch_bounds__(256) void shared_join_kernel(
     const bool prompt = there && a.psplits > 0 && n >= y.group_row(0) && n < y.group_row(y.groups);
     const int s0 = prompt ? 0 : a.psplits, s1 = there ? a.psplits + a.osplits : s0;
     const int64_t step = int64_t(y.rows) * hq;
-    float m = kLowest;
-    for (int s = s0; s < s1; ++s) {
-        const float2 x = *reinterpret_cast<const float2 *>(a.ml + 2 * (s * step + rh));
-        if (!(x.y == 0.f)) m = fmaxf(m, x.x);
-    }
-    float l = 0.f;
+    const float *ml = a.ml + 2 * rh, *po = a.po + rh * a.dp + c;
+    constexpr int N = 8;
+    float m = kLowest, l = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; ++s) {
-        const float2 x = *reinterpret_cast<const float2 *>(a.ml + 2 * (s * step + rh));
-        if (x.y == 0.f) continue;
-        const float w = fast_exp2(x.x - m);
-        l += w * x.y;
-        o += w * *reinterpret_cast<const floatx4 *>(a.po + (s * step + rh) * a.dp + c);
+    for (int s = s0; s < s1; s += N) {
+        float2 x[N];
+        floatx4 p[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = s + i < s1 ? *reinterpret_cast<const float2 *>(ml + 2 * (s + i) * step) : float2{kLowest, 0.f};
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            p[i] = x[i].y == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<const floatx4 *>(po + (s + i) * step * a.dp);
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = x[i].y == 0.f ? top : fmaxf(top, x[i].x);
+        const float keep = fast_exp2(m - top);
+        l *= keep;
+        o *= keep;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float w = x[i].y == 0.f ? 0.f : fast_exp2(x[i].x - top);
+            l += w * x[i].y;
+            o += w * p[i];
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
@@ -478,29 +613,34 @@ template <typename F> __global__ __launch_bounds__(256) void shared_join_kernel(
     if (a.lse != nullptr && c == 0) a.lse[rh] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-using Rows128 = Waves<4, 1, 2>;
-using Rows32 = Waves<1, 4, 1>;
-
 // Tiles and splits, from the call's shapes alone.
 struct Plan {
     bool tall_prefix, tall_own;
-    int ptiles, psplits, otiles, osplits;
+    int ptiles, psplits, otiles, osplits, pper, oper, omost;
 };
 Plan plan_of(const SharedCall &c) {
     Plan p{};
     const int64_t work_rows = c.rows * c.group();
-    const auto tiles = [&](int64_t ranges, bool tall) { return int(work_rows / (tall ? 128 : 32) + ranges); };
-    const auto splits = [&](int64_t tiles, int64_t keys, int64_t least) {
-        const int64_t want = 512 / std::max<int64_t>(1, tiles * c.hkv);
-        return int(std::max<int64_t>(1, std::min(want, keys / least)));
-    };
+    const auto div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     p.tall_own = work_rows > 32 * c.requests;
     p.tall_prefix = p.tall_own || (c.groups > 0 && work_rows > 32 * c.groups);
-    p.otiles = c.requests > 0 ? tiles(c.requests, p.tall_own) : 0;
-    p.osplits = splits(p.otiles, c.max_own(), 128);
+    if (c.requests > 0) {
+        const int64_t bm = p.tall_own ? 128 : 32;
+        p.oper = c.starts ? 0 : int(div(c.group(), bm));
+        p.otiles = int(p.oper > 0 ? p.oper * c.requests : work_rows / bm + c.requests);
+        const int64_t wgs = p.otiles * c.hkv;
+        if (wgs >= 512) {
+            p.omost = int(std::max<int64_t>(512, div(div(c.max_own(), 16), 128) * 128));
+            p.osplits = int(std::max<int64_t>(1, div(c.max_own(), p.omost)));
+        } else {
+            p.osplits = int(std::max<int64_t>(1, std::min({int64_t(128), 1024 / wgs, div(c.max_own(), 128)})));
+        }
+    }
     if (c.max_prefix() > 0) {
-        p.ptiles = tiles(c.groups, p.tall_prefix);
-        p.psplits = splits(p.ptiles, c.max_prefix(), 256);
+        const int64_t bm = p.tall_prefix ? 128 : 32;
+        p.pper = c.starts || c.group_starts ? 0 : int(div(c.requests / c.groups * c.group(), bm));
+        p.ptiles = int(p.pper > 0 ? p.pper * c.groups : c.groups == 1 ? div(work_rows, bm) : work_rows / bm + c.groups);
+        p.psplits = int(std::max<int64_t>(1, std::min({int64_t(128), 512 / std::max<int64_t>(1, p.ptiles * c.hkv), div(c.max_prefix(), 128)})));
     }
     return p;
 }
@@ -512,9 +652,9 @@ template <typename F, int D, bool PAD> hipError_t launch_d(const Args &a, const 
     if (!grid_fits(blocks, 256)) return hipErrorInvalidValue;
     if (blocks > 0) {
         const dim3 grid(static_cast<unsigned>(blocks)), block(256);
-        if (p.tall_own) shared_kernel<F, D, PAD, Rows128, Rows128><<<grid, block, 0, stream>>>(a);
-        else if (p.tall_prefix) shared_kernel<F, D, PAD, Rows128, Rows32><<<grid, block, 0, stream>>>(a);
-        else shared_kernel<F, D, PAD, Rows32, Rows32><<<grid, block, 0, stream>>>(a);
+        if (p.tall_own) shared_kernel<F, D, PAD, true, true><<<grid, block, 0, stream>>>(a);
+        else if (p.tall_prefix) shared_kernel<F, D, PAD, true, false><<<grid, block, 0, stream>>>(a);
+        else shared_kernel<F, D, PAD, false, false><<<grid, block, 0, stream>>>(a);
     }
     return hipGetLastError();
 }
@@ -539,10 +679,13 @@ template <typename F> hipError_t launch_f(const SharedCall &c, void *workspace, 
     a.psplits = p.psplits;
     a.otiles = p.otiles;
     a.osplits = p.osplits;
+    a.pper = p.pper;
+    a.oper = p.oper;
+    a.omost = p.omost;
     a.c = kLog2e / sqrtf(float(c.d));
     // Rows of a load instruction: 64 lanes of 16 bytes; lane offsets are 32 bits from the first of them.
     const int64_t rows_per_load = kWave * 16 / (a.dp * e);
-    a.one_page = c.page_size >= rows_per_load && a.k.token == a.v.token && a.k.token >= 0 && a.k.token < (int64_t(1) << 26);
+    a.one_page = c.page_size >= rows_per_load && a.k.token < (int64_t(1) << 26) && a.v.token < (int64_t(1) << 26);
     hipError_t rc;
     if (a.dp == 32) rc = a.width == 32 * e ? launch_d<F, 32, false>(a, p, stream) : launch_d<F, 32, true>(a, p, stream);
     else if (a.dp == 64) rc = a.width == 64 * e ? launch_d<F, 64, false>(a, p, stream) : launch_d<F, 64, true>(a, p, stream);
