@@ -9,13 +9,22 @@
 // workgroups; every workgroup leaves O (not yet divided), m and l in fp32 in the workspace, and a second launch joins
 // them.
 //
-// The walk itself is that of the packed attention forward: 4 waves, S^T = K Q^T so that a lane holds one row,
-// P in the accumulators' own order as operand of O^T += V^T P^T, the maximum raised only when a block exceeds it
-// by 2^8 (fp16 2^15), two LDS buffers filled by direct global -> LDS loads.  Loads find their rows through the page
-// table: where a load instruction's rows lie in one page (pages of at least 64 rows / (16-byte chunks a row)), the page
-// is looked up once a wave a block ahead, and the load takes it as a scalar base with fixed lane offsets; smaller pages and the
-// last block look up every lane's row.  P is rounded to 16 bits for the second product (the MFMA's operand type); l
-// adds the unrounded values.
+// The walk itself is that of the packed attention forward: S^T = K Q^T so that a lane holds one row, P in the
+// accumulators' own order as operand of O^T += V^T P^T, the maximum raised only when a block exceeds it by 2^8 (fp16
+// 2^15), tiles filled by direct global -> LDS loads.  128-row tiles are a workgroup's, whose 4 waves walk the same keys
+// through two buffers; where rows are fewer a wave walks its own stretch of keys for 32 rows by itself, with no barrier, K of
+// the next 32 keys on its way while it adds V of these.  (Four waves of a workgroup that walked a quarter each and joined
+// in LDS: 226 us and 72 for the requests' own keys of the two cases below, waves apart 220 and 71.)  Loads find their
+// rows through the page table: where a load instruction's rows lie in one page (pages of at least 64 rows / (16-byte chunks a
+// row)), the page is a scalar load a block ahead, and the load takes it as scalar base with fixed lane offsets;
+// smaller pages and a stretch's last block look up every lane's row.  P is rounded to 16 bits for the second product (the
+// MFMA's operand type); l adds the unrounded values.
+//
+// Measured, bf16, 32/8 heads of 128, one token a request: 256 requests of 1 to 2048 own tokens on a prompt of 32768 keys
+// 305 us (3.95 TB/s, 463 TFLOP/s, of a floor of 235 by bytes), their own keys alone 220 (4.9 TB/s, HBM), the prompt alone 175
+// (786 TFLOP/s, 35 % of the matrix cores' cycles with the launch's ends in them); 8 prompts of up to 2000 keys, 16 requests of 1 to 1024
+// each 80 us (4.07 TB/s, floor 64).  Deeper tile or operand prefetch changed neither (3 buffers of 64 keys, 4 and 5 of 32, 1 to 4 operands
+// ahead: 175 to 205 us for the prompt).
 #include "attn_launch.h"
 #include "attn_packed_tiles.h"
 #include "attn_shared.h"
@@ -69,8 +78,8 @@ struct Args {
     float c;         // log2(e) / sqrt(d)
 };
 
-// Rows of a tile: 128, of which each of the 4 waves takes 32 and all walk the same keys (tall), or 32, of whose keys every
-// wave walks a quarter.
+// Rows of a tile: 128, of which each of a workgroup's 4 waves takes 32 and all walk the same keys (tall), or 32 of a wave by
+// itself (flat).
 template <typename F, int D> struct Base {
     static constexpr int NW = 4;
     static constexpr int DT = D / 32;
@@ -92,7 +101,7 @@ template <typename F, int D> struct Tall : Base<F, D> {
 template <typename F, int D> struct Flat : Base<F, D> {
     using B = Base<F, D>;
     static constexpr int BM = 32;
-    static constexpr int BN = 32 * B::NW;  // of the workgroup; 32 keys a wave
+    static constexpr int BN = 32;
     static constexpr int KB = 32 * B::RB;
     static constexpr int LDS = B::NW * 2 * KB;  // a wave's K with V behind it
     static constexpr int NL = 32 / B::RPL;
@@ -432,13 +441,12 @@ template <int N> __device__ __forceinline__ void wait_loads_but() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// 32 rows, whose keys the waves walk apart, 32 of every block of 128 each, through LDS of their own: no barriers, and a
-// wave's next K is on its way while it adds V, its next V while it computes scores.
+// 32 rows of a wave by itself, through LDS of its own: no barriers, and the next K is on its way while V is added, the next
+// V while scores are computed.
 template <typename F, int D, bool PAD>
-__device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const int kvh, char *smem) {
+__device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const int kvh, const uint32_t kt) {
     using C = Flat<F, D>;
     const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane & 31, half = lane >> 5;
     const int group = a.lay.group, rows = it.tokens * group;
     const int row = it.r0 + col;
@@ -449,17 +457,15 @@ __device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const i
     const int end = seen((min(it.r0 + C::BM, rows) - 1) / group);
     WaveState<F, D> w;
     w.template init<PAD>(a.q.at(it.first + token, head), row < rows, a.width, half);
-    const uint32_t kt = lds_addr(smem) + uint32_t(wave * 2 * C::KB), vt = kt + uint32_t(C::KB);
+    const uint32_t vt = kt + uint32_t(C::KB);
     const uint32_t rk = kt + uint32_t(C::L::off(col, half));
     const uint32_t cv0 = vt + F::template col0<C::RB>(lane), cv1 = vt + F::template col1<C::RB>(lane);
     PagedLoads<Base<F, D>, C::NL, PAD> loads(a, it, kvh, 0, lane);
-    clear_padding<PAD, C::LDS>(smem);
 
-    // This wave's blocks begin at keys 32 wave + 128 n.
-    int j0 = 32 * wave;
+    int j0 = 0;
     bool fast = false;
     const auto load_k = [&](int j) __attribute__((always_inline)) {
-        fast = loads.fast(j, 32, end);
+        fast = loads.fast(j, C::BN, end);
         if (fast) {
             loads.load(loads.k, a.k, kt, j, end, true);
         } else {
@@ -471,10 +477,10 @@ __device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const i
         if (fast) loads.load(loads.v, a.v, vt, j, end, true);
         else loads.load(loads.v, a.v, vt, j, end, false);
     };
-    if (j0 < end) {
-        loads.look_up(j0, end);
-        load_k(j0);
-        load_v(j0);
+    if (end > 0) {
+        loads.look_up(0, end);
+        load_k(0);
+        load_v(0);
         while (true) {
             const int next = j0 + C::BN;
             const bool more = next < end;
@@ -488,7 +494,7 @@ __device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const i
                 loads.look_up(next, end);
                 load_k(next);
             }
-            if (j0 + 32 > whole) {
+            if (next > whole) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                     if (j0 + acc_row(r, half) >= row_end) c[0][r] = -INFINITY;
@@ -503,36 +509,6 @@ __device__ __forceinline__ void walk_flat(const Args &a, const Item &it, const i
             j0 = next;
         }
     }
-
-    // The waves join: m = max, O and l weighted by 2^(their m - m).  A wave that saw no key has the lowest m and l = 0.
-    constexpr int KS = C::NW, NR = C::DT * 16 + 2;
-    static_assert((KS - 1) * NR * kWave * 4 <= C::LDS, "join buffer");
-    float *jb = reinterpret_cast<float *>(smem);
-    lds_barrier();  // every wave is done with its tiles
-    if (wave > 0) {
-        float *to = jb + (wave - 1) * NR * kWave + lane;
-#pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) to[(dt * 16 + r) * kWave] = w.o[dt][r];
-        to[(NR - 2) * kWave] = w.m;
-        to[(NR - 1) * kWave] = w.l;
-    }
-    lds_barrier();
-    if (wave > 0) return;
-    // One after the other: all at once take more registers than there are.
-#pragma unroll 1
-    for (int i = 0; i < KS - 1; ++i) {
-        const float *from = jb + i * NR * kWave + lane;
-        const float mi = from[(NR - 2) * kWave], m = fmaxf(w.m, mi);
-        const float x = fast_exp2(w.m - m), y = fast_exp2(mi - m);
-        w.m = m;
-        w.l = w.l * x + from[(NR - 1) * kWave] * y;
-#pragma unroll
-        for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w.o[dt][r] = w.o[dt][r] * x + from[(dt * 16 + r) * kWave] * y;
-    }
     if (row < rows) w.template leave<PAD>(a, it, token, head, half, row_end > 0);
 }
 
@@ -546,22 +522,34 @@ template <typename F, int D, bool PAD, bool TP, bool TO>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Both<F, D, TP, TO>::WPE, 2))) void shared_kernel(Args a) {
     __shared__ __attribute__((aligned(1024))) char smem[Both<F, D, TP, TO>::LDS];
     const int hkv = a.lay.hkv;
-    const int kvh = blockIdx.x % hkv;
-    int slot = blockIdx.x / hkv;
+    const int pitems = a.ptiles * a.psplits * hkv, oitems = a.otiles * a.osplits * hkv;
     Item it;
-    const auto walk = [&](auto tall) __attribute__((always_inline)) {
-        if constexpr (decltype(tall)::value) walk_tall<F, D, PAD>(a, it, kvh, smem);
-        else walk_flat<F, D, PAD>(a, it, kvh, smem);
-    };
-    using P = std::conditional_t<TP, Tall<F, D>, Flat<F, D>>;
-    using O = std::conditional_t<TO, Tall<F, D>, Flat<F, D>>;
-    if (slot < a.ptiles * a.psplits) {
-        if (!prefix_item<P::BM, P::BN>(a, slot % a.ptiles, slot / a.ptiles, it)) return;
-        walk(std::bool_constant<TP>{});
+    if (TP && int(blockIdx.x) < pitems) {
+        const int slot = blockIdx.x / hkv;
+        if (prefix_item<Tall<F, D>::BM, Tall<F, D>::BN>(a, slot % a.ptiles, slot / a.ptiles, it))
+            walk_tall<F, D, PAD>(a, it, blockIdx.x % hkv, smem);
+        return;
+    }
+    if constexpr (TO) {
+        const int x = blockIdx.x - pitems, slot = x / hkv;
+        if (own_item<Tall<F, D>::BM, Tall<F, D>::BN>(a, slot % a.otiles, slot / a.otiles, it))
+            walk_tall<F, D, PAD>(a, it, x % hkv, smem);
     } else {
-        slot -= a.ptiles * a.psplits;
-        if (!own_item<O::BM, O::BN>(a, slot % a.otiles, slot / a.otiles, it)) return;
-        walk(std::bool_constant<TO>{});
+        // A wave's item: the key heads of a tile and stretch beside each other, prompts' before own.
+        clear_padding<PAD, Flat<F, D>::LDS>(smem);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        int x = (int(blockIdx.x) - (TP ? pitems : 0)) * 4 + wave;
+        const uint32_t tile = lds_addr(smem) + uint32_t(wave * 2 * Flat<F, D>::KB);
+        bool there;
+        if (!TP && x < pitems) {
+            const int slot = x / hkv;
+            there = prefix_item<Flat<F, D>::BM, Flat<F, D>::BN>(a, slot % a.ptiles, slot / a.ptiles, it);
+        } else {
+            if (!TP) x -= pitems;
+            const int slot = x / hkv;
+            there = x < oitems && own_item<Flat<F, D>::BM, Flat<F, D>::BN>(a, slot % a.otiles, slot / a.otiles, it);
+        }
+        if (there) walk_flat<F, D, PAD>(a, it, x % hkv, tile);
     }
 }
 
@@ -618,6 +606,14 @@ struct Plan {
     bool tall_prefix, tall_own;
     int ptiles, psplits, otiles, osplits, pper, oper, omost;
 };
+// A request's own keys that one work item takes, where `tiles` tiles of rows and key heads have up to `most` each.  Flat:
+// 4096 waves, two for every wave's place, and no more than 512 keys a wave, for lengths differ (256 requests of 1 to 2048
+// keys, 8 key heads of 128: 128 / 256 / 512 / 1024 keys 226 / 220 / 220 / 238 us; 128 requests of 1 to 1024:
+// 69 / 71 / 70 / 84).  At most 64 stretches.
+int64_t keys_each(int64_t tiles, int64_t most, bool tall) {
+    const int64_t x = tiles * most / 4096, lo = tall ? 256 : 64, hi = tall ? 1024 : 512;
+    return (std::max(std::min(std::max(x, lo), hi), most / 64) + 63) / 64 * 64;
+}
 Plan plan_of(const SharedCall &c) {
     Plan p{};
     const int64_t work_rows = c.rows * c.group();
@@ -628,19 +624,19 @@ Plan plan_of(const SharedCall &c) {
         const int64_t bm = p.tall_own ? 128 : 32;
         p.oper = c.starts ? 0 : int(div(c.group(), bm));
         p.otiles = int(p.oper > 0 ? p.oper * c.requests : work_rows / bm + c.requests);
-        const int64_t wgs = p.otiles * c.hkv;
-        if (wgs >= 512) {
-            p.omost = int(std::max<int64_t>(512, div(div(c.max_own(), 16), 128) * 128));
-            p.osplits = int(std::max<int64_t>(1, div(c.max_own(), p.omost)));
-        } else {
-            p.osplits = int(std::max<int64_t>(1, std::min({int64_t(128), 1024 / wgs, div(c.max_own(), 128)})));
-        }
+        p.omost = int(keys_each(p.otiles * c.hkv, c.max_own(), p.tall_own));
+        p.osplits = int(std::max<int64_t>(1, div(c.max_own(), p.omost)));
     }
     if (c.max_prefix() > 0) {
         const int64_t bm = p.tall_prefix ? 128 : 32;
         p.pper = c.starts || c.group_starts ? 0 : int(div(c.requests / c.groups * c.group(), bm));
         p.ptiles = int(p.pper > 0 ? p.pper * c.groups : c.groups == 1 ? div(work_rows, bm) : work_rows / bm + c.groups);
-        p.psplits = int(std::max<int64_t>(1, std::min({int64_t(128), 512 / std::max<int64_t>(1, p.ptiles * c.hkv), div(c.max_prefix(), 128)})));
+        // Tall: a workgroup a CU where the requests' own keys are as many, so that these stream in beside it, and two
+        // where not (32768 keys, 1024 rows of 8 key heads, with 1 to 2048 keys of 256 requests' own: 306 us with 256
+        // workgroups, 377 with 512; without: 211 and 175).
+        const bool beside = !p.tall_own && c.requests * c.max_own() >= c.groups * c.max_prefix();
+        const int64_t items = p.tall_prefix ? (beside ? 256 : 512) : 2048, least = p.tall_prefix ? 128 : 64;
+        p.psplits = int(std::max<int64_t>(1, std::min({int64_t(128), items / std::max<int64_t>(1, p.ptiles * c.hkv), div(c.max_prefix(), least)})));
     }
     return p;
 }
@@ -648,7 +644,10 @@ int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t dp_of(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 template <typename F, int D, bool PAD> hipError_t launch_d(const Args &a, const Plan &p, hipStream_t stream) {
-    const int64_t blocks = (int64_t(p.ptiles) * p.psplits + int64_t(p.otiles) * p.osplits) * a.lay.hkv;
+    const int64_t prompts = int64_t(p.ptiles) * p.psplits * a.lay.hkv, own = int64_t(p.otiles) * p.osplits * a.lay.hkv;
+    if (prompts + own > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const int64_t flat = (p.tall_own ? 0 : own) + (p.tall_prefix ? 0 : prompts);  // waves
+    const int64_t blocks = (p.tall_prefix ? prompts : 0) + (p.tall_own ? own : 0) + (flat + 3) / 4;
     if (!grid_fits(blocks, 256)) return hipErrorInvalidValue;
     if (blocks > 0) {
         const dim3 grid(static_cast<unsigned>(blocks)), block(256);
