@@ -34,6 +34,16 @@ constexpr int kList = 2048;       // tokens ranked in LDS
 constexpr int kBins = 1024;
 constexpr double kLog2e64 = 1.4426950408889634074;
 
+// A row whose border is found by all of the chip: tokens and w (in integers) of bins over x, and the tokens of the border's bin.
+struct Wide {
+    uint64_t mass[kBins];
+    uint64_t list[kList];
+    uint32_t cnt[kBins];
+    double whole;
+    float top;
+    int32_t count;
+};
+
 struct SampleArgs {
     const void *logits;
     const float *u;
@@ -47,11 +57,18 @@ struct SampleArgs {
     double *piece_sum;
     int64_t stride;
     int vocab, pieces, each;  // each: pieces of a wave of the first pass
+    Wide *wide;               // of the rows put off, up to `most` of them
+    int32_t *put_off;         // their number, and the rows
+    int most;
 };
 
+// exp((x - m) / t) as 2^((x - m) s).  Below `floor` it is 0.
+struct Scale {
+    double s, floor;
+};
 struct Row {
-    double t;      // the temperature of w: 1 for a greedy row
-    double scale;  // log2(e) / t
+    double t;  // the temperature of w: 1 for a greedy row
+    Scale scale;
     bool greedy;
 };
 __device__ __forceinline__ Row row_of(const SampleArgs &a, int64_t row) {
@@ -59,15 +76,18 @@ __device__ __forceinline__ Row row_of(const SampleArgs &a, int64_t row) {
     Row r;
     r.greedy = !(t > 0.0);
     r.t = r.greedy ? 1.0 : t;
-    r.scale = kLog2e64 / r.t;
+    r.scale.s = fmax(kLog2e64 / r.t, 1e-290);  // an infinite t too leaves -inf below the floor
+    r.scale.floor = -1100.0 / r.scale.s;
     return r;
 }
 
-// exp((x - m) / t), 1 where x is m (infinite too), 0 for x = -inf.  (2^f - 1) / f on [-1/2, 1/2] is a polynomial of
-// degree 8 through its values at the Chebyshev points, so that 2^0 is 1 exactly.
-__device__ __forceinline__ double weight(float x, float m, double scale) {
-    const double e = x == m ? 0.0 : fmax((double(x) - double(m)) * scale, -1100.0);
-    const double n = rint(e), f = e - n;
+// w for finite m: 1 where x is m, 0 for x = -inf.  (2^f - 1) / f on [-1/2, 1/2] is a polynomial of degree 8 through its
+// values at the Chebyshev points, so that 2^0 is 1 exactly.  Adding 1.5 2^52 rounds to an integer, in the low word.
+__device__ __forceinline__ double weight_finite(float x, double m, const Scale &c) {
+    constexpr double kMagic = 6755399441055744.0;
+    const double d = fmax(double(x) - m, c.floor);
+    const double t = fma(d, c.s, kMagic);
+    const double f = fma(d, c.s, kMagic - t);
     double p = 1.0203121063391729e-07;
     p = fma(p, f, 1.3255224878668817e-06);
     p = fma(p, f, 1.525268684626772e-05);
@@ -77,7 +97,66 @@ __device__ __forceinline__ double weight(float x, float m, double scale) {
     p = fma(p, f, 0.055504108664760424);
     p = fma(p, f, 0.24022650695812989);
     p = fma(p, f, 0.69314718055994529);
-    return ldexp(fma(p, f, 1.0), int(n));
+    return ldexp(fma(p, f, 1.0), __double2loint(t));
+}
+// An infinite m is the value of all that is not 0.
+__device__ __forceinline__ double weight(float x, float m, const Scale &c) {
+    return m == INFINITY ? (x == m ? 1.0 : 0.0) : weight_finite(x, double(m), c);
+}
+
+// What a row draws from: the first k ranks, `share` of their w (above 1: all), w of at least `least`.
+struct Choice {
+    int64_t k;
+    double share, least;
+    float u;
+};
+__device__ __forceinline__ Choice choice_of(const SampleArgs &a, int64_t row, bool greedy) {
+    Choice c;
+    c.u = a.u != nullptr ? a.u[row] : 0.f;
+    if (!(c.u >= 0.f)) c.u = 0.f;
+    c.k = a.top_k != nullptr ? int64_t(a.top_k[row]) : a.top_k_all;
+    const double p = a.top_p != nullptr ? double(a.top_p[row]) : a.top_p_all;
+    c.share = p < 1.0 ? p : 2.0;
+    c.least = a.min_p != nullptr ? double(a.min_p[row]) : a.min_p_all;
+    if (!(c.least > 0.0)) c.least = 0.0;
+    if (c.k <= 0 || c.k > a.vocab) c.k = a.vocab;
+    if (greedy || c.share <= 0.0 || c.least > 1.0) c.k = 1;
+    return c;
+}
+__device__ __forceinline__ void finish_row(const SampleArgs &a, int64_t row, int64_t token, float value, float top, double t, double whole) {
+    a.tokens[row] = token;
+    const double d = value == top ? 0.0 : (double(value) - double(top)) / t;
+    a.logprobs[row] = float(d - log(whole));
+}
+
+// A double's two words of the lane that DPP control CTRL names, and the sum over a wave in every lane, as wave_sum_dpp.
+template <int CTRL> __device__ __forceinline__ double dpp64(double x) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, 0xf, 0xf, true),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ double wave_sum64(double x) {
+    x += dpp64<0xB1>(x);
+    x += dpp64<0x4E>(x);
+    x += dpp64<0x141>(x);
+    x += dpp64<0x140>(x);
+    uint32_t lo = uint32_t(__double2loint(x)), hi = uint32_t(__double2hiint(x));
+    auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    auto h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    x = __hiloint2double(int(h[0]), int(l[0])) + __hiloint2double(int(h[1]), int(l[1]));
+    lo = uint32_t(__double2loint(x));
+    hi = uint32_t(__double2hiint(x));
+    l = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    return __hiloint2double(int(h[0]), int(l[0])) + __hiloint2double(int(h[1]), int(l[1]));
+}
+template <typename A> __device__ __forceinline__ A wave_scan(A x) {
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const A y = __shfl_up(x, off, kWave);
+        if (lane >= off) x += y;
+    }
+    return x;
 }
 
 // 8 logits of a lane; past the row's end and where there is none -inf; -0 becomes 0.
@@ -94,7 +173,7 @@ template <typename T> struct Eight {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float y = Gran<T>::get(g[e / Gran<T>::EPC], e % Gran<T>::EPC);
-            x[e] = y == y ? y + 0.f : -INFINITY;
+            x[e] = fmaxf(y, -INFINITY) + 0.f;  // fmaxf takes the number of a NaN and a number
         }
     }
 };
@@ -109,24 +188,31 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 }
 
 // A piece's maximum and its sum of w relative to it, the same in every lane.
-__device__ __forceinline__ void piece_stats(const float (&x)[8], double scale, float &m, double &s) {
+__device__ __forceinline__ void piece_stats(const float (&x)[8], const Scale &c, float &m, double &s) {
     m = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
-    m = wave_max(m);
+    m = wave_max_dpp(m);
     s = 0.0;
     if (m == -INFINITY) return;
+    if (m == INFINITY) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += weight(x[e], m, scale);
-    s = wave_sum(s);
+        for (int e = 0; e < 8; ++e) s += x[e] == m ? 1.0 : 0.0;
+    } else {
+        const double md = double(m);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += weight_finite(x[e], md, c);
+    }
+    s = wave_sum64(s);
 }
 
 template <typename T> __global__ __launch_bounds__(256) void sample_stats_kernel(SampleArgs a) {
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     const int64_t row = blockIdx.y;
     const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-    const double scale = row_of(a, row).scale;
+    const Scale scale = row_of(a, row).scale;
     const int p0 = (blockIdx.x * 4 + wave) * a.each, p1 = p0 + a.each < a.pieces ? p0 + a.each : a.pieces;
+    if (a.put_off != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.put_off[0] = 0;
     if (p0 >= p1) return;
     Eight<T> now, next;
     next.load(x, p0, a.vocab);
@@ -155,42 +241,41 @@ struct Shared {
         uint64_t comp[kList];  // (key, ~id)
     };
     double w[kList];
-    uint64_t sorted[kList];
+    uint64_t sums[kMaxPieces];
+    uint32_t sub[kBins];
     uint64_t scratch[2 * kWaves];
     int32_t found, count;
     uint32_t key;
-    double sum;
     int64_t token;
 };
 
-// Running sums of a[0 .. n), in place, in one order.
-template <typename A> __device__ void scan_array(A *a, int n, uint64_t *scratch) {
+// Running sums of a[0 .. n), n up to N, in place, in one order.
+template <int N, typename A> __device__ __forceinline__ void scan_array(A *a, int n, uint64_t *scratch) {
+    constexpr int Q = (N + kThreads - 1) / kThreads;
     A *waves = reinterpret_cast<A *>(scratch);
     const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
-    const int q = (n + kThreads - 1) / kThreads, i0 = t * q, i1 = i0 + q < n ? i0 + q : n;
-    A s = 0;
-    for (int i = i0; i < i1; ++i) s += a[i];
+    const int q = (n + kThreads - 1) / kThreads, i0 = t * q;
+    A r[Q];
 #pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const A y = __shfl_up(s, off, kWave);
-        if (lane >= off) s += y;
-    }
-    __syncthreads();
+    for (int i = 0; i < Q; ++i) r[i] = i < q && i0 + i < n ? a[i0 + i] : A(0);
+#pragma unroll
+    for (int i = 1; i < Q; ++i) r[i] += r[i - 1];
+    const A s = wave_scan(r[Q - 1]);
     if (lane == kWave - 1) waves[wave] = s;
     __syncthreads();
     A run = __shfl_up(s, 1, kWave);
     if (lane == 0) run = 0;
     A before = 0;
-    for (int w = 0; w < wave; ++w) before += waves[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) before += w < wave ? waves[w] : A(0);
     run += before;
-    for (int i = i0; i < i1; ++i) {
-        run += a[i];
-        a[i] = run;
-    }
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+        if (i < q && i0 + i < n) a[i0 + i] = run + r[i];
     __syncthreads();
 }
 // The first i of [0, n) that holds, or n, in every thread.
-template <typename Fn> __device__ int first_of(int n, Shared &sh, Fn holds) {
+template <typename Fn> __device__ __forceinline__ int first_of(int n, Shared &sh, Fn holds) {
     __syncthreads();
     if (threadIdx.x == 0) sh.found = n;
     __syncthreads();
@@ -202,23 +287,62 @@ template <typename Fn> __device__ int first_of(int n, Shared &sh, Fn holds) {
     __syncthreads();
     return sh.found;
 }
-// The row's pieces, one after the other a wave's, the next one's loads ahead; fn(piece, values).
+// The wanted pieces, spread over the waves, three pieces' loads ahead; fn(piece, values, first id).
 template <typename T, typename Want, typename Fn>
 __device__ __forceinline__ void each_piece(const T *x, int pieces, int vocab, Want want, Fn fn) {
-    int p = threadIdx.x / kWave;
-    while (p < pieces && !want(p)) p += kWaves;
-    Eight<T> now, next;
-    if (p < pieces) next.load(x, p, vocab);
-    while (p < pieces) {
-        now = next;
-        int q = p + kWaves;
-        while (q < pieces && !want(q)) q += kWaves;
-        if (q < pieces) next.load(x, q, vocab);
+    constexpr int N = 3;
+    Eight<T> ahead[N];
+    int at[N], p = threadIdx.x / kWave;
+    const auto fetch = [&](int i) {
+        while (p < pieces && !want(p)) p += kWaves;
+        at[i] = p;
+        if (p < pieces) ahead[i].load(x, p, vocab);
+        p += kWaves;
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) fetch(i);
+    while (at[0] < pieces) {
+        const Eight<T> now = ahead[0];
+        const int here = at[0];
+#pragma unroll
+        for (int i = 0; i + 1 < N; ++i) {
+            ahead[i] = ahead[i + 1];
+            at[i] = at[i + 1];
+        }
+        fetch(N - 1);
         float v[8];
         now.get(v);
-        fn(p, v, now.c0);
-        p = q;
+        fn(here, v, now.c0);
     }
+}
+
+// 1024 bins over x, 32 to a factor of two in w; the first holds the largest, the last all of the rest.
+struct Bins {
+    float m, by;
+    __device__ __forceinline__ int of(float v) const { return v == m ? 0 : int(fminf((m - v) * by, float(kBins - 1))); }
+    // The lowest key of a bin <= at_most: the bins fall with the key.
+    __device__ uint32_t edge(int at_most) const {
+        uint32_t p = key_of(-INFINITY), q = key_of(m);
+        while (p < q) {
+            const uint32_t mid = p + (q - p) / 2;
+            if (of(value_of(mid)) <= at_most) q = mid;
+            else p = mid + 1;
+        }
+        return p;
+    }
+    __device__ uint32_t lowest(int b) const { return edge(b); }
+    __device__ uint32_t highest(int b) const { return b > 0 ? edge(b - 1) - 1 : key_of(m); }
+};
+__device__ __forceinline__ Bins bins_of(float m, const Scale &scale) { return {m, float(scale.s * 32.0)}; }
+// w in integers, whose sums do not depend on their order: the whole row's sum takes 62 bits, half a step a token is lost.
+struct Fixed {
+    double fix, unfix;
+    __device__ __forceinline__ uint64_t of(double w) const { return uint64_t(fma(w, fix, 0.5)); }
+    __device__ __forceinline__ double sum(uint64_t x) const { return double(x) * unfix; }
+};
+__device__ __forceinline__ Fixed fixed_of(double whole) {
+    const int bits = ilogb(whole) + 1;
+    return {ldexp(1.0, 62 - bits), ldexp(1.0, bits - 62)};
 }
 
 // Which tokens a draw takes: keys above `key` and the first `ties` ids of that key, of w at least `least`.
@@ -231,7 +355,7 @@ struct Kept {
 // The first token of a piece at which `base` and the sum of kept w pass `target` (the last with any, where rounding
 // lets none; none, where the piece has none), by one wave.  `before`: tokens of the border's key in earlier pieces.
 template <typename T>
-__device__ void draw_in_piece(const T *x, int piece, int vocab, float m, double scale, const Kept &k, int64_t before,
+__device__ __forceinline__ void draw_in_piece(const T *x, int piece, int vocab, float m, const Scale &scale, const Kept &k, int64_t before,
                               double base, double target, Shared &sh) {
     const int lane = threadIdx.x & (kWave - 1);
     Eight<T> g;
@@ -286,49 +410,91 @@ __device__ void draw_in_piece(const T *x, int piece, int vocab, float m, double 
     }
 }
 
-// Ranks the n listed tokens (comp): sorted[rank] = comp, w[rank] = its weight.  Thread t keeps its own tokens' ranks.
-__device__ __forceinline__ void rank_list(Shared &sh, int n, float m, double scale, uint64_t (&mine)[4], int (&rank)[4], int (&place)[4]) {
+// Sorts the n listed tokens (comp) by rank, and puts their weights beside them (w).  Few by counting those before each,
+// many by a bitonic network (2048: 66 steps, about 10 us; counting takes 130).
+__device__ __forceinline__ void sort_list(Shared &sh, int n, float m, const Scale &scale) {
     const int t = threadIdx.x;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        mine[k] = t + k * kThreads < n ? sh.comp[t + k * kThreads] : 0;
-        rank[k] = place[k] = 0;
-    }
-    // Beside the rank by value the place by id: ids are complemented in the low half.
-    const int used = (n + kThreads - 1) / kThreads;
-    for (int j = 0; j < n; ++j) {
-        const uint64_t c = sh.comp[j];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (k >= used) break;
-            rank[k] += c > mine[k] ? 1 : 0;
-            place[k] += uint32_t(c) > uint32_t(mine[k]) ? 1 : 0;
+    if (n <= kThreads) {
+        const uint64_t mine = t < n ? sh.comp[t] : 0;
+        int rank = 0;
+        if (t < n) {
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) rank += sh.comp[j] > mine ? 1 : 0;
         }
+        __syncthreads();
+        if (t < n) sh.comp[rank] = mine;
+    } else {
+        int size = 2 * kThreads;
+        while (size < n) size *= 2;
+        for (int i = n + t; i < size; i += kThreads) sh.comp[i] = 0;
+        for (int k = 2; k <= size; k *= 2)
+            for (int j = k / 2; j > 0; j /= 2) {
+                __syncthreads();
+                for (int q = t; q < size / 2; q += kThreads) {
+                    const int i = 2 * (q & ~(j - 1)) + (q & (j - 1));
+                    const uint64_t x = sh.comp[i], y = sh.comp[i + j];
+                    if ((x < y) == ((i & k) == 0)) {
+                        sh.comp[i] = y;
+                        sh.comp[i + j] = x;
+                    }
+                }
+            }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (t + k * kThreads < n) {
-            sh.sorted[rank[k]] = mine[k];
-            sh.w[rank[k]] = weight(value_of(uint32_t(mine[k] >> 32)), m, scale);
-        }
     __syncthreads();
+    for (int i = t; i < n; i += kThreads) sh.w[i] = weight(value_of(uint32_t(sh.comp[i] >> 32)), m, scale);
+    __syncthreads();
+}
+__device__ __forceinline__ uint32_t list_key(const Shared &sh, int i) { return uint32_t(sh.comp[i] >> 32); }
+__device__ __forceinline__ int list_id(const Shared &sh, int i) { return int(~uint32_t(sh.comp[i])); }
+
+// The first `keep` listed tokens are kept: the border that says so, and their w, where it is at least `least`, added to
+// their pieces' sums in ps, through sums.  In 64-bit integers (the whole row's sum takes 62 bits), whose sum does not
+// depend on the order of the atomics.
+__device__ __forceinline__ void keep_listed(Shared &sh, int n, int keep, int pieces, float m, const Scale &scale, double whole, Kept &kept) {
+    const int t = threadIdx.x;
+    const uint32_t key = list_key(sh, keep - 1);
+    const int first = first_of(n, sh, [&](int i) { return list_key(sh, i) == key; });
+    kept.key = key;
+    kept.ties = keep - first;
+    const Fixed f = fixed_of(whole);
+    for (int i = t; i < keep; i += kThreads) {
+        const double w = weight(value_of(list_key(sh, i)), m, scale);
+        if (w >= kept.least)
+            atomicAdd(reinterpret_cast<unsigned long long *>(&sh.sums[list_id(sh, i) / kPiece]), (unsigned long long)f.of(w));
+    }
+    __syncthreads();
+    for (int p = t; p < pieces; p += kThreads) sh.ps[p] += f.sum(sh.sums[p]);
+    __syncthreads();
+}
+// Lists a piece's tokens with lo <= key <= hi, one atomic a wave; the order in the list is arbitrary.
+__device__ __forceinline__ void append(Shared &sh, const float (&v)[8], int c0, int vocab, uint32_t lo, uint32_t hi) {
+    uint64_t in[8];
+    int total = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t key = key_of(v[e]);
+        in[e] = __ballot(c0 + e < vocab && key >= lo && key <= hi);
+        total += __popcll(in[e]);
+    }
+    if (total == 0) return;
+    const int lane = threadIdx.x & (kWave - 1);
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh.count, total);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int mine = at + int(__builtin_amdgcn_mbcnt_hi(uint32_t(in[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(in[e]), 0)));
+        if ((in[e] >> lane & 1) && mine < kList) sh.comp[mine] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(c0 + e));
+        at += __popcll(in[e]);
+    }
 }
 // Lists the tokens with lo <= key <= hi of the wanted pieces; their number, which may pass the list's length.
 template <typename T, typename Want>
-__device__ int collect(const T *x, int pieces, int vocab, uint32_t lo, uint32_t hi, Want want, Shared &sh) {
+__device__ __forceinline__ int collect(const T *x, int pieces, int vocab, uint32_t lo, uint32_t hi, Want want, Shared &sh) {
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    each_piece(x, pieces, vocab, want, [&](int, const float (&v)[8], int c0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t key = key_of(v[e]);
-            if (c0 + e < vocab && key >= lo && key <= hi) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kList) sh.comp[at] = uint64_t(key) << 32 | uint32_t(~(c0 + e));
-            }
-        }
-    });
+    each_piece(x, pieces, vocab, want, [&](int, const float (&v)[8], int c0) { append(sh, v, c0, vocab, lo, hi); });
     __syncthreads();
     return sh.count;
 }
@@ -342,13 +508,10 @@ struct Border {
 // The border of a run of ranks: the first `want` of them (by_count), or those whose sum of w before them is less than
 // `share` of the whole row's (by_mass: share of `of`, or of the row where that is negative).
 template <typename T>
-__device__ Border find_border(const T *x, const SampleArgs &a, float m, double scale, double whole, bool by_count, int64_t want,
+__device__ __forceinline__ Border find_border(const T *x, const SampleArgs &a, float m, const Scale &scale, double whole, bool by_count, int64_t want,
                               double share, double of, Shared &sh) {
-    // The whole row's sum takes 62 bits, half a step a token is lost.
-    const int bits = ilogb(whole) + 1;
-    const double fix = ldexp(1.0, 62 - bits), unfix = ldexp(1.0, bits - 62);
-    const float bins = float(scale * 32.0);  // 32 bins to a factor of two in w
-    const auto linear = [&](float v) { return v == m ? 0 : int(fminf((m - v) * bins, float(kBins - 1))); };
+    const Fixed f = fixed_of(whole);
+    const Bins bins = bins_of(m, scale);
     uint32_t lo = 0, hi = 0xFFFFFFFFu;
     int shift = -1;  // bins over x first, then over keys
     int64_t before = 0;
@@ -366,19 +529,19 @@ __device__ Border find_border(const T *x, const SampleArgs &a, float m, double s
             for (int e = 0; e < 8; ++e) {
                 const uint32_t key = key_of(v[e]);
                 if (c0 + e < a.vocab && key >= lo && key <= hi) {
-                    const int b = shift < 0 ? linear(v[e]) : int((hi - key) >> shift);
+                    const int b = shift < 0 ? bins.of(v[e]) : int((hi - key) >> shift);
                     atomicAdd(&sh.cnt[b], 1u);
-                    const uint64_t w = uint64_t(fma(weight(v[e], m, scale), fix, 0.5));
+                    const uint64_t w = f.of(weight(v[e], m, scale));
                     if (w != 0) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)w);
                 }
             }
         });
         __syncthreads();
-        scan_array(sh.cnt, kBins, sh.scratch);
-        scan_array(sh.mass, kBins, sh.scratch);
-        if (shift < 0 && !by_count && of < 0.0) target = share * (double(sh.mass[kBins - 1]) * unfix);
+        scan_array<kBins>(sh.cnt, kBins, sh.scratch);
+        scan_array<kBins>(sh.mass, kBins, sh.scratch);
+        if (shift < 0 && !by_count && of < 0.0) target = share * (f.sum(sh.mass[kBins - 1]));
         int b = first_of(kBins, sh, [&](int i) {
-            return by_count ? before + int64_t(sh.cnt[i]) >= want : double(mass + sh.mass[i]) * unfix >= target;
+            return by_count ? before + int64_t(sh.cnt[i]) >= want : f.sum(mass + sh.mass[i]) >= target;
         });
         if (b >= kBins) b = first_of(kBins, sh, [&](int i) { return sh.cnt[i] == sh.cnt[kBins - 1]; });  // the last with any
         const int64_t in = int64_t(sh.cnt[b]) - (b > 0 ? int64_t(sh.cnt[b - 1]) : 0);
@@ -387,19 +550,8 @@ __device__ Border find_border(const T *x, const SampleArgs &a, float m, double s
             mass += sh.mass[b - 1];
         }
         if (shift < 0) {
-            // The bin's keys: the bins fall with the key.
-            uint32_t l = key_of(-INFINITY), h = key_of(m);
-            const auto edge = [&](int at_most) {  // the lowest key of a bin <= at_most
-                uint32_t p = l, q = h;
-                while (p < q) {
-                    const uint32_t mid = p + (q - p) / 2;
-                    if (linear(value_of(mid)) <= at_most) q = mid;
-                    else p = mid + 1;
-                }
-                return p;
-            };
-            lo = edge(b);
-            hi = b > 0 ? edge(b - 1) - 1 : h;
+            lo = bins.lowest(b);
+            hi = bins.highest(b);
         } else {
             hi -= uint32_t(b) << shift;
             const uint32_t width = (1u << shift) - 1;
@@ -410,11 +562,11 @@ __device__ Border find_border(const T *x, const SampleArgs &a, float m, double s
             int64_t ties = want - before;
             if (!by_count) {
                 // As many as have less than the target before them.
-                const double need = (target - double(mass) * unfix) / w;
+                const double need = (target - f.sum(mass)) / w;
                 ties = need < double(in) ? int64_t(ceil(need)) : in;
             }
             ties = ties < 1 ? 1 : ties > in ? in : ties;
-            return {hi, ties, double(mass) * unfix + double(ties) * w};
+            return {hi, ties, f.sum(mass) + double(ties) * w};
         }
         if (in <= kList) break;
         const int width = 32 - __clz(hi - lo);
@@ -422,78 +574,93 @@ __device__ Border find_border(const T *x, const SampleArgs &a, float m, double s
     }
     int n = collect(x, a.pieces, a.vocab, lo, hi, [](int) { return true; }, sh);
     n = n < kList ? n : kList;
-    uint64_t mine[4];
-    int rank[4], place[4];
-    rank_list(sh, n, m, scale, mine, rank, place);
-    scan_array(sh.w, n, sh.scratch);
-    const double base = double(mass) * unfix;
+    sort_list(sh, n, m, scale);
+    scan_array<kList>(sh.w, n, sh.scratch);
+    const double base = f.sum(mass);
     int j = by_count ? int(want - before) - 1 : first_of(n, sh, [&](int i) { return base + sh.w[i] >= target; });
     j = j < 0 ? 0 : j >= n ? n - 1 : j;
-    const uint32_t key = uint32_t(sh.sorted[j] >> 32);
-    const int first = first_of(n, sh, [&](int i) { return uint32_t(sh.sorted[i] >> 32) == key; });
+    const uint32_t key = list_key(sh, j);
+    const int first = first_of(n, sh, [&](int i) { return list_key(sh, i) == key; });
     const Border out{key, j - first + 1, base + sh.w[j]};
     __syncthreads();
     return out;
 }
 
-template <typename T> __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a) {
-    __shared__ Shared sh;
-    const int t = threadIdx.x, lane = t & (kWave - 1);
-    const int64_t row = blockIdx.x;
-    const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-    const Row r = row_of(a, row);
-    const int np = a.pieces, vocab = a.vocab;
-    const auto every = [](int) { return true; };
-
-    if (a.piece_max != nullptr) {
-        for (int p = t; p < np; p += kThreads) {
-            sh.pm[p] = a.piece_max[row * np + p];
-            sh.ps[p] = a.piece_sum[row * np + p];
-        }
-    } else {
-        each_piece(x, np, vocab, every, [&](int p, const float (&v)[8], int) {
-            float m;
-            double s;
-            piece_stats(v, r.scale, m, s);
-            if (lane == 0) {
-                sh.pm[p] = m;
-                sh.ps[p] = s;
-            }
-        });
+// Of the n listed tokens, all with lo <= key <= hi, leaves those of the one of 1024 bins over the keys that holds the border:
+// the first `want` listed, or those with less than `target` of w before them.  The w of the ones above are added to their pieces in
+// sums, their number and w to `above` and `base`.  Returns how many are left.
+__device__ __forceinline__ int narrow(Shared &sh, int n, uint32_t lo, uint32_t hi, bool by_count, int64_t want, double target, double least,
+                                      float m, const Scale &scale, double whole, int64_t &above, double &base) {
+    const int t = threadIdx.x;
+    const int width = 32 - __clz(int((hi - lo) | 1u)), shift = width > 10 ? width - 10 : 0;
+    const Fixed f = fixed_of(whole);
+    uint64_t *const mass = reinterpret_cast<uint64_t *>(sh.w);
+    for (int i = t; i < kBins; i += kThreads) {
+        sh.sub[i] = 0;
+        mass[i] = 0;
     }
     __syncthreads();
-    float top = -INFINITY;
-    for (int p = lane; p < np; p += kWave) top = fmaxf(top, sh.pm[p]);
-    top = wave_max(top);
-    if (top == -INFINITY) {  // no token is left
-        if (t == 0) {
-            a.tokens[row] = -1;
-            a.logprobs[row] = -INFINITY;
-        }
-        return;
+    constexpr int Q = kList / kThreads;
+    uint64_t mine[Q], fixed[Q];
+    int bin[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int i = t + q * kThreads;
+        mine[q] = fixed[q] = 0;
+        bin[q] = kBins;
+        if (i >= n) continue;
+        mine[q] = sh.comp[i];
+        const double w = weight(value_of(uint32_t(mine[q] >> 32)), m, scale);
+        fixed[q] = f.of(w);
+        bin[q] = int((hi - uint32_t(mine[q] >> 32)) >> shift);
+        atomicAdd(&sh.sub[bin[q]], 1u);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&mass[bin[q]]), (unsigned long long)fixed[q]);
+        if (!(w >= least)) fixed[q] = 0;
     }
-    for (int p = t; p < np; p += kThreads) sh.ps[p] = sh.pm[p] == -INFINITY ? 0.0 : sh.ps[p] * weight(sh.pm[p], top, r.scale);
     __syncthreads();
-    scan_array(sh.ps, np, sh.scratch);
-    const double whole = sh.ps[np - 1];
+    scan_array<kBins>(sh.sub, kBins, sh.scratch);
+    scan_array<kBins>(mass, kBins, sh.scratch);
+    const int b = first_of(kBins, sh, [&](int i) {
+        return by_count ? above + int64_t(sh.sub[i]) >= want : base + f.sum(mass[i]) >= target;
+    });
+    if (b >= kBins) return 0;
+    if (b > 0) {
+        above += sh.sub[b - 1];
+        base += f.sum(mass[b - 1]);
+    }
+    if (t == 0) sh.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        if (bin[q] < b)
+            atomicAdd(reinterpret_cast<unsigned long long *>(&sh.sums[int(~uint32_t(mine[q])) / kPiece]), (unsigned long long)fixed[q]);
+        if (bin[q] == b) sh.comp[atomicAdd(&sh.count, 1)] = mine[q];
+    }
+    __syncthreads();
+    return sh.count;
+}
 
-    float u = a.u != nullptr ? a.u[row] : 0.f;
-    if (!(u >= 0.f)) u = 0.f;
-    int64_t k = a.top_k != nullptr ? int64_t(a.top_k[row]) : a.top_k_all;
-    const double p_ = a.top_p != nullptr ? double(a.top_p[row]) : a.top_p_all;
-    const double share = p_ < 1.0 ? p_ : 2.0;  // 2: no nucleus
-    double least = a.min_p != nullptr ? double(a.min_p[row]) : a.min_p_all;
-    if (!(least > 0.0)) least = 0.0;
-    if (k <= 0 || k > vocab) k = vocab;
-    if (r.greedy || share <= 0.0 || least > 1.0) k = 1;
-    const auto finish = [&](int64_t token, float value) {
-        a.tokens[row] = token;
-        const double d = value == top ? 0.0 : (double(value) - double(top)) / r.t;
-        a.logprobs[row] = float(d - log(whole));
-    };
+// What the kernels of a workgroup a row share.
+template <typename T> struct RowWork {
+    const SampleArgs &a;
+    Shared &sh;
+    const int64_t row;
+    const T *const x;
+    const Row r;
+    const Choice c;
+    const int np, vocab, t, lane;
+    float top;
+    double whole;
+
+    __device__ __forceinline__ RowWork(const SampleArgs &a_, Shared &sh_, int64_t row_)
+        : a(a_), sh(sh_), row(row_), x(static_cast<const T *>(a_.logits) + row_ * a_.stride), r(row_of(a_, row_)),
+          c(choice_of(a_, row_, r.greedy)), np(a_.pieces), vocab(a_.vocab), t(threadIdx.x), lane(threadIdx.x & (kWave - 1)) {}
+
+    __device__ __forceinline__ double w_of(float v) const { return weight(v, top, r.scale); }
+    __device__ __forceinline__ void finish(int64_t token, float value) const { finish_row(a, row, token, value, top, r.t, whole); }
 
     // The first token of the first piece that holds the maximum, which every run of ranks keeps.
-    const auto largest = [&]() {
+    __device__ __forceinline__ void largest() {
         const int p = first_of(np, sh, [&](int i) { return sh.pm[i] == top; });
         if (t < kWave) {
             Eight<T> g;
@@ -507,171 +674,607 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_select_
             const uint64_t some = __ballot(at < 8);
             if (lane == __ffsll((unsigned long long)some) - 1) finish(g.c0 + at, top);
         }
-    };
-    // A draw from piece p on, whose earlier ones sum to `base`; piece sums are rounded by themselves, and where one is said to
-    // hold the draw and does not, the row's largest is taken.
-    const auto draw = [&](int p, const Kept &kept, int64_t before, double base, double target) {
+    }
+    // The draw from the kept tokens: ps holds the pieces' sums of them (running ones if `running`); `n` listed tokens hold
+    // all of the border's key, or with n = 0 cnt the running numbers of such tokens by piece.
+    __device__ __forceinline__ void draw(const Kept &kept, int n, bool running) {
+        if (!running) scan_array<kMaxPieces>(sh.ps, np, sh.scratch);
+        const double total = sh.ps[np - 1], target = double(c.u) * total;
+        int p = first_of(np, sh, [&](int i) { return sh.ps[i] > target; });
+        if (p >= np) p = first_of(np, sh, [&](int i) { return sh.ps[i] == total; });
+        int64_t before = 0;  // tokens of the border's key in earlier pieces
+        if (n > 0) {
+            if (t == 0) sh.count = 0;
+            __syncthreads();
+            for (int i = t; i < n; i += kThreads)
+                if (list_key(sh, i) == kept.key && list_id(sh, i) < p * kPiece) atomicAdd(&sh.count, 1);
+            __syncthreads();
+            before = sh.count;
+        } else if (p > 0 && !running) {
+            before = sh.cnt[p - 1];
+        }
+        // Piece sums are rounded by themselves: where one is said to hold the draw and does not, the row's largest is taken.
         if (t == 0) sh.token = -1;
         __syncthreads();
-        if (t < kWave) draw_in_piece(x, p, vocab, top, r.scale, kept, before, base, target, sh);
+        if (t < kWave) draw_in_piece(x, p, vocab, top, r.scale, kept, before, p > 0 ? sh.ps[p - 1] : 0.0, target, sh);
         __syncthreads();
         if (sh.token < 0) largest();
         else if (t == 0) finish(sh.token, value_of(sh.key));
-    };
-    if (k == 1) {
-        largest();
-        return;
     }
-    if (k == vocab && share > 1.0 && least == 0.0) {
-        const double target = double(u) * whole;
-        int p = first_of(np, sh, [&](int i) { return sh.ps[i] > target; });
-        if (p >= np) p = first_of(np, sh, [&](int i) { return sh.ps[i] == whole; });
-        draw(p, Kept{0, 0, 0.0}, 0, p > 0 ? sh.ps[p - 1] : 0.0, target);
-        return;
+    // The whole row by this workgroup alone, in as many histograms as it takes.
+    __device__ __forceinline__ void draw_alone() {
+        Kept kept{0, 0, c.least};
+        double of = -1.0;
+        for (int by = 0; by < 2; ++by) {
+            if (by == 0 ? c.k >= vocab : c.share > 1.0) continue;
+            const Border b = find_border(x, a, top, r.scale, whole, by == 0, c.k, c.share, of, sh);
+            of = b.mass;
+            if (by == 0 || b.key > kept.key || (b.key == kept.key && b.ties < kept.ties)) {
+                kept.key = b.key;
+                kept.ties = b.ties;
+            }
+        }
+        const double edge = w_of(value_of(kept.key));  // of the border's own tokens
+        const bool with_ties = kept.ties > 0 && edge >= c.least;
+        __syncthreads();
+        each_piece(x, np, vocab, [](int) { return true; }, [&](int p, const float (&v)[8], int c0) {
+            double s = 0.0;
+            int ties = 0;
+            if (key_of(sh.pm[p]) >= kept.key) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t key = key_of(v[e]);
+                    const double w = w_of(v[e]);
+                    if (key > kept.key && w >= c.least) s += w;
+                    ties += with_ties && c0 + e < vocab && key == kept.key ? 1 : 0;
+                }
+                s = wave_sum64(s);
+#pragma unroll
+                for (int off = kWave / 2; off > 0; off >>= 1) ties += __shfl_xor(ties, off, kWave);
+            }
+            if (lane == 0) {
+                sh.ps[p] = s;
+                sh.cnt[p] = uint32_t(ties);
+            }
+        });
+        __syncthreads();
+        scan_array<kMaxPieces>(sh.cnt, np, sh.scratch);
+        for (int p = t; p < np; p += kThreads) {
+            const int64_t before = p > 0 ? sh.cnt[p - 1] : 0, here = int64_t(sh.cnt[p]) - before;
+            const int64_t room = kept.ties - before, in = room < 0 ? 0 : room < here ? room : here;
+            sh.ps[p] += double(in) * edge;
+        }
+        __syncthreads();
+        draw(kept, 0, false);
     }
+};
 
+// A workgroup a row: all draws but those whose border is not among the few tokens that reach a bound.  These it puts off
+// for the whole chip (PUT_OFF), or makes alone.
+template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void sample_select_kernel(SampleArgs a) {
+    __shared__ Shared sh;
+    RowWork<T> w(a, sh, blockIdx.x);
+    const int np = w.np, vocab = w.vocab, t = w.t, lane = w.lane;
+    const Choice &c = w.c;
+    if (a.piece_max != nullptr) {
+        for (int p = t; p < np; p += kThreads) {
+            sh.pm[p] = a.piece_max[w.row * np + p];
+            sh.ps[p] = a.piece_sum[w.row * np + p];
+        }
+    } else {
+        each_piece(w.x, np, vocab, [](int) { return true; }, [&](int p, const float (&v)[8], int) {
+            float m;
+            double s;
+            piece_stats(v, w.r.scale, m, s);
+            if (lane == 0) {
+                sh.pm[p] = m;
+                sh.ps[p] = s;
+            }
+        });
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int p = lane; p < np; p += kWave) top = fmaxf(top, sh.pm[p]);
+    w.top = top = wave_max_dpp(top);
+    if (top == -INFINITY) {  // no token is left
+        if (t == 0) {
+            a.tokens[w.row] = -1;
+            a.logprobs[w.row] = -INFINITY;
+        }
+        return;
+    }
+    for (int p = t; p < np; p += kThreads) sh.ps[p] = sh.pm[p] == -INFINITY ? 0.0 : sh.ps[p] * w.w_of(sh.pm[p]);
+    __syncthreads();
+    scan_array<kMaxPieces>(sh.ps, np, sh.scratch);
+    const double whole = w.whole = sh.ps[np - 1];
+    if (c.k == 1) {
+        w.largest();
+        return;
+    }
+    if (c.k == vocab && c.share > 1.0 && c.least == 0.0) {
+        w.draw(Kept{0, 0, 0.0}, 0, true);
+        return;
+    }
     // A bound that all kept tokens reach, if enough of them do.
-    bool listed = true, complete = true;
+    bool listed = true, complete = true;  // complete: no token that may be kept is below the bound
     float bound = -INFINITY;
     if (vocab > kList) {
         // Tokens of less w than `least`: a little below, for the rounding of the logarithm.
         float low = -INFINITY;
-        if (least > 0.0 && (k == vocab || share > 1.0)) {
-            const double under = -r.t * log(least);
+        if (c.least > 0.0 && (c.k == vocab || c.share > 1.0)) {
+            const double under = -w.r.t * log(c.least);
             low = isinf(top) ? top : float(double(top) - under - 1e-6 * (fabs(double(top)) + under));
         }
-        const int64_t reach = k < vocab ? k : share < 1.0 ? 128 : 0;
-        if (reach == 0) {
-            bound = low;
-        } else if (reach <= np) {
+        const int64_t reach = c.k < vocab ? c.k : c.share < 1.0 ? 128 : 0;
+        if (reach > np && low == -INFINITY) listed = false;
+        if (reach > 0 && reach <= np) {
             // The piece whose maximum has that rank.
-            __syncthreads();
             for (int i = t; i < np; i += kThreads) {
                 const float mi = sh.pm[i];
                 int rank = 0;
-                for (int j = 0; j < np; ++j) rank += sh.pm[j] > mi || (sh.pm[j] == mi && j < i) ? 1 : 0;
+#pragma unroll 8
+                for (int j = 0; j < np; ++j) rank += int(sh.pm[j] > mi) | (int(sh.pm[j] == mi) & int(j < i));
                 if (rank == int(reach) - 1) sh.key = key_of(mi);
             }
             __syncthreads();
-            bound = fmaxf(value_of(sh.key), low);
-            complete = k < vocab || bound == low;
-        } else if (low > -INFINITY) {
-            bound = low;
-        } else {
-            listed = false;
+            bound = value_of(sh.key);
+            complete = c.k < vocab || low >= bound;
         }
+        bound = fmaxf(bound, low);
     }
     if (listed) {
-        const float b = bound;
-        const int n = collect(x, np, vocab, key_of(b), 0xFFFFFFFFu, [&](int p) { return sh.pm[p] >= b; }, sh);
+        const int n = collect(w.x, np, vocab, key_of(bound), 0xFFFFFFFFu, [&](int p) { return sh.pm[p] >= bound; }, sh);
         if (n <= kList) {
-            uint64_t mine[4];
-            int rank[4], place[4];
-            rank_list(sh, n, top, r.scale, mine, rank, place);
-            // w by rank, then its running sums; the weights themselves come back from the keys.
-            scan_array(sh.w, n, sh.scratch);
-            const int kn = k < n ? int(k) : n;
-            const double mass = k < vocab ? sh.w[kn - 1] : whole;
-            if (complete || sh.w[n - 1] >= share * mass) {
+            sort_list(sh, n, top, w.r.scale);
+            scan_array<kList>(sh.w, n, sh.scratch);
+            const int kn = c.k < n ? int(c.k) : n;
+            const double mass = c.k < vocab ? sh.w[kn - 1] : whole;
+            if (complete || sh.w[n - 1] >= c.share * mass) {
                 const int keep = first_of(n, sh, [&](int i) {
-                    return i > 0 && (i >= kn || !(sh.w[i - 1] < share * mass || share > 1.0) ||
-                                     !(weight(value_of(uint32_t(sh.sorted[i] >> 32)), top, r.scale) >= least));
+                    return i > 0 && (i >= kn || !(sh.w[i - 1] < c.share * mass || c.share > 1.0) || !(w.w_of(value_of(list_key(sh, i))) >= c.least));
                 });
+                for (int p = t; p < np; p += kThreads) {
+                    sh.ps[p] = 0.0;
+                    sh.sums[p] = 0;
+                }
                 __syncthreads();
-                // The kept ones' weights in the order of ids, at the places of all that are listed.
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (t + q * kThreads < n) {
-                        const uint32_t key = uint32_t(mine[q] >> 32);
-                        sh.w[place[q]] = rank[q] < keep ? weight(value_of(key), top, r.scale) : 0.0;
-                        sh.sorted[place[q]] = mine[q];
-                    }
-                __syncthreads();
-                scan_array(sh.w, n, sh.scratch);
-                const double total = sh.w[n - 1], target = double(u) * total;
-                int at = first_of(n, sh, [&](int i) { return sh.w[i] > target; });
-                if (at >= n) at = first_of(n, sh, [&](int i) { return sh.w[i] == total; });
-                if (t == 0) finish(int64_t(~uint32_t(sh.sorted[at])), value_of(uint32_t(sh.sorted[at] >> 32)));
+                Kept kept{0, 0, 0.0};  // `least` is in `keep` already
+                keep_listed(sh, n, keep, np, top, w.r.scale, whole, kept);
+                w.draw(kept, n, false);
                 return;
             }
         }
     }
-
-    // The whole row.
-    Kept kept{0, 0, least};
-    double of = -1.0;
-    if (k < vocab) {
-        const Border b = find_border(x, a, top, r.scale, whole, true, k, 0.0, 0.0, sh);
-        kept.key = b.key;
-        kept.ties = b.ties;
-        of = b.mass;
-    }
-    if (share < 1.0) {
-        const Border b = find_border(x, a, top, r.scale, whole, false, 0, share, of, sh);
-        if (b.key > kept.key || (b.key == kept.key && b.ties < kept.ties)) {
-            kept.key = b.key;
-            kept.ties = b.ties;
+    if constexpr (PUT_OFF) {
+        if (t == 0) sh.count = atomicAdd(a.put_off, 1);
+        __syncthreads();
+        const int at = sh.count;
+        if (t == 0) a.put_off[1 + at] = int32_t(w.row);
+        if (at >= a.most) return;
+        Wide &wide = a.wide[at];
+        for (int i = t; i < kBins; i += kThreads) {
+            wide.mass[i] = 0;
+            wide.cnt[i] = 0;
         }
+        if (t == 0) {
+            wide.whole = whole;
+            wide.top = top;
+            wide.count = 0;
+        }
+    } else {
+        w.draw_alone();
     }
-    const double edge = weight(value_of(kept.key), top, r.scale);  // of the border's own tokens
-    const bool with_ties = kept.ties > 0 && edge >= least;
+}
+
+// Of the rows put off that all workgroups work on together: the place, chunk by chunk of 16 pieces; fn(row, its place, first piece).
+constexpr int kChunk = 16;
+template <typename Fn> __device__ __forceinline__ void each_chunk(const SampleArgs &a, Fn fn) {
+    const int rows = a.put_off[0] < a.most ? a.put_off[0] : a.most;
+    const int chunks = (a.pieces + kChunk - 1) / kChunk;
+    for (int item = blockIdx.x; item < rows * chunks; item += gridDim.x) {
+        const int at = item / chunks;
+        fn(int64_t(a.put_off[1 + at]), a.wide[at], (item - at * chunks) * kChunk);
+    }
+}
+// By one alone of top-k and top-p: the other's border would need the first's sum.
+__device__ __forceinline__ bool together(const Choice &c, int vocab) { return (c.k < vocab) != (c.share < 1.0); }
+
+template <typename T> __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
+    __shared__ uint32_t cnt[kBins];
+    __shared__ uint64_t mass[kBins];
+    const int t = threadIdx.x, wave = t / kWave;
+    each_chunk(a, [&](int64_t row, Wide &wide, int p0) {
+        const Row r = row_of(a, row);
+        if (!together(choice_of(a, row, r.greedy), a.vocab)) return;
+        const T *x = static_cast<const T *>(a.logits) + row * a.stride;
+        const Bins bins = bins_of(wide.top, r.scale);
+        const Fixed f = fixed_of(wide.whole);
+        __syncthreads();
+        for (int i = t; i < kBins; i += 256) {
+            cnt[i] = 0;
+            mass[i] = 0;
+        }
+        __syncthreads();
+        Eight<T> g[kChunk / 4];
+#pragma unroll
+        for (int q = 0; q < kChunk / 4; ++q)
+            if (p0 + 4 * q + wave < a.pieces) g[q].load(x, p0 + 4 * q + wave, a.vocab);
+#pragma unroll
+        for (int q = 0; q < kChunk / 4; ++q) {
+            if (p0 + 4 * q + wave >= a.pieces) break;
+            float v[8];
+            g[q].get(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (g[q].c0 + e < a.vocab) {
+                    const int b = bins.of(v[e]);
+                    atomicAdd(&cnt[b], 1u);
+                    const uint64_t w = f.of(weight(v[e], wide.top, r.scale));
+                    if (w != 0) atomicAdd(reinterpret_cast<unsigned long long *>(&mass[b]), (unsigned long long)w);
+                }
+        }
+        __syncthreads();
+        for (int i = t; i < kBins; i += 256)
+            if (cnt[i] != 0) {
+                atomicAdd(&wide.cnt[i], cnt[i]);
+                atomicAdd(reinterpret_cast<unsigned long long *>(&wide.mass[i]), (unsigned long long)mass[i]);
+            }
+    });
+}
+
+// The border's bin, as every workgroup finds it for itself from the row's bins: how many tokens and how much w are above.
+struct BorderBin {
+    uint32_t lo, hi;
+    int64_t above;
+    double base;
+};
+// By a workgroup of NT threads, each of which sums 1024 / NT bins.
+template <int NT> __device__ __forceinline__ BorderBin border_bin(const Wide &wide, const Choice &c, int vocab, const Bins &bins, uint64_t *scratch, int *found) {
+    constexpr int Q = kBins / NT, W = NT / kWave;
+    const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
+    const Fixed f = fixed_of(wide.whole);
+    uint64_t mass[Q], cnt[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        mass[q] = wide.mass[t * Q + q] + (q > 0 ? mass[q - 1] : 0);
+        cnt[q] = wide.cnt[t * Q + q] + (q > 0 ? cnt[q - 1] : 0);
+    }
+    uint64_t sm = wave_scan(mass[Q - 1]), sc = wave_scan(cnt[Q - 1]);
     __syncthreads();
-    each_piece(x, np, vocab, every, [&](int p, const float (&v)[8], int c0) {
-        double s = 0.0;
-        int ties = 0;
-        if (key_of(sh.pm[p]) >= kept.key) {
+    if (lane == kWave - 1) {
+        scratch[wave] = sm;
+        scratch[W + wave] = sc;
+    }
+    if (t == 0) *found = kBins;
+    __syncthreads();
+    sm -= mass[Q - 1];
+    sc -= cnt[Q - 1];
+    uint64_t all = 0;
+    for (int v = 0; v < W; ++v) {
+        if (v < wave) {
+            sm += scratch[v];
+            sc += scratch[W + v];
+        }
+        all += scratch[v];
+    }
+    const double target = c.share * f.sum(all);
+    int b = kBins;
+#pragma unroll
+    for (int q = Q - 1; q >= 0; --q)
+        if (c.k < vocab ? int64_t(sc + cnt[q]) >= c.k : f.sum(sm + mass[q]) >= target) b = t * Q + q;
+    if (b < kBins) atomicMin(found, b);
+    __syncthreads();
+    const int first = *found < kBins ? *found : kBins - 1;
+    __syncthreads();
+    if (first / Q == t) {
+        const int q = first - t * Q;
+        uint64_t m = sm, n = sc;
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+            if (i + 1 == q) {
+                m += mass[i];
+                n += cnt[i];
+            }
+        scratch[0] = m;
+        scratch[1] = n;
+    }
+    __syncthreads();
+    const BorderBin out{bins.lowest(first), bins.highest(first), int64_t(scratch[1]), f.sum(scratch[0])};
+    __syncthreads();
+    return out;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void sample_list_kernel(SampleArgs a) {
+    __shared__ uint64_t scratch[8];
+    __shared__ int found;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    each_chunk(a, [&](int64_t row, Wide &wide, int p0) {
+        const Row r = row_of(a, row);
+        const Choice c = choice_of(a, row, r.greedy);
+        if (!together(c, a.vocab)) return;
+        const T *x = static_cast<const T *>(a.logits) + row * a.stride;
+        Eight<T> g[kChunk / 4];
+#pragma unroll
+        for (int q = 0; q < kChunk / 4; ++q)
+            if (p0 + 4 * q + wave < a.pieces) g[q].load(x, p0 + 4 * q + wave, a.vocab);
+        const BorderBin b = border_bin<256>(wide, c, a.vocab, bins_of(wide.top, r.scale), scratch, &found);
+#pragma unroll
+        for (int q = 0; q < kChunk / 4; ++q) {
+            const int p = p0 + 4 * q + wave;
+            if (p >= a.pieces) break;
+            float v[8];
+            g[q].get(v);
+            uint64_t in[8];
+            int total = 0;
+            double s = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t key = key_of(v[e]);
-                const double w = weight(v[e], top, r.scale);
-                if (key > kept.key && w >= least) s += w;
-                ties += with_ties && c0 + e < vocab && key == kept.key ? 1 : 0;
+                in[e] = __ballot(g[q].c0 + e < a.vocab && key >= b.lo && key <= b.hi);
+                total += __popcll(in[e]);
+                const double w = weight(v[e], wide.top, r.scale);
+                s += key > b.hi && w >= c.least ? w : 0.0;
             }
-            s = wave_sum(s);
+            s = wave_sum64(s);
+            if (lane == 0) a.piece_sum[row * a.pieces + p] = s;  // in place of the sum of all
+            if (total == 0) continue;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&wide.count, total);
+            at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-            for (int off = kWave / 2; off > 0; off >>= 1) ties += __shfl_xor(ties, off, kWave);
-        }
-        if (lane == 0) {
-            sh.ps[p] = s;
-            sh.cnt[p] = uint32_t(ties);
+            for (int e = 0; e < 8; ++e) {
+                const int mine = at + int(__builtin_amdgcn_mbcnt_hi(uint32_t(in[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(in[e]), 0)));
+                if ((in[e] >> lane & 1) && mine < kList) wide.list[mine] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(g[q].c0 + e));
+                at += __popcll(in[e]);
+            }
         }
     });
-    __syncthreads();
-    scan_array(sh.cnt, np, sh.scratch);
-    for (int p = t; p < np; p += kThreads) {
-        const int64_t before = p > 0 ? sh.cnt[p - 1] : 0, here = int64_t(sh.cnt[p]) - before;
-        const int64_t room = kept.ties - before, in = room < 0 ? 0 : room < here ? room : here;
-        sh.ps[p] += double(in) * edge;
+}
+
+template <typename T> __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
+    __shared__ Shared sh;
+    const int rows = a.put_off[0];
+    for (int at = blockIdx.x; at < rows; at += gridDim.x) {
+        __syncthreads();
+        RowWork<T> w(a, sh, a.put_off[1 + at]);
+        const int np = w.np, vocab = w.vocab, t = w.t, lane = w.lane;
+        const Choice &c = w.c;
+        float top = -INFINITY;
+        for (int p = t; p < np; p += kThreads) sh.pm[p] = a.piece_max[w.row * np + p];
+        __syncthreads();
+        for (int p = lane; p < np; p += kWave) top = fmaxf(top, sh.pm[p]);
+        w.top = wave_max_dpp(top);
+        int n = 0;
+        if (at < a.most) {
+            w.whole = a.wide[at].whole;
+            n = together(c, vocab) ? a.wide[at].count : 0;
+        } else {  // no place of its own: its sums are as the first pass left them
+            for (int p = t; p < np; p += kThreads) sh.ps[p] = sh.pm[p] == -INFINITY ? 0.0 : a.piece_sum[w.row * np + p] * w.w_of(sh.pm[p]);
+            __syncthreads();
+            scan_array<kMaxPieces>(sh.ps, np, sh.scratch);
+            w.whole = sh.ps[np - 1];
+        }
+        bool drawn = false;
+        if (n > 0 && n <= kList) {
+            const Wide &wide = a.wide[at];
+            BorderBin b = border_bin<kThreads>(wide, c, vocab, bins_of(w.top, w.r.scale), sh.scratch, &sh.found);
+            for (int p = t; p < np; p += kThreads) {
+                sh.ps[p] = a.piece_sum[w.row * np + p];
+                sh.sums[p] = 0;
+            }
+            for (int i = t; i < n; i += kThreads) sh.comp[i] = wide.list[i];
+            __syncthreads();
+            const Fixed f = fixed_of(w.whole);
+            // Where min-p leaves nothing of the bin, any border in it will do.
+            const bool none = !(w.w_of(value_of(b.hi)) >= c.least);
+            const bool by_count = none || c.k < vocab;
+            // The target is a share of the integers' sum, as the bins are.
+            uint64_t all = 0;
+            for (int i = lane; i < kBins; i += kWave) all += wide.mass[i];
+#pragma unroll
+            for (int off = kWave / 2; off > 0; off >>= 1) all += __shfl_xor(all, off, kWave);
+            const double target = c.share * f.sum(all);
+            n = narrow(sh, n, b.lo, b.hi, by_count, none ? b.above + 1 : c.k, target, c.least, w.top, w.r.scale, w.whole, b.above, b.base);
+            if (n > 0) {
+                sort_list(sh, n, w.top, w.r.scale);
+                scan_array<kList>(sh.w, n, sh.scratch);
+                int keep = 1;
+                if (by_count) keep = none ? 1 : int(c.k - b.above);
+                else keep = 1 + first_of(n, sh, [&](int i) { return b.base + sh.w[i] >= target; });
+                keep = keep > n ? n : keep;  // the integers' sum passes the target, this one by its rounding may not
+                if (keep > 0) {
+                    __syncthreads();
+                    Kept kept{0, 0, c.least};
+                    keep_listed(sh, n, keep, np, w.top, w.r.scale, w.whole, kept);
+                    w.draw(kept, n, false);
+                    drawn = true;
+                }
+            }
+        }
+        if (!drawn) w.draw_alone();
     }
-    __syncthreads();
-    scan_array(sh.ps, np, sh.scratch);
-    const double total = sh.ps[np - 1], target = double(u) * total;
-    int p = first_of(np, sh, [&](int i) { return sh.ps[i] > target; });
-    if (p >= np) p = first_of(np, sh, [&](int i) { return sh.ps[i] == total; });
-    draw(p, kept, p > 0 ? int64_t(sh.cnt[p - 1]) : 0, p > 0 ? sh.ps[p - 1] : 0.0, target);
+}
+
+// Rows of at most 512 logits, a wave each: logit 64 e + lane is the lane's e-th, ranks are counted over all of them.
+template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel(SampleArgs a, int64_t rows) {
+    __shared__ uint64_t lists[4][kPiece];
+    __shared__ double weights[4][kPiece];
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    const int64_t row = int64_t(blockIdx.x) * 4 + wave;
+    if (row >= rows) return;  // no barriers below
+    const T *x = static_cast<const T *>(a.logits) + row * a.stride;
+    const int vocab = a.vocab, used = (vocab + kWave - 1) / kWave;
+    const Row r = row_of(a, row);
+    const Choice c = choice_of(a, row, r.greedy);
+    float v[8], top = -INFINITY;
+    double w[8], whole = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = 64 * e + lane < vocab ? fmaxf(to_f32(x[64 * e + lane]), -INFINITY) + 0.f : -INFINITY;
+        top = fmaxf(top, v[e]);
+    }
+    top = wave_max_dpp(top);
+    if (top == -INFINITY) {
+        if (lane == 0) {
+            a.tokens[row] = -1;
+            a.logprobs[row] = -INFINITY;
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        w[e] = e < used ? weight(v[e], top, r.scale) : 0.0;
+        whole += w[e];
+    }
+    whole = wave_sum64(whole);
+    if (c.k < vocab || c.share < 1.0 || c.least > 0.0) {
+        uint64_t *const list = lists[wave];
+        double *const ranked = weights[wave];
+        uint64_t mine[8];
+        int rank[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            mine[e] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(64 * e + lane));
+            rank[e] = 0;
+            list[64 * e + lane] = mine[e];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes
+#pragma unroll 8
+        for (int j = 0; j < vocab; ++j) {
+            const uint64_t o = list[j];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < used) rank[e] += o > mine[e] ? 1 : 0;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (64 * e + lane < vocab) ranked[rank[e]] = w[e];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        // A lane sums `used` ranks in a row.
+        const int k = int(c.k);
+        double mass = 0.0, first = 0.0;
+        for (int i = 0; i < used; ++i) {
+            const int q = lane * used + i;
+            const double y = q < vocab ? ranked[q] : 0.0;
+            mass += y;
+            first += q < k ? y : 0.0;
+        }
+        double before = wave_scan(mass) - mass;
+        first = wave_sum64(first);
+        if (lane == 0) before = 0.0;
+        int keep = 0;
+        for (int i = 0; i < used; ++i) {
+            const int q = lane * used + i;
+            if (q >= vocab) break;
+            const double y = ranked[q];
+            if (q == 0 || (q < k && (c.share > 1.0 || before < c.share * first) && y >= c.least)) ++keep;
+            before += y;
+        }
+#pragma unroll
+        for (int off = kWave / 2; off > 0; off >>= 1) keep += __shfl_xor(keep, off, kWave);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (rank[e] >= keep) w[e] = 0.0;
+    }
+    // The draw in the order of ids: 64 of them a step.
+    double upto[8], total = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        upto[e] = total;
+        if (e < used) {
+            upto[e] += wave_scan(w[e]);
+            total = __shfl(upto[e], kWave - 1, kWave);
+        }
+    }
+    const double target = double(c.u) * total;
+    int64_t token = -1;
+    float value = top;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+        const uint64_t past = __ballot(upto[e] > target && w[e] > 0.0);
+        if (past != 0) {
+            const int from = __ffsll((unsigned long long)past) - 1;
+            token = 64 * e + from;
+            value = __shfl(v[e], from, kWave);
+        }
+    }
+    if (token < 0) {  // rounding passed the last: the last that is kept
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint64_t some = __ballot(w[e] > 0.0);
+            if (some != 0) {
+                const int from = 63 - __clzll((long long)some);
+                token = 64 * e + from;
+                value = __shfl(v[e], from, kWave);
+            }
+        }
+    }
+    if (lane == 0) finish_row(a, row, token, value, top, r.t, whole);
 }
 
 // Rows of few pieces need no pass of their own over the chip.
 constexpr int kInline = 16;
 
+int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
+// Sums and maxima of the pieces, the rows put off, and a place for the histogram and list of up to 1024 of them.
+struct Space {
+    int64_t sums, maxima, put_off, wide, bytes;
+    int most;
+};
+Space space_of(int64_t rows, int64_t vocab) {
+    Space s{};
+    if (pieces_of(vocab) <= kInline) return s;
+    const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    s.most = int(std::min<int64_t>(rows, 1024));
+    s.maxima = up(rows * pieces_of(vocab) * 8);
+    s.put_off = s.maxima + up(rows * pieces_of(vocab) * 4);
+    s.wide = s.put_off + up((rows + 1) * 4);
+    s.bytes = s.wide + s.most * int64_t(sizeof(Wide));
+    return s;
+}
+
 template <typename T> hipError_t sample(SampleArgs &a, int64_t rows, void *workspace, hipStream_t st) {
-    if (a.pieces > kInline) {
-        a.piece_sum = static_cast<double *>(workspace);
-        a.piece_max = reinterpret_cast<float *>(a.piece_sum + rows * a.pieces);
-        // 4 pieces a wave where that leaves the chip 4096 waves.
-        a.each = rows * a.pieces >= 4 * 4096 ? 4 : 1;
-        const dim3 grid(unsigned((a.pieces + 4 * a.each - 1) / (4 * a.each)), unsigned(rows));
-        sample_stats_kernel<T><<<grid, 256, 0, st>>>(a);
-        if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (a.vocab <= kPiece) {
+        sample_small_kernel<T><<<unsigned((rows + 3) / 4), 256, 0, st>>>(a, rows);
+        return hipGetLastError();
     }
-    sample_select_kernel<T><<<unsigned(rows), kThreads, 0, st>>>(a);
+    if (a.pieces <= kInline) {
+        sample_select_kernel<T, false><<<unsigned(rows), kThreads, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    const Space space = space_of(rows, a.vocab);
+    char *const ws = static_cast<char *>(workspace);
+    a.piece_sum = reinterpret_cast<double *>(ws);
+    a.piece_max = reinterpret_cast<float *>(ws + space.maxima);
+    // 4 pieces a wave where that leaves the chip 4096 waves.
+    a.each = rows * a.pieces >= 4 * 4096 ? 4 : 1;
+    // A border that is not near the top is for the whole chip, unless top-k says that it is (or a bound by min-p alone).
+    const bool near = !a.top_k && ((a.top_k_all > 0 && a.top_k_all <= a.pieces) ||
+                                   (!a.top_p && !(a.top_p_all < 1.0) && (a.top_k_all <= 0 || a.top_k_all >= a.vocab)));
+    if (!near) {
+        a.put_off = reinterpret_cast<int32_t *>(ws + space.put_off);
+        a.wide = reinterpret_cast<Wide *>(ws + space.wide);
+        a.most = space.most;
+    }
+    const dim3 grid(unsigned((a.pieces + 4 * a.each - 1) / (4 * a.each)), unsigned(rows));
+    sample_stats_kernel<T><<<grid, 256, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (near) {
+        sample_select_kernel<T, false><<<unsigned(rows), kThreads, 0, st>>>(a);
+        return hipGetLastError();
+    }
+    sample_select_kernel<T, true><<<unsigned(rows), kThreads, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const int64_t chunks = std::min<int64_t>(1024, rows * ((a.pieces + kChunk - 1) / kChunk));
+    sample_bins_kernel<T><<<unsigned(chunks), 256, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    sample_list_kernel<T><<<unsigned(chunks), 256, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    sample_finish_kernel<T><<<unsigned(std::min<int64_t>(rows, 512)), kThreads, 0, st>>>(a);
     return hipGetLastError();
 }
 
-int64_t pieces_of(int64_t vocab) { return (vocab + kPiece - 1) / kPiece; }
-int64_t workspace_of(int64_t rows, int64_t vocab) {
-    return pieces_of(vocab) > kInline ? rows * pieces_of(vocab) * 12 : 0;
-}
+int64_t workspace_of(int64_t rows, int64_t vocab) { return space_of(rows, vocab).bytes; }
 int check_sizes(const char *fn, int64_t rows, int64_t vocab) {
     if (rows < 0 || rows > 65535 || vocab < 1 || vocab > int64_t(kMaxPieces) * kPiece)
         return capi::fail(hipErrorInvalidValue, "%s: %lld rows (up to 65535) of %lld logits (1 to %d)", fn, (long long)rows,
