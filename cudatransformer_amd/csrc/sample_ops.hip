@@ -166,8 +166,18 @@ template <typename T> struct Eight {
     int c0;
     __device__ __forceinline__ void load(const T *row, int piece, int vocab) {
         c0 = piece * kPiece + int(threadIdx.x & (kWave - 1)) * 8;
+        if ((piece + 1) * kPiece <= vocab) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) g[i] = Gran<T>::load_tail(row, c0 + i * Gran<T>::EPC, vocab, -INFINITY);
+            for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const typename Gran<T>::raw_t *>(row + c0 + i * Gran<T>::EPC);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[i] = Gran<T>::load_tail(row, c0 + i * Gran<T>::EPC, vocab, -INFINITY);
+        }
+    }
+    // As they are, NaN and -0 too.
+    __device__ __forceinline__ void get_raw(float (&x)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = Gran<T>::get(g[e / Gran<T>::EPC], e % Gran<T>::EPC);
     }
     __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
@@ -187,12 +197,13 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// A piece's maximum and its sum of w relative to it, the same in every lane.
+// A piece's maximum and its sum of w relative to it, the same in every lane, from raw values: fmaxf and fmax take the
+// number of a NaN and a number, so that a NaN has the w of -inf.
 __device__ __forceinline__ void piece_stats(const float (&x)[8], const Scale &c, float &m, double &s) {
-    m = x[0];
+    m = -INFINITY;
 #pragma unroll
-    for (int e = 1; e < 8; ++e) m = fmaxf(m, x[e]);
-    m = wave_max_dpp(m);
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+    m = wave_max_dpp(m) + 0.f;
     s = 0.0;
     if (m == -INFINITY) return;
     if (m == INFINITY) {
@@ -221,7 +232,7 @@ template <typename T> __global__ __launch_bounds__(256) void sample_stats_kernel
         if (p + 1 < p1) next.load(x, p + 1, a.vocab);
         float v[8], m;
         double s;
-        now.get(v);
+        now.get_raw(v);
         piece_stats(v, scale, m, s);
         if (lane == 0) {
             a.piece_max[row * a.pieces + p] = m;
@@ -287,21 +298,33 @@ template <typename Fn> __device__ __forceinline__ int first_of(int n, Shared &sh
     __syncthreads();
     return sh.found;
 }
-// The wanted pieces, spread over the waves, three pieces' loads ahead; fn(piece, values, first id).
+// The wanted pieces, spread over the waves, four pieces' loads ahead; fn(piece, the lane's eight).
 template <typename T, typename Want, typename Fn>
 __device__ __forceinline__ void each_piece(const T *x, int pieces, int vocab, Want want, Fn fn) {
-    constexpr int N = 3;
+    constexpr int N = 4;
+    static_assert(kMaxPieces <= 2 * kWave * kWaves, "two masks a wave");
+    // Which of pieces wave, wave + kWaves, .. are wanted, a bit each.
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+    const int p0 = wave + kWaves * lane, p1 = p0 + kWaves * kWave;
+    uint64_t mask = __ballot(p0 < pieces && want(p0)), rest = __ballot(p1 < pieces && want(p1));
+    int from = wave;
     Eight<T> ahead[N];
-    int at[N], p = threadIdx.x / kWave;
+    int at[N];
     const auto fetch = [&](int i) {
-        while (p < pieces && !want(p)) p += kWaves;
-        at[i] = p;
-        if (p < pieces) ahead[i].load(x, p, vocab);
-        p += kWaves;
+        if (mask == 0) {
+            mask = rest;
+            rest = 0;
+            from = wave + kWaves * kWave;
+        }
+        at[i] = -1;
+        if (mask == 0) return;
+        at[i] = from + kWaves * (__ffsll((unsigned long long)mask) - 1);
+        mask &= mask - 1;
+        ahead[i].load(x, at[i], vocab);
     };
 #pragma unroll
     for (int i = 0; i < N; ++i) fetch(i);
-    while (at[0] < pieces) {
+    while (at[0] >= 0) {
         const Eight<T> now = ahead[0];
         const int here = at[0];
 #pragma unroll
@@ -310,9 +333,7 @@ __device__ __forceinline__ void each_piece(const T *x, int pieces, int vocab, Wa
             at[i] = at[i + 1];
         }
         fetch(N - 1);
-        float v[8];
-        now.get(v);
-        fn(here, v, now.c0);
+        fn(here, now);
     }
 }
 
@@ -466,27 +487,22 @@ __device__ __forceinline__ void keep_listed(Shared &sh, int n, int keep, int pie
     for (int p = t; p < pieces; p += kThreads) sh.ps[p] += f.sum(sh.sums[p]);
     __syncthreads();
 }
-// Lists a piece's tokens with lo <= key <= hi, one atomic a wave; the order in the list is arbitrary.
-__device__ __forceinline__ void append(Shared &sh, const float (&v)[8], int c0, int vocab, uint32_t lo, uint32_t hi) {
-    uint64_t in[8];
-    int total = 0;
+// Lists a piece's tokens with lo <= key <= hi; few lanes have any.  The order in the list is arbitrary.
+__device__ __forceinline__ void append(int32_t *count, uint64_t *list, const float (&v)[8], int c0, int vocab, uint32_t lo, uint32_t hi) {
+    int in = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const uint32_t key = key_of(v[e]);
-        in[e] = __ballot(c0 + e < vocab && key >= lo && key <= hi);
-        total += __popcll(in[e]);
+        in |= int(c0 + e < vocab) & int(key >= lo) & int(key <= hi) ? 1 << e : 0;
     }
-    if (total == 0) return;
-    const int lane = threadIdx.x & (kWave - 1);
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&sh.count, total);
-    at = __builtin_amdgcn_readfirstlane(at);
+    if (in == 0) return;
+    int at = atomicAdd(count, __popc(in));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int mine = at + int(__builtin_amdgcn_mbcnt_hi(uint32_t(in[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(in[e]), 0)));
-        if ((in[e] >> lane & 1) && mine < kList) sh.comp[mine] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(c0 + e));
-        at += __popcll(in[e]);
-    }
+    for (int e = 0; e < 8; ++e)
+        if (in >> e & 1) {
+            if (at < kList) list[at] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(c0 + e));
+            ++at;
+        }
 }
 // Lists the tokens with lo <= key <= hi of the wanted pieces; their number, which may pass the list's length.
 template <typename T, typename Want>
@@ -494,7 +510,11 @@ __device__ __forceinline__ int collect(const T *x, int pieces, int vocab, uint32
     __syncthreads();
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    each_piece(x, pieces, vocab, want, [&](int, const float (&v)[8], int c0) { append(sh, v, c0, vocab, lo, hi); });
+    each_piece(x, pieces, vocab, want, [&](int, const Eight<T> &g) {
+        float v[8];
+        g.get(v);
+        append(&sh.count, sh.comp, v, g.c0, vocab, lo, hi);
+    });
     __syncthreads();
     return sh.count;
 }
@@ -524,7 +544,10 @@ __device__ __forceinline__ Border find_border(const T *x, const SampleArgs &a, f
             sh.mass[i] = 0;
         }
         __syncthreads();
-        each_piece(x, a.pieces, a.vocab, [](int) { return true; }, [&](int, const float (&v)[8], int c0) {
+        each_piece(x, a.pieces, a.vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
+            float v[8];
+            g.get(v);
+            const int c0 = g.c0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t key = key_of(v[e]);
@@ -640,6 +663,22 @@ __device__ __forceinline__ int narrow(Shared &sh, int n, uint32_t lo, uint32_t h
     return sh.count;
 }
 
+// The value of rank `rank` (from 1) among v[0 .. n), n up to 64 Q, bit by bit, by every wave for itself.
+template <int Q> __device__ __forceinline__ float rank_value(const float *v, int n, int rank) {
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t keys[Q], key = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) keys[q] = q * kWave + lane < n ? key_of(v[q * kWave + lane]) : 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t with = key | 1u << bit;
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) count += __popcll(__ballot(keys[q] >= with));
+        if (count >= rank) key = with;
+    }
+    return value_of(key);
+}
+
 // What the kernels of a workgroup a row share.
 template <typename T> struct RowWork {
     const SampleArgs &a;
@@ -717,7 +756,10 @@ template <typename T> struct RowWork {
         const double edge = w_of(value_of(kept.key));  // of the border's own tokens
         const bool with_ties = kept.ties > 0 && edge >= c.least;
         __syncthreads();
-        each_piece(x, np, vocab, [](int) { return true; }, [&](int p, const float (&v)[8], int c0) {
+        each_piece(x, np, vocab, [](int) { return true; }, [&](int p, const Eight<T> &g) {
+            float v[8];
+            g.get(v);
+            const int c0 = g.c0;
             double s = 0.0;
             int ties = 0;
             if (key_of(sh.pm[p]) >= kept.key) {
@@ -762,9 +804,10 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
             sh.ps[p] = a.piece_sum[w.row * np + p];
         }
     } else {
-        each_piece(w.x, np, vocab, [](int) { return true; }, [&](int p, const float (&v)[8], int) {
-            float m;
+        each_piece(w.x, np, vocab, [](int) { return true; }, [&](int p, const Eight<T> &g) {
+            float v[8], m;
             double s;
+            g.get_raw(v);
             piece_stats(v, w.r.scale, m, s);
             if (lane == 0) {
                 sh.pm[p] = m;
@@ -806,18 +849,24 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
             low = isinf(top) ? top : float(double(top) - under - 1e-6 * (fabs(double(top)) + under));
         }
         const int64_t reach = c.k < vocab ? c.k : c.share < 1.0 ? 128 : 0;
-        if (reach > np && low == -INFINITY) listed = false;
-        if (reach > 0 && reach <= np) {
-            // The piece whose maximum has that rank.
-            for (int i = t; i < np; i += kThreads) {
-                const float mi = sh.pm[i];
-                int rank = 0;
-#pragma unroll 8
-                for (int j = 0; j < np; ++j) rank += int(sh.pm[j] > mi) | (int(sh.pm[j] == mi) & int(j < i));
-                if (rank == int(reach) - 1) sh.key = key_of(mi);
-            }
+        const bool by_thread = reach > np && reach <= kThreads && c.k < vocab;  // more ranks than pieces: maxima of every thread
+        if (reach > np && !by_thread && low == -INFINITY) listed = false;
+        if (by_thread) {
+            float m = -INFINITY;
+            each_piece(w.x, np, vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
+                float v[8];
+                g.get(v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
+            });
+            float *const maxima = reinterpret_cast<float *>(sh.w);
+            maxima[t] = m;
             __syncthreads();
-            bound = value_of(sh.key);
+            bound = rank_value<kThreads / kWave>(maxima, kThreads, int(reach));
+        } else if (reach > 0 && reach <= np) {
+            bound = np <= 2 * kWave   ? rank_value<2>(sh.pm, np, int(reach))
+                    : np <= 6 * kWave ? rank_value<6>(sh.pm, np, int(reach))
+                                      : rank_value<kMaxPieces / kWave>(sh.pm, np, int(reach));
             complete = c.k < vocab || low >= bound;
         }
         bound = fmaxf(bound, low);
@@ -1004,29 +1053,15 @@ template <typename T> __global__ __launch_bounds__(256) void sample_list_kernel(
             if (p >= a.pieces) break;
             float v[8];
             g[q].get(v);
-            uint64_t in[8];
-            int total = 0;
             double s = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t key = key_of(v[e]);
-                in[e] = __ballot(g[q].c0 + e < a.vocab && key >= b.lo && key <= b.hi);
-                total += __popcll(in[e]);
                 const double w = weight(v[e], wide.top, r.scale);
-                s += key > b.hi && w >= c.least ? w : 0.0;
+                s += key_of(v[e]) > b.hi && w >= c.least ? w : 0.0;
             }
             s = wave_sum64(s);
             if (lane == 0) a.piece_sum[row * a.pieces + p] = s;  // in place of the sum of all
-            if (total == 0) continue;
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&wide.count, total);
-            at = __builtin_amdgcn_readfirstlane(at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int mine = at + int(__builtin_amdgcn_mbcnt_hi(uint32_t(in[e] >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(in[e]), 0)));
-                if ((in[e] >> lane & 1) && mine < kList) wide.list[mine] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(g[q].c0 + e));
-                at += __popcll(in[e]);
-            }
+            append(&wide.count, wide.list, v, g[q].c0, a.vocab, b.lo, b.hi);
         }
     });
 }
