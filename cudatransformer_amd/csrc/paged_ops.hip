@@ -360,8 +360,11 @@ int ctattn_page_release(const void *done, const int32_t *lens, const int32_t *ta
     ReleaseArgs a{static_cast<const uint8_t *>(done), lens, table, table_row, {free_pages, counters, counters_out, free_places},
                   lens_out, requests, table_width, shift_of(page_size)};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (requests <= 256) page_release_kernel<256><<<4, 256, 0, st>>>(a);
-    else page_release_kernel<1024><<<16, 1024, 0, st>>>(a);
+    // A workgroup for 8 requests, whose pages a wave copies one request after the other (1024 requests, a third done: 16
+    // workgroups 11.8 us, 128 6.8 us).
+    const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>(128, requests / 8)));
+    if (requests <= 256) page_release_kernel<256><<<blocks, 256, 0, st>>>(a);
+    else page_release_kernel<1024><<<blocks, 1024, 0, st>>>(a);
     return finish(fn, hipGetLastError(), st);
 }
 

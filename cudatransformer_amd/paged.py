@@ -10,6 +10,7 @@ that a captured step replays on what they hold.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -19,13 +20,13 @@ _Strides10, _Strides12 = ctypes.c_int64 * 10, ctypes.c_int64 * 12
 
 
 def _check_ints(name, what, t, shape, dtype, device):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} "
                          f"on {t.device}")
 
 
 def _check_table(name, what, t, rows, device):
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1):
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != rows or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1):
         raise ValueError(f"{name}: {what} must be int32 [{rows}, pages] with contiguous rows on {device}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
 
@@ -43,6 +44,14 @@ def _check_pool(name, lens, table, free, counters, page_size):
     if page_size < 1 or page_size & (page_size - 1):
         raise ValueError(f"{name}: page size {page_size}, a power of two is wanted")
     return device, n
+
+
+def _on(device, stream, fn, *args):
+    """fn(*args) where the tensors' device is current, and `stream` if given."""
+    if stream is None and device.index == torch.cuda.current_device():
+        return fn(*args)
+    with on_device(device, stream):
+        return fn(*args)
 
 
 def _given(name, what, t, make, shape, dtype, device):
@@ -70,17 +79,23 @@ def page_reserve(lens, new_lens, table, free, counters, page_size: int, max_toke
         raise ValueError(f"{name}: max_tokens {max_tokens}")
     if out is not None and len(out) != 5:
         raise ValueError(f"{name}: out must be (slots, positions, starts, lens, counters)")
-    want = (("slots", (max_tokens,), torch.int64), ("positions", (max_tokens,), torch.int64), ("starts", (n + 1,), torch.int32),
-            ("lens", (n,), torch.int32), ("counters", (2,), torch.int64))
-    with on_device(device, stream):
-        out = tuple(_given(name, f"out's {what}", t, lens.new_empty, shape, dtype, device)
-                    for (what, shape, dtype), t in zip(want, out or (None,) * 5))
-        slots, positions, starts, lens_out, counters_out = out
-        rc = load().ctattn_page_reserve(_ptr(lens), _ptr(new_lens), _ptr(offsets), _ptr(table), _ptr(free), _ptr(counters),
-                                        _ptr(slots), _ptr(positions), _ptr(starts), _ptr(lens_out), _ptr(counters_out), n,
-                                        table.stride(0), table.shape[1], free.shape[0], page_size, max_tokens,
-                                        _stream_handle(stream))
-    _check(rc, "ctattn_page_reserve")
+    return _on(device, stream, _reserve, name, lens, new_lens, table, free, counters, page_size, max_tokens, offsets, out, device, n, stream)
+
+
+def _reserve(name, lens, new_lens, table, free, counters, page_size, max_tokens, offsets, out, device, n, stream):
+    want = (((max_tokens,), torch.int64), ((max_tokens,), torch.int64), ((n + 1,), torch.int32), ((n,), torch.int32), ((2,), torch.int64))
+    if out is None:
+        out = tuple(lens.new_empty(shape, dtype=dtype) for shape, dtype in want)
+    else:
+        names = "slots", "positions", "starts", "lens", "counters"
+        out = tuple(_given(name, f"out's {what}", t, lens.new_empty, *w, device) for what, t, w in zip(names, out, want))
+    slots, positions, starts, lens_out, counters_out = out
+    rc = load().ctattn_page_reserve(lens.data_ptr(), new_lens.data_ptr(), _ptr(offsets), table.data_ptr(), free.data_ptr(),
+                                    counters.data_ptr(), slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
+                                    lens_out.data_ptr(), counters_out.data_ptr(), n, table.stride(0), table.shape[1], free.shape[0],
+                                    page_size, max_tokens, _stream_handle(stream))
+    if rc != 0:
+        _check(rc, "ctattn_page_reserve")
     return out
 
 
@@ -92,14 +107,18 @@ def page_release(done, lens, table, free, counters, page_size: int, out=None, st
     _check_ints(name, "done", done, (n,), torch.bool, device)
     if out is not None and len(out) != 2:
         raise ValueError(f"{name}: out must be (lens, counters)")
-    with on_device(device, stream):
-        lens_out, counters_out = out or (None, None)
-        lens_out = _given(name, "out's lens", lens_out, lens.new_empty, (n,), torch.int32, device)
-        counters_out = _given(name, "out's counters", counters_out, lens.new_empty, (2,), torch.int64, device)
-        rc = load().ctattn_page_release(_ptr(done), _ptr(lens), _ptr(table), _ptr(free), _ptr(counters), _ptr(lens_out),
-                                        _ptr(counters_out), n, table.stride(0), table.shape[1], free.shape[0], page_size,
-                                        _stream_handle(stream))
-    _check(rc, "ctattn_page_release")
+    return _on(device, stream, _release, name, done, lens, table, free, counters, page_size, out, device, n, stream)
+
+
+def _release(name, done, lens, table, free, counters, page_size, out, device, n, stream):
+    lens_out, counters_out = out or (None, None)
+    lens_out = _given(name, "out's lens", lens_out, lens.new_empty, (n,), torch.int32, device)
+    counters_out = _given(name, "out's counters", counters_out, lens.new_empty, (2,), torch.int64, device)
+    rc = load().ctattn_page_release(done.data_ptr(), lens.data_ptr(), table.data_ptr(), free.data_ptr(), counters.data_ptr(),
+                                    lens_out.data_ptr(), counters_out.data_ptr(), n, table.stride(0), table.shape[1],
+                                    free.shape[0], page_size, _stream_handle(stream))
+    if rc != 0:
+        _check(rc, "ctattn_page_release")
     return lens_out, counters_out
 
 
@@ -140,21 +159,31 @@ def cache_write(k, v, k_cache, v_cache, slots, stream=None):
         if t.stride(2) != 1 and d > 1:
             raise ValueError(f"{name}: a head's elements must be contiguous")
     _check_ints(name, "slots", slots, (rows,), torch.int64, k.device)
-    with on_device(k.device, stream):
-        strides = _Strides10(*k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
-        rc = load().ctattn_cache_write(_DTYPE_CODE[k.dtype], _ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(slots), strides,
-                                       rows, heads, d, k_cache.shape[0], k_cache.shape[1], _stream_handle(stream))
-    _check(rc, "ctattn_cache_write")
+    _on(k.device, stream, _write, k, v, k_cache, v_cache, slots, rows, heads, d, stream)
+
+
+def _write(k, v, k_cache, v_cache, slots, rows, heads, d, stream):
+    strides = _Strides10(*k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3])
+    rc = load().ctattn_cache_write(_DTYPE_CODE[k.dtype], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                   slots.data_ptr(), strides, rows, heads, d, k_cache.shape[0], k_cache.shape[1],
+                                   _stream_handle(stream))
+    if rc != 0:
+        _check(rc, "ctattn_cache_write")
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_prefix_need(code, *sizes):
+    n = load().ctattn_shared_prefix_workspace_bytes(code, *sizes)
+    if n < 0:
+        raise ValueError(last_error())
+    return n
 
 
 def shared_prefix_workspace_bytes(dtype, rows: int, requests: int, groups: int, num_heads: int, num_kv_heads: int, d: int,
                                   page_size: int, table_width: int, prefix_width: int) -> int:
     """Bytes of the workspace of flash_attn_shared_prefix."""
-    n = load().ctattn_shared_prefix_workspace_bytes(_DTYPE_CODE[dtype], rows, requests, groups, num_heads, num_kv_heads, d,
-                                                    page_size, table_width, prefix_width)
-    if n < 0:
-        raise ValueError(last_error())
-    return n
+    return _shared_prefix_need(_DTYPE_CODE[dtype], rows, requests, groups, num_heads, num_kv_heads, d, page_size, table_width,
+                               prefix_width)
 
 
 def flash_attn_shared_prefix(q, k_cache, v_cache, table, lens, prefix_table=None, prefix_lens=None, group_starts=None, starts=None,
@@ -205,25 +234,28 @@ def flash_attn_shared_prefix(q, k_cache, v_cache, table, lens, prefix_table=None
         _check_ints(name, "lse", lse, (rows, hq), _stat_dtype(dtype), device)
     if workspace is not None and (not workspace.is_contiguous() or workspace.device != device):
         raise ValueError(f"{name}: workspace must be contiguous on {device}")
+    return _on(device, stream, _shared_prefix, q, k_cache, v_cache, table, lens, prefix_table, prefix_lens, group_starts, starts,
+               out, lse, workspace, rows, n, groups, hq, hkv, d, pages, page_size, stream)
+
+
+def _shared_prefix(q, k_cache, v_cache, table, lens, prefix_table, prefix_lens, group_starts, starts, out, lse, workspace, rows, n,
+                   groups, hq, hkv, d, pages, page_size, stream):
     width, pwidth = table.shape[1], prefix_table.shape[1] if groups else 0
-    lib, code = load(), _DTYPE_CODE[dtype]
-    need = lib.ctattn_shared_prefix_workspace_bytes(code, rows, n, groups, hq, hkv, d, page_size, width, pwidth)
-    if need < 0:
-        raise ValueError(last_error())
-    with on_device(device, stream):
-        fill = out is None
-        out = q.new_empty((rows, hq, d)) if out is None else out
-        lse = q.new_empty((rows, hq), dtype=_stat_dtype(dtype)) if lse is None else lse
-        if workspace is None:
-            workspace = q.new_empty(max(need, 1), dtype=torch.uint8)
-        strides = _Strides12(q.stride(0), q.stride(1), out.stride(0), out.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3],
-                             table.stride(0), prefix_table.stride(0) if groups else 0)
-        rc = lib.ctattn_shared_prefix_fwd(code, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(table), _ptr(lens), _ptr(prefix_table),
-                                          _ptr(prefix_lens), _ptr(group_starts), _ptr(starts), _ptr(out), _ptr(lse),
-                                          _ptr(workspace), workspace.numel() * workspace.element_size(), strides, rows, n,
-                                          groups, hq, hkv, d, pages, page_size, width, pwidth, int(fill),
-                                          _stream_handle(stream))
-    _check(rc, "ctattn_shared_prefix_fwd")
+    code, fill = _DTYPE_CODE[q.dtype], out is None
+    need = _shared_prefix_need(code, rows, n, groups, hq, hkv, d, page_size, width, pwidth)
+    out = q.new_empty((rows, hq, d)) if out is None else out
+    lse = q.new_empty((rows, hq), dtype=_stat_dtype(q.dtype)) if lse is None else lse
+    if workspace is None:
+        workspace = q.new_empty(max(need, 1), dtype=torch.uint8)
+    strides = _Strides12(*q.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0),
+                         prefix_table.stride(0) if groups else 0)
+    rc = load().ctattn_shared_prefix_fwd(code, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                                         _ptr(prefix_table), _ptr(prefix_lens), _ptr(group_starts), _ptr(starts), out.data_ptr(),
+                                         lse.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), strides,
+                                         rows, n, groups, hq, hkv, d, pages, page_size, width, pwidth, int(fill),
+                                         _stream_handle(stream))
+    if rc != 0:
+        _check(rc, "ctattn_shared_prefix_fwd")
     return out, lse
 
 

@@ -1,6 +1,7 @@
 """Next tokens from logits and given random numbers over torch device tensors (ctattn_sample of include/ctattn.h)."""
 from __future__ import annotations
 
+import functools
 import operator
 
 import torch
@@ -8,12 +9,17 @@ import torch
 from ._capi import _DTYPE_CODE, _check, _ptr, _stream_handle, last_error, load, on_device
 
 
-def sample_workspace_bytes(rows: int, vocab: int) -> int:
-    """Bytes of the workspace of sample_tokens."""
+@functools.lru_cache(maxsize=256)
+def _need(rows, vocab):
     need = load().ctattn_sample_workspace_bytes(rows, vocab)
     if need < 0:
         raise ValueError(last_error())
     return need
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    """Bytes of the workspace of sample_tokens."""
+    return _need(rows, vocab)
 
 
 def sample_tokens(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, logprobs=None, workspace=None,
@@ -34,12 +40,15 @@ def sample_tokens(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
         raise ValueError(f"{name}: dtype {logits.dtype} unsupported (float32, bfloat16, float16)")
     (rows, vocab), device = logits.shape, logits.device
 
+    def check(what, x, dtype):
+        if x.dtype is not dtype or x.shape != (rows,) or x.device != device or not x.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous {dtype} [{rows}] on {device}, got {x.dtype} {list(x.shape)} on "
+                             f"{x.device}")
+
     def each(what, x, dtype, number):
         if not isinstance(x, torch.Tensor):
             return None, number(x)
-        if x.dtype != dtype or tuple(x.shape) != (rows,) or x.device != device or not x.is_contiguous():
-            raise ValueError(f"{name}: {what} must be a number or contiguous {dtype} [{rows}] on {device}, got {x.dtype} {list(x.shape)} "
-                             f"on {x.device}")
+        check(what, x, dtype)
         return x, number(0)
 
     t, t_all = each("temperature", temperature, torch.float32, float)
@@ -50,25 +59,33 @@ def sample_tokens(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
         if t is not None or t_all > 0:
             raise ValueError(f"{name}: random numbers may be left out for temperature 0 alone")
     else:
-        each("u", u, torch.float32, float)
         if not isinstance(u, torch.Tensor):
             raise ValueError(f"{name}: u must be a tensor")
-    for what, x, dtype in (("tokens", tokens, torch.int64), ("logprobs", logprobs, torch.float32)):
-        if x is not None:
-            each(what, x, dtype, float)
+        check("u", u, torch.float32)
+    if tokens is not None:
+        check("tokens", tokens, torch.int64)
+    if logprobs is not None:
+        check("logprobs", logprobs, torch.float32)
     if workspace is not None and (not workspace.is_contiguous() or workspace.device != device):
         raise ValueError(f"{name}: workspace must be contiguous on {device}")
-    need = sample_workspace_bytes(rows, vocab)
+    if stream is None and device.index == torch.cuda.current_device():
+        return _sample(logits, u, t, k, p, m, t_all, k_all, p_all, m_all, tokens, logprobs, workspace, rows, vocab, None)
     with on_device(device, stream):
-        tokens = logits.new_empty(rows, dtype=torch.int64) if tokens is None else tokens
-        logprobs = logits.new_empty(rows, dtype=torch.float32) if logprobs is None else logprobs
-        if workspace is None and need > 0:
-            workspace = logits.new_empty(need, dtype=torch.uint8)
-        rc = load().ctattn_sample(_DTYPE_CODE[logits.dtype], _ptr(logits), _ptr(u), _ptr(t), _ptr(k), _ptr(p), _ptr(m), t_all, k_all,
-                                  p_all, m_all, _ptr(tokens), _ptr(logprobs), _ptr(workspace),
-                                  0 if workspace is None else workspace.numel() * workspace.element_size(), rows, vocab,
-                                  logits.stride(0), _stream_handle(stream))
-    _check(rc, "ctattn_sample")
+        return _sample(logits, u, t, k, p, m, t_all, k_all, p_all, m_all, tokens, logprobs, workspace, rows, vocab, stream)
+
+
+def _sample(logits, u, t, k, p, m, t_all, k_all, p_all, m_all, tokens, logprobs, workspace, rows, vocab, stream):
+    need = _need(rows, vocab)
+    tokens = logits.new_empty(rows, dtype=torch.int64) if tokens is None else tokens
+    logprobs = logits.new_empty(rows, dtype=torch.float32) if logprobs is None else logprobs
+    if workspace is None and need > 0:
+        workspace = logits.new_empty(need, dtype=torch.uint8)
+    rc = load().ctattn_sample(_DTYPE_CODE[logits.dtype], logits.data_ptr(), _ptr(u), _ptr(t), _ptr(k), _ptr(p), _ptr(m), t_all, k_all,
+                              p_all, m_all, tokens.data_ptr(), logprobs.data_ptr(), _ptr(workspace),
+                              0 if workspace is None else workspace.numel() * workspace.element_size(), rows, vocab,
+                              logits.stride(0), _stream_handle(stream))
+    if rc != 0:
+        _check(rc, "ctattn_sample")
     return tokens, logprobs
 
 
