@@ -24,7 +24,8 @@ over all tokens on logits (mathematically -log softmax), weights initialised N(0
 Beyond the reference: key / value heads shared by query heads (``n_kv_heads``), a scaled token
 embedding (``embedding_scale``), and batches of whole documents packed behind each other
 (``forward(ids, plan)``), on the packed attention and the sorted embedding gradient; the blocks'
-matrices can be trained with ``muon.Muon`` (``muon_parameters``).
+matrices can be trained with ``muon.Muon`` (``muon_parameters``); many continuations of shared prompts
+(``generate(prompts, new_tokens, samples=…)``) on the paged cache, where an id outside the vocabulary embeds as zeros.
 """
 from __future__ import annotations
 
@@ -34,6 +35,7 @@ import torch.nn.functional as F
 
 from ._capi import flash_attention
 from .embedding import embedding
+from .generate import generate
 from .packed import flash_attention_packed
 
 CONFIG5 = dict(vocab=65, max_seq_len=256, d_model=384, n_heads=6, head_dim=64, mlp_dim=1536,
@@ -80,6 +82,13 @@ class Attention(nn.Module):
             o = torch.cat([q[:, :0], *o], dim=1).transpose(0, 1)
         return self.o(o.reshape(n, self.n_heads * self.head_dim))
 
+    def forward_cached(self, x, cache, layer):
+        """x [tokens, d_model], new tokens of requests whose keys and values `cache` keeps."""
+        n = x.shape[0]
+        q = self.q(x).view(n, self.n_heads, self.head_dim)
+        k, v = (f(x).view(n, self.n_kv_heads, self.head_dim) for f in (self.k, self.v))
+        return self.o(cache.attend(layer, q, k, v).reshape(n, self.n_heads * self.head_dim))
+
     def forward(self, x, plan=None):
         if plan is not None:
             return self.forward_packed(x, plan)
@@ -112,6 +121,10 @@ class Block(nn.Module):
 
     def forward(self, x, plan=None):
         x = self.attn(self.ln1(x), plan)
+        return self.fc2(self.act(self.fc1(self.ln2(x))))
+
+    def forward_cached(self, x, cache, layer):
+        x = self.attn.forward_cached(self.ln1(x), cache, layer)
         return self.fc2(self.act(self.fc1(self.ln2(x))))
 
 
@@ -179,6 +192,17 @@ class NanoGPT(nn.Module):
         for blk in self.blocks:
             x = blk(x, plan)
         return self.unembed(x)
+
+    def forward_cached(self, ids, cache, rows=None):
+        """Logits of new tokens ids [tokens] whose places and positions `cache` (generate.PromptCache) says, or of some rows."""
+        x = self.tok(ids, self.embedding_scale) + self.pos(cache.positions)
+        for i, blk in enumerate(self.blocks):
+            x = blk.forward_cached(x, cache, i)
+        return self.unembed(x if rows is None else x[rows])
+
+    def generate(self, prompts, new_tokens, **kw):
+        """(tokens, logprobs) of continuations of prompts: ``generate.generate``."""
+        return generate(self, prompts, new_tokens, **kw)
 
     def loss(self, ids, targets, plan=None):
         logits = self.forward(ids, plan)
