@@ -120,7 +120,11 @@ __device__ __forceinline__ Choice choice_of(const SampleArgs &a, int64_t row, bo
     c.least = a.min_p != nullptr ? double(a.min_p[row]) : a.min_p_all;
     if (!(c.least > 0.0)) c.least = 0.0;
     if (c.k <= 0 || c.k > a.vocab) c.k = a.vocab;
-    if (greedy || c.share <= 0.0 || c.least > 1.0) c.k = 1;
+    if (greedy || c.share <= 0.0 || c.least > 1.0) {
+        c.k = 1;
+        c.share = 2.0;
+        c.least = 0.0;
+    }
     return c;
 }
 __device__ __forceinline__ void finish_row(const SampleArgs &a, int64_t row, int64_t token, float value, float top, double t, double whole) {
@@ -838,40 +842,41 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
         w.draw(Kept{0, 0, 0.0}, 0, true);
         return;
     }
-    // A bound that all kept tokens reach, if enough of them do.
-    bool listed = true, complete = true;  // complete: no token that may be kept is below the bound
-    float bound = -INFINITY;
-    if (vocab > kList) {
-        // Tokens of less w than `least`: a little below, for the rounding of the logarithm.
-        float low = -INFINITY;
-        if (c.least > 0.0 && (c.k == vocab || c.share > 1.0)) {
-            const double under = -w.r.t * log(c.least);
-            low = isinf(top) ? top : float(double(top) - under - 1e-6 * (fabs(double(top)) + under));
-        }
-        const int64_t reach = c.k < vocab ? c.k : c.share < 1.0 ? 128 : 0;
-        const bool by_thread = reach > np && reach <= kThreads && c.k < vocab;  // more ranks than pieces: maxima of every thread
-        if (reach > np && !by_thread && low == -INFINITY) listed = false;
-        if (by_thread) {
-            float m = -INFINITY;
-            each_piece(w.x, np, vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
-                float v[8];
-                g.get(v);
+    // A bound that all kept tokens reach, if enough of them do; for rows that fit in the list then all.
+    for (int attempt = vocab > kThreads ? 0 : 1; attempt < (vocab > kList ? 1 : 2); ++attempt) {
+        bool complete = true;  // no token that may be kept is below the bound
+        float bound = -INFINITY;
+        if (attempt == 0) {
+            // Tokens of less w than `least`: a little below, for the rounding of the logarithm.
+            float low = -INFINITY;
+            if (c.least > 0.0 && (c.k == vocab || c.share > 1.0)) {
+                const double under = -w.r.t * log(c.least);
+                low = isinf(top) ? top : float(double(top) - under - 1e-6 * (fabs(double(top)) + under));
+            }
+            const int64_t reach = c.k < vocab ? c.k : c.share < 1.0 ? 128 : 0;
+            const bool by_thread = reach > np && reach <= kThreads;  // more ranks than pieces: maxima of every thread
+            if (reach > np && !by_thread && low == -INFINITY) continue;
+            if (by_thread) {
+                float m = -INFINITY;
+                each_piece(w.x, np, vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
+                    float v[8];
+                    g.get(v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
-            });
-            float *const maxima = reinterpret_cast<float *>(sh.w);
-            maxima[t] = m;
-            __syncthreads();
-            bound = rank_value<kThreads / kWave>(maxima, kThreads, int(reach));
-        } else if (reach > 0 && reach <= np) {
-            bound = np <= 2 * kWave   ? rank_value<2>(sh.pm, np, int(reach))
-                    : np <= 6 * kWave ? rank_value<6>(sh.pm, np, int(reach))
-                                      : rank_value<kMaxPieces / kWave>(sh.pm, np, int(reach));
-            complete = c.k < vocab || low >= bound;
+                    for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
+                });
+                float *const maxima = reinterpret_cast<float *>(sh.w);
+                maxima[t] = m;
+                __syncthreads();
+                bound = rank_value<kThreads / kWave>(maxima, kThreads, int(reach));
+                complete = c.k < vocab || low >= bound;
+            } else if (reach > 0 && reach <= np) {
+                bound = np <= 2 * kWave   ? rank_value<2>(sh.pm, np, int(reach))
+                        : np <= 6 * kWave ? rank_value<6>(sh.pm, np, int(reach))
+                                          : rank_value<kMaxPieces / kWave>(sh.pm, np, int(reach));
+                complete = c.k < vocab || low >= bound;
+            }
+            bound = fmaxf(bound, low);
         }
-        bound = fmaxf(bound, low);
-    }
-    if (listed) {
         const int n = collect(w.x, np, vocab, key_of(bound), 0xFFFFFFFFu, [&](int p) { return sh.pm[p] >= bound; }, sh);
         if (n <= kList) {
             sort_list(sh, n, top, w.r.scale);
@@ -1130,10 +1135,13 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_finish_
     }
 }
 
-// Rows of at most 512 logits, a wave each: logit 64 e + lane is the lane's e-th, ranks are counted over all of them.
+// Rows of at most 128 logits, a wave each: logit 64 e + lane is the lane's e-th, ranks are counted over all of them.  (Up to 512
+// so, 500 logits take 34 us, a workgroup a row 25.)
+constexpr int kSmall = 128;
 template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel(SampleArgs a, int64_t rows) {
-    __shared__ uint64_t lists[4][kPiece];
-    __shared__ double weights[4][kPiece];
+    __shared__ uint64_t lists[4][kSmall];
+    __shared__ double weights[4][kSmall];
+    constexpr int E = kSmall / kWave;
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     const int64_t row = int64_t(blockIdx.x) * 4 + wave;
     if (row >= rows) return;  // no barriers below
@@ -1141,10 +1149,10 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
     const int vocab = a.vocab, used = (vocab + kWave - 1) / kWave;
     const Row r = row_of(a, row);
     const Choice c = choice_of(a, row, r.greedy);
-    float v[8], top = -INFINITY;
-    double w[8], whole = 0.0;
+    float v[E], top = -INFINITY;
+    double w[E], whole = 0.0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < E; ++e) {
         v[e] = 64 * e + lane < vocab ? fmaxf(to_f32(x[64 * e + lane]), -INFINITY) + 0.f : -INFINITY;
         top = fmaxf(top, v[e]);
     }
@@ -1157,7 +1165,7 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < E; ++e) {
         w[e] = e < used ? weight(v[e], top, r.scale) : 0.0;
         whole += w[e];
     }
@@ -1165,10 +1173,10 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
     if (c.k < vocab || c.share < 1.0 || c.least > 0.0) {
         uint64_t *const list = lists[wave];
         double *const ranked = weights[wave];
-        uint64_t mine[8];
-        int rank[8];
+        uint64_t mine[E];
+        int rank[E];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
             mine[e] = uint64_t(key_of(v[e])) << 32 | uint32_t(~(64 * e + lane));
             rank[e] = 0;
             list[64 * e + lane] = mine[e];
@@ -1178,11 +1186,11 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
         for (int j = 0; j < vocab; ++j) {
             const uint64_t o = list[j];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < E; ++e)
                 if (e < used) rank[e] += o > mine[e] ? 1 : 0;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
             if (64 * e + lane < vocab) ranked[rank[e]] = w[e];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         // A lane sums `used` ranks in a row.
@@ -1208,13 +1216,13 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
 #pragma unroll
         for (int off = kWave / 2; off > 0; off >>= 1) keep += __shfl_xor(keep, off, kWave);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
             if (rank[e] >= keep) w[e] = 0.0;
     }
     // The draw in the order of ids: 64 of them a step.
-    double upto[8], total = 0.0;
+    double upto[E], total = 0.0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < E; ++e) {
         upto[e] = total;
         if (e < used) {
             upto[e] += wave_scan(w[e]);
@@ -1225,7 +1233,7 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
     int64_t token = -1;
     float value = top;
 #pragma unroll
-    for (int e = 7; e >= 0; --e) {
+    for (int e = E - 1; e >= 0; --e) {
         const uint64_t past = __ballot(upto[e] > target && w[e] > 0.0);
         if (past != 0) {
             const int from = __ffsll((unsigned long long)past) - 1;
@@ -1235,7 +1243,7 @@ template <typename T> __global__ __launch_bounds__(256) void sample_small_kernel
     }
     if (token < 0) {  // rounding passed the last: the last that is kept
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
             const uint64_t some = __ballot(w[e] > 0.0);
             if (some != 0) {
                 const int from = 63 - __clzll((long long)some);
@@ -1269,7 +1277,7 @@ Space space_of(int64_t rows, int64_t vocab) {
 }
 
 template <typename T> hipError_t sample(SampleArgs &a, int64_t rows, void *workspace, hipStream_t st) {
-    if (a.vocab <= kPiece) {
+    if (a.vocab <= kSmall) {
         sample_small_kernel<T><<<unsigned((rows + 3) / 4), 256, 0, st>>>(a, rows);
         return hipGetLastError();
     }
