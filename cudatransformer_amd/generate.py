@@ -102,6 +102,8 @@ def generate(model, prompts, new_tokens: int, samples: int = 1, temperature=1.0,
                 replay = g.replay
             replay()
             tokens[t], logprobs[t] = now, logprob
+        if replay is not step:
+            torch.cuda.current_stream().synchronize()  # the graph goes when this returns
     return tokens.t().contiguous(), logprobs.t().contiguous()
 
 
