@@ -83,7 +83,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs &a, int64_t row) {
     Row r;
     r.greedy = !(t > 0.0);
     r.t = r.greedy ? 1.0 : t;
-    r.scale.s = fmax(kLog2e64 / r.t, 1e-290);  // an infinite t too leaves -inf below the floor
+    r.scale.s = fmin(fmax(kLog2e64 / r.t, 1e-290), 1e290);  // an infinite t too leaves -inf below the floor, and 0 s is 0
     r.scale.floor = -1100.0 / r.scale.s;
     return r;
 }

@@ -122,3 +122,14 @@ def test_reservation_of_many_tokens_by_few_requests():
     known = pos >= 16  # the first page was held before, and the table had none
     assert torch.equal(slots[3:30003][known], (own * 16 + pos % 16)[known])
     assert slots[30005:].tolist() == [-1] * 5
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [60, 400, 3001, 40000])
+@pytest.mark.parametrize("how", [dict(), dict(top_k=9), dict(top_p=0.9), dict(min_p=0.2)])
+@pytest.mark.parametrize("temperature", [5e-324, 1e-310, 1e-40])
+def test_least_temperatures_draw_the_largest(vocab, how, temperature):
+    x = torch.randn((3, vocab), generator=torch.Generator().manual_seed(vocab)).cuda()
+    assert (x.topk(2).values[:, 0] > x.topk(2).values[:, 1]).all()
+    tokens, logprobs = ct.sample_tokens(x, torch.tensor([0.0, 0.5, 0.999], device="cuda"), temperature, **how)
+    assert torch.equal(tokens, x.argmax(1)) and (logprobs == 0).all()
