@@ -7,10 +7,10 @@
 // that near a border).
 //
 // A row is pieces of 512 logits, 8 a lane of a wave.  One pass over the logits, spread over the chip, leaves each
-// piece's maximum and its sum of w relative to it; a workgroup a row does the rest.  A draw from all tokens then needs
-// the pieces' sums and one piece.  Top-k and most nuclei lie among a few hundred tokens: the R-th largest of the pieces'
-// maxima is a bound that at least R tokens reach, so only pieces that reach it are read again, and what reaches it is
-// ranked in LDS.  Where that is not enough (a nucleus of thousands of tokens, more than 2048 at the bound) the row is put off:
+// piece's sum of w relative to its maximum, and the maxima of its quarters; a workgroup a row does the rest.  A draw from all tokens then needs
+// the pieces' sums and one piece.  Top-k and most nuclei lie among a few hundred tokens: the R-th largest of these
+// maxima is a bound that at least R tokens reach, so only quarters that reach it are read again, and what reaches it is
+// ranked in LDS (with a maximum a piece, 200 of 256 pieces were read for 200 ranks: 27 us of 50).  Where that is not enough (a nucleus of thousands of tokens, more than 2048 at the bound) the row is put off:
 // all workgroups together count its tokens and sum its w in bins over x, and list those of the border's bin; its own
 // workgroup then finds the border in bins over that bin's keys.  Sums that atomics make are of 64-bit integers, whose order does
 // not matter.  Few cases are left to a workgroup alone, in as many histograms as they take: top-k beyond the bound together
@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kPiece = 512;
 constexpr int kMaxPieces = 1024;  // the pieces' sums stay in LDS
+constexpr int kParts = 4;         // of a piece, the 128 logits of 16 lanes, each with a maximum of its own
 constexpr int kThreads = 512;     // of a row's workgroup
 constexpr int kWaves = kThreads / kWave;
 constexpr int kList = 2048;       // tokens ranked in LDS
@@ -60,7 +61,7 @@ struct SampleArgs {
     int64_t top_k_all;
     int64_t *tokens;
     float *logprobs;
-    float *piece_max;  // [rows][pieces], null: the row's workgroup makes them itself
+    float *part_max;  // [rows][pieces][kParts], null: the row's workgroup makes them itself
     double *piece_sum;
     int64_t stride;
     int vocab, pieces, each;  // each: pieces of a wave of the first pass
@@ -160,6 +161,14 @@ __device__ __forceinline__ double wave_sum64(double x) {
     h = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
     return __hiloint2double(int(h[0]), int(l[0])) + __hiloint2double(int(h[1]), int(l[1]));
 }
+// The maximum over a wave of what the lanes of each 16 have in common.
+__device__ __forceinline__ float max_of_rows(float x) {
+    uint32_t b = __float_as_uint(x);
+    auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    b = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+    r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 template <typename A> __device__ __forceinline__ A wave_scan(A x) {
     const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
@@ -176,8 +185,11 @@ template <typename T> struct Eight {
     gran_raw g[N];
     int c0;
     __device__ __forceinline__ void load(const T *row, int piece, int vocab) {
-        c0 = piece * kPiece + int(threadIdx.x & (kWave - 1)) * 8;
-        if ((piece + 1) * kPiece <= vocab) {
+        load_at(row, piece * kPiece + int(threadIdx.x & (kWave - 1)) * 8, (piece + 1) * kPiece <= vocab, vocab);
+    }
+    __device__ __forceinline__ void load_at(const T *row, int at, bool full, int vocab) {
+        c0 = at;
+        if (full) {
 #pragma unroll
             for (int i = 0; i < N; ++i) g[i] = *reinterpret_cast<const typename Gran<T>::raw_t *>(row + c0 + i * Gran<T>::EPC);
         } else {
@@ -208,13 +220,17 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// A piece's maximum and its sum of w relative to it, the same in every lane, from raw values: fmaxf and fmax take the
-// number of a NaN and a number, so that a NaN has the w of -inf.
-__device__ __forceinline__ void piece_stats(const float (&x)[8], const Scale &c, float &m, double &s) {
-    m = -INFINITY;
+// The maxima of a piece's parts in each lane of theirs, and its sum of w relative to the whole piece's maximum in every lane,
+// from raw values: fmaxf and fmax take the number of a NaN and a number, so that a NaN has the w of -inf.
+__device__ __forceinline__ void piece_stats(const float (&x)[8], const Scale &c, float &part, double &s) {
+    float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
-    m = wave_max_dpp(m) + 0.f;
+    m = fmaxf(m, dpp<0xB1>(m));
+    m = fmaxf(m, dpp<0x4E>(m));
+    m = fmaxf(m, dpp<0x141>(m));
+    part = fmaxf(m, dpp<0x140>(m)) + 0.f;
+    m = max_of_rows(part);
     s = 0.0;
     if (m == -INFINITY) return;
     if (m == INFINITY) {
@@ -241,14 +257,12 @@ template <typename T> __global__ __launch_bounds__(256) void sample_stats_kernel
     for (int p = p0; p < p1; ++p) {
         now = next;
         if (p + 1 < p1) next.load(x, p + 1, a.vocab);
-        float v[8], m;
+        float v[8], part;
         double s;
         now.get_raw(v);
-        piece_stats(v, scale, m, s);
-        if (lane == 0) {
-            a.piece_max[row * a.pieces + p] = m;
-            a.piece_sum[row * a.pieces + p] = s;
-        }
+        piece_stats(v, scale, part, s);
+        if (lane % 16 == 0) a.part_max[(row * a.pieces + p) * kParts + lane / 16] = part;
+        if (lane == 0) a.piece_sum[row * a.pieces + p] = s;
     }
 }
 
@@ -262,8 +276,14 @@ struct Shared {
         };
         uint64_t comp[kList];  // (key, ~id)
     };
-    double w[kList];
-    uint64_t sums[kMaxPieces];
+    union {
+        double w[kList];
+        float part_max[kMaxPieces * kParts];  // until tokens are listed
+    };
+    union {
+        uint64_t sums[kMaxPieces];
+        uint16_t wanted[kMaxPieces * kParts];  // parts to list tokens from
+    };
     uint32_t sub[kBins];
     uint64_t scratch[2 * kWaves];
     int32_t found, count;
@@ -352,15 +372,22 @@ __device__ __forceinline__ void each_piece(const T *x, int pieces, int vocab, Wa
 struct Bins {
     float m, by;
     __device__ __forceinline__ int of(float v) const { return v == m ? 0 : int(fminf((m - v) * by, float(kBins - 1))); }
-    // The lowest key of a bin <= at_most: the bins fall with the key.
-    __device__ uint32_t edge(int at_most) const {
-        uint32_t p = key_of(-INFINITY), q = key_of(m);
+    // The lowest key of a bin <= at_most: the bins fall with the key.  A wave's lanes try 64 keys at a time.
+    __device__ __forceinline__ uint32_t edge(int at_most) const {
+        const uint32_t lane = threadIdx.x & (kWave - 1);
+        uint32_t p = key_of(-INFINITY), q = key_of(m);  // it is one of p .. q
         while (p < q) {
-            const uint32_t mid = p + (q - p) / 2;
-            if (of(value_of(mid)) <= at_most) q = mid;
-            else p = mid + 1;
+            const uint32_t step = q - p < kWave ? 1u : (q - p) / kWave, key = p + lane * step;
+            const uint64_t in = __ballot(key >= q || of(value_of(key)) <= at_most);
+            if (in == 0) {
+                p += (kWave - 1) * step + 1;
+                continue;
+            }
+            const uint32_t first = uint32_t(__ffsll((unsigned long long)in) - 1), at = p + first * step;
+            if (first > 0) p = at - step + 1;
+            q = at < q ? at : q;
         }
-        return p;
+        return q;
     }
     __device__ uint32_t lowest(int b) const { return edge(b); }
     __device__ uint32_t highest(int b) const { return b > 0 ? edge(b - 1) - 1 : key_of(m); }
@@ -674,20 +701,79 @@ __device__ __forceinline__ int narrow(Shared &sh, int n, uint32_t lo, uint32_t h
     return sh.count;
 }
 
-// The value of rank `rank` (from 1) among v[0 .. n), n up to 64 Q, bit by bit, by every wave for itself.
-template <int Q> __device__ __forceinline__ float rank_value(const float *v, int n, int rank) {
-    const int lane = threadIdx.x & (kWave - 1);
-    uint32_t keys[Q], key = 0;
+// A value that at least `rank` of v[0 .. n) reach, n up to N, and few more: the upper BITS of the key of that rank, 8 at a
+// time in histograms of hist[], 256 numbers of zero for each.  Every wave finds the digits for itself.
+template <int BITS, int N> __device__ __forceinline__ float rank_bound(const float *v, int n, int rank, uint32_t *hist) {
+    constexpr int Q = N / kThreads;
+    const int t = threadIdx.x, lane = t & (kWave - 1);
+    uint32_t prefix = 0;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) keys[q] = q * kWave + lane < n ? key_of(v[q * kWave + lane]) : 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t with = key | 1u << bit;
-        int count = 0;
+    for (int shift = 24; shift >= 32 - BITS; shift -= 8, hist += 256) {
 #pragma unroll
-        for (int q = 0; q < Q; ++q) count += __popcll(__ballot(keys[q] >= with));
-        if (count >= rank) key = with;
+        for (int q = 0; q < Q; ++q) {
+            if (q * kThreads + t >= n) break;
+            const uint32_t key = key_of(v[q * kThreads + t]);
+            if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&hist[255 - (key >> shift & 255)], 1u);
+        }
+        __syncthreads();
+        uint32_t c[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * lane + i];
+        uint32_t run = wave_scan(sum);
+        const uint64_t past = __ballot(run >= uint32_t(rank));
+        const int at = past != 0 ? __ffsll((unsigned long long)past) - 1 : kWave - 1;
+        run -= sum;
+        int digit = 4 * lane + 3, left = rank - int(run);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (digit == 4 * lane + 3) {
+                if (left <= int(c[i])) digit = 4 * lane + i;
+                else left -= int(c[i]);
+            }
+        prefix = prefix << 8 | uint32_t(255 - __builtin_amdgcn_readlane(digit, at));
+        rank = __builtin_amdgcn_readlane(left, at);
     }
-    return value_of(key);
+    const uint32_t key = prefix << (32 - BITS), none = key_of(-INFINITY);
+    return value_of(key > none ? key : none);
+}
+// Lists the tokens that reach the bound, from the parts that hold any, 16 lanes a part; their number, which may pass the list's
+// length.
+template <typename T> __device__ __forceinline__ int collect_top(const T *x, int parts, int vocab, float bound, Shared &sh) {
+    constexpr int N = 16 / sizeof(T), G = kThreads / 16, P = kPiece / kParts;
+    const int t = threadIdx.x, lane = t & (kWave - 1);
+    __syncthreads();
+    if (t == 0) sh.count = sh.found = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < parts; i0 += kThreads) {
+        const bool want = i0 + t < parts && (bound == -INFINITY || sh.part_max[i0 + t] >= bound);
+        const uint64_t mask = __ballot(want);
+        if (mask == 0) continue;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&sh.found, __popcll(mask));
+        at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t(1) << lane) - 1));
+        if (want) sh.wanted[at] = uint16_t(i0 + t);
+    }
+    __syncthreads();
+    const int n = sh.found;
+    const uint32_t lo = key_of(bound);
+    for (int i0 = t / 16; i0 < n; i0 += N * G) {
+        Eight<T> g[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i0 + i * G < n) {
+                const int part = sh.wanted[i0 + i * G];
+                g[i].load_at(x, part * P + (t & 15) * 8, (part + 1) * P <= vocab, vocab);
+            }
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i0 + i * G < n) {
+                float v[8];
+                g[i].get(v);
+                append(&sh.count, sh.comp, v, g[i].c0, vocab, lo, 0xFFFFFFFFu);
+            }
+    }
+    __syncthreads();
+    return sh.count;
 }
 
 // What the kernels of a workgroup a row share.
@@ -709,6 +795,16 @@ template <typename T> struct RowWork {
     __device__ __forceinline__ double w_of(float v) const { return weight(v, top, r.scale); }
     __device__ __forceinline__ void finish(int64_t token, float value) const { finish_row(a, row, token, value, top, r.t, whole); }
 
+    // The first pass's maxima of the pieces, and of their parts where asked.
+    __device__ __forceinline__ void load_maxima(float *parts) const {
+        static_assert(kParts == 4, "16 bytes a piece");
+        const float4 *const from = reinterpret_cast<const float4 *>(a.part_max) + row * np;
+        for (int p = t; p < np; p += kThreads) {
+            const float4 m = from[p];
+            sh.pm[p] = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+            if (parts != nullptr) reinterpret_cast<float4 *>(parts)[p] = m;
+        }
+    }
     // The first token of the first piece that holds the maximum, which every run of ranks keeps.
     __device__ __forceinline__ void largest() {
         const int p = first_of(np, sh, [&](int i) { return sh.pm[i] == top; });
@@ -809,17 +905,18 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
     RowWork<T> w(a, sh, blockIdx.x);
     const int np = w.np, vocab = w.vocab, t = w.t, lane = w.lane;
     const Choice &c = w.c;
-    if (a.piece_max != nullptr) {
-        for (int p = t; p < np; p += kThreads) {
-            sh.pm[p] = a.piece_max[w.row * np + p];
-            sh.ps[p] = a.piece_sum[w.row * np + p];
-        }
+    for (int i = t; i < kBins; i += kThreads) sh.sub[i] = 0;
+    if (a.part_max != nullptr) {
+        w.load_maxima(sh.part_max);
+        for (int p = t; p < np; p += kThreads) sh.ps[p] = a.piece_sum[w.row * np + p];
     } else {
         each_piece(w.x, np, vocab, [](int) { return true; }, [&](int p, const Eight<T> &g) {
-            float v[8], m;
+            float v[8], part;
             double s;
             g.get_raw(v);
-            piece_stats(v, w.r.scale, m, s);
+            piece_stats(v, w.r.scale, part, s);
+            if (lane % 16 == 0) sh.part_max[p * kParts + lane / 16] = part;
+            const float m = max_of_rows(part);
             if (lane == 0) {
                 sh.pm[p] = m;
                 sh.ps[p] = s;
@@ -850,6 +947,8 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
         return;
     }
     // A bound that all kept tokens reach, if enough of them do; for rows that fit in the list then all.
+    const int parts = np * kParts;
+    constexpr int kBits = std::is_same<T, bf16_t>::value ? 16 : 24;  // of a key that a bound looks at
     for (int attempt = vocab > kThreads ? 0 : 1; attempt < (vocab > kList ? 1 : 2); ++attempt) {
         bool complete = true;  // no token that may be kept is below the bound
         float bound = -INFINITY;
@@ -861,8 +960,8 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
                 low = isinf(top) ? top : float(double(top) - under - 1e-6 * (fabs(double(top)) + under));
             }
             const int64_t reach = c.k < vocab ? c.k : c.share < 1.0 ? 128 : 0;
-            const bool by_thread = reach > np && reach <= kThreads;  // more ranks than pieces: maxima of every thread
-            if (reach > np && !by_thread && low == -INFINITY) continue;
+            const bool by_thread = reach > parts && reach <= kThreads;  // more ranks than parts: maxima of every thread
+            if (reach > parts && !by_thread && low == -INFINITY) continue;
             if (by_thread) {
                 float m = -INFINITY;
                 each_piece(w.x, np, vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
@@ -871,20 +970,17 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
 #pragma unroll
                     for (int e = 0; e < 8; ++e) m = fmaxf(m, v[e]);
                 });
-                float *const maxima = reinterpret_cast<float *>(sh.w);
-                maxima[t] = m;
-                __syncthreads();
-                bound = rank_value<kThreads / kWave>(maxima, kThreads, int(reach));
+                float *const maxima = reinterpret_cast<float *>(sh.comp);
+                maxima[t] = m;  // read by itself alone
+                bound = rank_bound<kBits, kThreads>(maxima, kThreads, int(reach), sh.sub);
                 complete = c.k < vocab || low >= bound;
-            } else if (reach > 0 && reach <= np) {
-                bound = np <= 2 * kWave   ? rank_value<2>(sh.pm, np, int(reach))
-                        : np <= 6 * kWave ? rank_value<6>(sh.pm, np, int(reach))
-                                          : rank_value<kMaxPieces / kWave>(sh.pm, np, int(reach));
+            } else if (reach > 0 && reach <= parts) {
+                bound = rank_bound<kBits, kMaxPieces * kParts>(sh.part_max, parts, int(reach), sh.sub);
                 complete = c.k < vocab || low >= bound;
             }
             bound = fmaxf(bound, low);
         }
-        const int n = collect(w.x, np, vocab, key_of(bound), 0xFFFFFFFFu, [&](int p) { return sh.pm[p] >= bound; }, sh);
+        const int n = collect_top(w.x, parts, vocab, bound, sh);
         if (n <= kList) {
             sort_list(sh, n, top, w.r.scale);
             scan_array<kList>(sh.w, n, sh.scratch);
@@ -1087,7 +1183,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_finish_
         const int np = w.np, vocab = w.vocab, t = w.t, lane = w.lane;
         const Choice &c = w.c;
         float top = -INFINITY;
-        for (int p = t; p < np; p += kThreads) sh.pm[p] = a.piece_max[w.row * np + p];
+        w.load_maxima(nullptr);
         __syncthreads();
         for (int p = lane; p < np; p += kWave) top = fmaxf(top, sh.pm[p]);
         w.top = wave_max_dpp(top);
@@ -1277,7 +1373,7 @@ Space space_of(int64_t rows, int64_t vocab) {
     const auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     s.most = int(std::min<int64_t>(rows, 1024));
     s.maxima = up(rows * pieces_of(vocab) * 8);
-    s.put_off = s.maxima + up(rows * pieces_of(vocab) * 4);
+    s.put_off = s.maxima + up(rows * pieces_of(vocab) * kParts * 4);
     s.wide = s.put_off + up((rows + 1) * 4);
     s.bytes = s.wide + s.most * int64_t(sizeof(Wide));
     return s;
@@ -1295,11 +1391,11 @@ template <typename T> hipError_t sample(SampleArgs &a, int64_t rows, void *works
     const Space space = space_of(rows, a.vocab);
     char *const ws = static_cast<char *>(workspace);
     a.piece_sum = reinterpret_cast<double *>(ws);
-    a.piece_max = reinterpret_cast<float *>(ws + space.maxima);
+    a.part_max = reinterpret_cast<float *>(ws + space.maxima);
     // 4 pieces a wave where that leaves the chip 4096 waves.
     a.each = rows * a.pieces >= 4 * 4096 ? 4 : 1;
     // A border that is not near the top is for the whole chip, unless top-k says that it is (or a bound by min-p alone).
-    const bool near = !a.top_k && ((a.top_k_all > 0 && a.top_k_all <= a.pieces) ||
+    const bool near = !a.top_k && ((a.top_k_all > 0 && a.top_k_all <= a.pieces * kParts) ||
                                    (!a.top_p && !(a.top_p_all < 1.0) && (a.top_k_all <= 0 || a.top_k_all >= a.vocab)));
     if (!near) {
         a.put_off = reinterpret_cast<int32_t *>(ws + space.put_off);
