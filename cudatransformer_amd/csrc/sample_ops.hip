@@ -42,8 +42,15 @@ constexpr int kList = 2048;       // tokens ranked in LDS
 constexpr int kBins = 1024;
 constexpr double kLog2e64 = 1.4426950408889634074;
 
+// A bin that holds a border: its keys, how many tokens and how much w are above it, and the w that the border leaves above itself.
+struct BorderBin {
+    uint32_t lo, hi;
+    int64_t above;
+    double base, target;
+};
 // A row whose border is found by all of the chip: tokens and w (in integers) of bins over x, and the tokens of the border's bin.
 struct Wide {
+    BorderBin border;
     uint64_t mass[kBins];
     uint64_t list[kList];
     uint32_t cnt[kBins];
@@ -1079,15 +1086,9 @@ template <typename T> __global__ __launch_bounds__(256) void sample_bins_kernel(
     });
 }
 
-// The border's bin, as every workgroup finds it for itself from the row's bins: how many tokens and how much w are above.
-struct BorderBin {
-    uint32_t lo, hi;
-    int64_t above;
-    double base;
-};
-// By a workgroup of NT threads, each of which sums 1024 / NT bins.
-template <int NT> __device__ __forceinline__ BorderBin border_bin(const Wide &wide, const Choice &c, int vocab, const Bins &bins, uint64_t *scratch, int *found) {
-    constexpr int Q = kBins / NT, W = NT / kWave;
+// The border's bin, as every workgroup of 256 threads finds it for itself from the row's bins, 4 a thread.
+__device__ __forceinline__ BorderBin border_bin(const Wide &wide, const Choice &c, int vocab, const Bins &bins, uint64_t *scratch, int *found) {
+    constexpr int Q = kBins / 256, W = 256 / kWave;
     const int t = threadIdx.x, lane = t & (kWave - 1), wave = t / kWave;
     const Fixed f = fixed_of(wide.whole);
     uint64_t mass[Q], cnt[Q];
@@ -1114,7 +1115,7 @@ template <int NT> __device__ __forceinline__ BorderBin border_bin(const Wide &wi
         }
         all += scratch[v];
     }
-    const double target = c.share * f.sum(all);
+    const double target = c.share * f.sum(all);  // of the integers' sum, as the bins are
     int b = kBins;
 #pragma unroll
     for (int q = Q - 1; q >= 0; --q)
@@ -1136,7 +1137,7 @@ template <int NT> __device__ __forceinline__ BorderBin border_bin(const Wide &wi
         scratch[1] = n;
     }
     __syncthreads();
-    const BorderBin out{bins.lowest(first), bins.highest(first), int64_t(scratch[1]), f.sum(scratch[0])};
+    const BorderBin out{bins.lowest(first), bins.highest(first), int64_t(scratch[1]), f.sum(scratch[0]), target};
     __syncthreads();
     return out;
 }
@@ -1154,7 +1155,8 @@ template <typename T> __global__ __launch_bounds__(256) void sample_list_kernel(
 #pragma unroll
         for (int q = 0; q < kChunk / 4; ++q)
             if (p0 + 4 * q + wave < a.pieces) g[q].load(x, p0 + 4 * q + wave, a.vocab);
-        const BorderBin b = border_bin<256>(wide, c, a.vocab, bins_of(wide.top, r.scale), scratch, &found);
+        const BorderBin b = border_bin(wide, c, a.vocab, bins_of(wide.top, r.scale), scratch, &found);
+        if (p0 == 0 && threadIdx.x == 0) wide.border = b;
 #pragma unroll
         for (int q = 0; q < kChunk / 4; ++q) {
             const int p = p0 + 4 * q + wave;
@@ -1200,30 +1202,23 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_finish_
         bool drawn = false;
         if (n > 0 && n <= kList) {
             const Wide &wide = a.wide[at];
-            BorderBin b = border_bin<kThreads>(wide, c, vocab, bins_of(w.top, w.r.scale), sh.scratch, &sh.found);
+            BorderBin b = wide.border;
             for (int p = t; p < np; p += kThreads) {
                 sh.ps[p] = a.piece_sum[w.row * np + p];
                 sh.sums[p] = 0;
             }
             for (int i = t; i < n; i += kThreads) sh.comp[i] = wide.list[i];
             __syncthreads();
-            const Fixed f = fixed_of(w.whole);
             // Where min-p leaves nothing of the bin, any border in it will do.
             const bool none = !(w.w_of(value_of(b.hi)) >= c.least);
             const bool by_count = none || c.k < vocab;
-            // The target is a share of the integers' sum, as the bins are.
-            uint64_t all = 0;
-            for (int i = lane; i < kBins; i += kWave) all += wide.mass[i];
-#pragma unroll
-            for (int off = kWave / 2; off > 0; off >>= 1) all += __shfl_xor(all, off, kWave);
-            const double target = c.share * f.sum(all);
-            n = narrow(sh, n, b.lo, b.hi, by_count, none ? b.above + 1 : c.k, target, c.least, w.top, w.r.scale, w.whole, b.above, b.base);
+            n = narrow(sh, n, b.lo, b.hi, by_count, none ? b.above + 1 : c.k, b.target, c.least, w.top, w.r.scale, w.whole, b.above, b.base);
             if (n > 0) {
                 sort_list(sh, n, w.top, w.r.scale);
                 scan_array<kList>(sh.w, n, sh.scratch);
                 int keep = 1;
                 if (by_count) keep = none ? 1 : int(c.k - b.above);
-                else keep = 1 + first_of(n, sh, [&](int i) { return b.base + sh.w[i] >= target; });
+                else keep = 1 + first_of(n, sh, [&](int i) { return b.base + sh.w[i] >= b.target; });
                 keep = keep > n ? n : keep;  // the integers' sum passes the target, this one by its rounding may not
                 if (keep > 0) {
                     __syncthreads();
