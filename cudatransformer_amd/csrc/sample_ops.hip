@@ -7,19 +7,21 @@
 // that near a border).
 //
 // A row is pieces of 512 logits, 8 a lane of a wave.  One pass over the logits, spread over the chip, leaves each
-// piece's sum of w relative to its maximum, and the maxima of its quarters; a workgroup a row does the rest.  A draw from all tokens then needs
-// the pieces' sums and one piece.  Top-k and most nuclei lie among a few hundred tokens: the R-th largest of these
-// maxima is a bound that at least R tokens reach, so only quarters that reach it are read again, and what reaches it is
-// ranked in LDS (with a maximum a piece, 200 of 256 pieces were read for 200 ranks: 27 us of 50).  Where that is not enough (a nucleus of thousands of tokens, more than 2048 at the bound) the row is put off:
-// all workgroups together count its tokens and sum its w in bins over x, and list those of the border's bin; its own
-// workgroup then finds the border in bins over that bin's keys.  Sums that atomics make are of 64-bit integers, whose order does
-// not matter.  Few cases are left to a workgroup alone, in as many histograms as they take: top-k beyond the bound together
-// with top-p, thousands of equal logits.
+// piece's sum of w relative to its maximum, and the maxima of its quarters; a workgroup a row does the rest.  A draw from
+// all tokens then needs the pieces' sums and one piece.  Top-k and most nuclei lie among a few hundred tokens: the R-th
+// largest of these maxima is a bound that at least R tokens reach, so only quarters that reach it are read again, and
+// what reaches it is ranked in LDS (with a maximum a piece instead, 200 of 256 pieces were read for 200 ranks: 27 us of
+// the workgroup's 50).  Where that is not enough (a nucleus of thousands of tokens, more than 2048 at the bound) the row is
+// put off: all workgroups together count its tokens and sum its w in bins over x, and list those of the border's bin; its
+// own workgroup then finds the border in bins over that bin's keys.  Sums that atomics make are of 64-bit integers, whose
+// order does not matter.  Few cases are left to a workgroup alone, in as many histograms as they take: top-k beyond the bound
+// together with top-p, thousands of equal logits.
 //
 // Measured, 256 rows of 131072 bf16 logits: the first pass 31 us (2.1 TB/s, of 13 us at 5.1: 18 64-bit operations a logit keep
-// the vector units busy), without filters 38 in all, top-k 50 with top-p 60 (the row's workgroup is latencies: LDS, barriers, a
-// few loads one after the other), each row its own parameters 140, where 18 rows are put off (10 us of bins, 17 of lists, 36
-// of borders; by their own workgroups alone 303).  One row of 50257, top-k 50: 3 + 21 us.
+// the vector units busy; by a table of 64 roots in LDS, 13 of them, 30), without filters 38 in all, top-k 50 54 and top-k 200
+// 62 (the row's workgroup is latencies: LDS, barriers, a few loads one after the other), each row its own parameters 107 to
+// 113, where 18 rows are put off (10 us of bins, 16 of lists, 27 of borders; by their own workgroups alone over 200).  One row
+// of 50257, top-k 50: 3 + 18 us.  1024 threads a row instead of 512 cost 20 us more.
 #include "attn_common.h"
 #include "attn_launch.h"
 #include "capi_bytes.h"
