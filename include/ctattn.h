@@ -719,8 +719,8 @@ CTATTN_API int ctattn_muon_update_multi(int dtype, int count, void *const *param
 
 /*
  * Pages for new_lens[i] new tokens of each request, that holds lens[i] (numbers below 0 count as 0), and where each goes.
- * Requests are served in order; one whose tokens do not all find room (in the table's width, in max_tokens rows, among
- * the free pages) gets none, and those behind it that need no fresh page or fit in what is left are served.
+ * Requests are served in order, whole or not at all: one whose tokens pass the table's width or max_tokens rows gets nothing
+ * and takes no pages; behind one for which too few pages are free only those that need no fresh page are served.
  *   table        [requests][table_row]: entries of the fresh pages are written, no others
  *   starts       [requests + 1]: the first row of each request's new tokens, served or not; at the end their number
  *   slots        [max_tokens]: page * page_size + place of each row, -1 for rows of unserved requests and behind the last

@@ -238,3 +238,23 @@ def test_c_refusals():
                dict(ws_bytes=5), dict(ws=(1 << 30) + 8), dict(tokens=1 << 12), dict(ws=1 << 20), dict(logprobs=1 << 13)):
         assert call(**kw) != 0, kw
     assert lib.ctattn_sample_workspace_bytes(-1, 5) == -1 and lib.ctattn_sample_workspace_bytes(5, 0) == -1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1500, 20000, 131072])
+def test_ranks_about_the_number_of_parts(dtype, vocab):
+    """As many ranks as there are runs of 128 logits, one fewer and more; few tokens that are not masked; logits all below zero,
+    of large values, in few places."""
+    parts = 4 * -(-vocab // 512)
+    x, u = logits_of(6, vocab, dtype, vocab + 1)
+    x[1] -= 60.0  # all below zero
+    x[2, torch.randperm(vocab, generator=torch.Generator().manual_seed(2))[:vocab - 5].cuda()] = -math.inf
+    x[3, 300:] = -math.inf  # in three runs of 128
+    x[4] *= 300.0
+    x[5] = x[5].sort().values  # the largest behind each other
+    for k in (128, parts - 1, parts, parts + 1, 511, 512, 513):
+        for how in (dict(k=k), dict(k=k, p=0.7, t=3.0), dict(k=k, m=0.01)):
+            check(x, u, **how)
+    for how in (dict(p=0.3), dict(p=0.9, t=4.0), dict(m=1e-4, p=0.99)):
+        check(x, u, **how)
