@@ -296,6 +296,7 @@ struct Shared {
     uint32_t sub[kBins];
     uint64_t scratch[2 * kWaves];
     int32_t found, count;
+    int32_t place;  // of a row put off; not `count`, which waves may still be reading as the list's length then
     uint32_t key;
     int64_t token;
 };
@@ -1012,9 +1013,9 @@ template <typename T, bool PUT_OFF> __global__ __launch_bounds__(kThreads) void 
         }
     }
     if constexpr (PUT_OFF) {
-        if (t == 0) sh.count = atomicAdd(a.put_off, 1);
+        if (t == 0) sh.place = atomicAdd(a.put_off, 1);
         __syncthreads();
-        const int at = sh.count;
+        const int at = sh.place;
         if (t == 0) a.put_off[1 + at] = int32_t(w.row);
         if (at >= a.most) return;
         Wide &wide = a.wide[at];

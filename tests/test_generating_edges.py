@@ -133,3 +133,18 @@ def test_least_temperatures_draw_the_largest(vocab, how, temperature):
     assert (x.topk(2).values[:, 0] > x.topk(2).values[:, 1]).all()
     tokens, logprobs = ct.sample_tokens(x, torch.tensor([0.0, 0.5, 0.999], device="cuda"), temperature, **how)
     assert torch.equal(tokens, x.argmax(1)) and (logprobs == 0).all()
+
+
+@gpu
+def test_lists_that_overflow_in_every_row():
+    """Rows whose list of candidates is too long, so that each takes a place among those put off while its waves read the
+    list's length: 300 at once, the same tokens in every call."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randint(-4, 4, (300, 20000), generator=g).to(torch.bfloat16).cuda()  # 2500 equal ones at the top
+    u = torch.rand(300, generator=g).cuda()
+    first = check(x, u, p=0.95)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, ct.sample_tokens(x, u, top_p=0.95)))
+    # Beside rows that draw from their list at once.
+    k = torch.tensor([5, 0, 3000], dtype=torch.int32, device="cuda").repeat(100)
+    check(x, u, k=k)
