@@ -76,7 +76,9 @@ hipError_t launch_shared_generic(const SharedCall &c, hipStream_t stream);
 // MFMA kernels: fp32, bf16, fp16; d whole 16-byte chunks up to 128, at most 128 query heads to a key head;
 // pointers and strides of q, o and the caches on 16 bytes.
 bool shared_mfma_supported(int dtype, int64_t d, int64_t group);
+// What a call needs, and the most that any call of these sizes does, with or without starts and group_starts.
 int64_t shared_workspace_bytes(const SharedCall &c);
+int64_t shared_workspace_most(const SharedCall &c);
 hipError_t launch_shared(const SharedCall &c, void *workspace, hipStream_t stream);
 
 }  // namespace ctattn

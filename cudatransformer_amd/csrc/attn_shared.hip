@@ -601,7 +601,7 @@ template <typename F> __global__ __launch_bounds__(256) void shared_join_kernel(
     if (a.lse != nullptr && c == 0) a.lse[rh] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
-// Tiles and splits, from the call's shapes alone.
+// Tiles and splits, from the call's shapes and whether it says which rows and requests belong together.
 struct Plan {
     bool tall_prefix, tall_own;
     int ptiles, psplits, otiles, osplits, pper, oper, omost;
@@ -614,7 +614,7 @@ int64_t keys_each(int64_t tiles, int64_t most, bool tall) {
     const int64_t x = tiles * most / 4096, lo = tall ? 256 : 64, hi = tall ? 1024 : 512;
     return (std::max(std::min(std::max(x, lo), hi), most / 64) + 63) / 64 * 64;
 }
-Plan plan_of(const SharedCall &c) {
+Plan plan_of(const SharedCall &c, bool starts, bool group_starts) {
     Plan p{};
     const int64_t work_rows = c.rows * c.group();
     const auto div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
@@ -622,14 +622,14 @@ Plan plan_of(const SharedCall &c) {
     p.tall_prefix = p.tall_own || (c.groups > 0 && work_rows > 32 * c.groups);
     if (c.requests > 0) {
         const int64_t bm = p.tall_own ? 128 : 32;
-        p.oper = c.starts ? 0 : int(div(c.group(), bm));
+        p.oper = starts ? 0 : int(div(c.group(), bm));
         p.otiles = int(p.oper > 0 ? p.oper * c.requests : work_rows / bm + c.requests);
         p.omost = int(keys_each(p.otiles * c.hkv, c.max_own(), p.tall_own));
         p.osplits = int(std::max<int64_t>(1, div(c.max_own(), p.omost)));
     }
     if (c.max_prefix() > 0) {
         const int64_t bm = p.tall_prefix ? 128 : 32;
-        p.pper = c.starts || c.group_starts ? 0 : int(div(c.requests / c.groups * c.group(), bm));
+        p.pper = starts || group_starts ? 0 : int(div(c.requests / c.groups * c.group(), bm));
         p.ptiles = int(p.pper > 0 ? p.pper * c.groups : c.groups == 1 ? div(work_rows, bm) : work_rows / bm + c.groups);
         // Tall: a workgroup a CU where the requests' own keys are as many, so that these stream in beside it, and two
         // where not (32768 keys, 1024 rows of 8 key heads, with 1 to 2048 keys of 256 requests' own: 306 us with 256
@@ -640,8 +640,13 @@ Plan plan_of(const SharedCall &c) {
     }
     return p;
 }
+Plan plan_of(const SharedCall &c) { return plan_of(c, c.starts != nullptr, c.group_starts != nullptr); }
 int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
 int64_t dp_of(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+int64_t workspace_of(const SharedCall &c, const Plan &p) {
+    const int64_t row_heads = (p.psplits + p.osplits) * c.rows * c.hq;
+    return up(row_heads * dp_of(c.d) * 4) + up(row_heads * 8);
+}
 
 template <typename F, int D, bool PAD> hipError_t launch_d(const Args &a, const Plan &p, hipStream_t stream) {
     const int64_t prompts = int64_t(p.ptiles) * p.psplits * a.lay.hkv, own = int64_t(p.otiles) * p.osplits * a.lay.hkv;
@@ -704,10 +709,16 @@ bool shared_mfma_supported(int dtype, int64_t d, int64_t group) {
     return dtype <= 2 && d <= 128 && (d * e) % 16 == 0 && group <= 128;
 }
 
-int64_t shared_workspace_bytes(const SharedCall &c) {
-    const Plan p = plan_of(c);
-    const int64_t row_heads = (p.psplits + p.osplits) * c.rows * c.hq;
-    return up(row_heads * dp_of(c.d) * 4) + up(row_heads * 8);
+int64_t shared_workspace_bytes(const SharedCall &c) { return workspace_of(c, plan_of(c)); }
+
+int64_t shared_workspace_most(const SharedCall &c) {
+    // With starts the groups' make no difference; other than one row a request is never without.
+    int64_t most = workspace_of(c, plan_of(c, true, false));
+    if (c.rows == c.requests) {
+        most = std::max(most, workspace_of(c, plan_of(c, false, true)));
+        if (c.groups == 0 || c.requests % c.groups == 0) most = std::max(most, workspace_of(c, plan_of(c, false, false)));
+    }
+    return most;
 }
 
 hipError_t launch_shared(const SharedCall &c, void *workspace, hipStream_t stream) {

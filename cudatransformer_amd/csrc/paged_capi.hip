@@ -63,7 +63,7 @@ int64_t ctattn_shared_prefix_workspace_bytes(int dtype, int64_t rows, int64_t re
     c.table_width = table_width;
     c.prefix_width = prefix_width;
     if (check_sizes("ctattn_shared_prefix_workspace_bytes", c) != 0) return -1;
-    return rows > 0 && shared_mfma_supported(dtype, d, c.group()) ? shared_workspace_bytes(c) : 0;
+    return rows > 0 && shared_mfma_supported(dtype, d, c.group()) ? shared_workspace_most(c) : 0;
 }
 
 int ctattn_shared_prefix_fwd(int dtype, const void *q, const void *k_cache, const void *v_cache, const int32_t *table,

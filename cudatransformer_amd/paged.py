@@ -181,7 +181,7 @@ def _shared_prefix_need(code, *sizes):
 
 def shared_prefix_workspace_bytes(dtype, rows: int, requests: int, groups: int, num_heads: int, num_kv_heads: int, d: int,
                                   page_size: int, table_width: int, prefix_width: int) -> int:
-    """Bytes of the workspace of flash_attn_shared_prefix."""
+    """Bytes of the workspace of flash_attn_shared_prefix, with or without starts and group_starts."""
     return _shared_prefix_need(_DTYPE_CODE[dtype], rows, requests, groups, num_heads, num_kv_heads, d, page_size, table_width,
                                prefix_width)
 

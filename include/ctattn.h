@@ -756,7 +756,8 @@ CTATTN_API int ctattn_cache_write(int dtype, const void *k, const void *v, void 
                                   const int64_t *slots, const int64_t *strides, int64_t rows, int64_t hkv, int64_t d,
                                   int64_t pages, int64_t page_size, void *stream);
 
-/* Bytes of device workspace ctattn_shared_prefix_fwd needs, or -1 on invalid arguments. */
+/* Bytes of device workspace that suffice for every call of ctattn_shared_prefix_fwd of these sizes, with or without starts and
+ * group_starts, or -1 on invalid arguments. */
 CTATTN_API int64_t ctattn_shared_prefix_workspace_bytes(int dtype, int64_t rows, int64_t requests, int64_t groups,
                                                         int64_t hq, int64_t hkv, int64_t d, int64_t page_size,
                                                         int64_t table_width, int64_t prefix_width);

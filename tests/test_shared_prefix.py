@@ -1,6 +1,7 @@
 """Attention of requests that share a prompt in a paged cache (cudatransformer_amd.paged) against 64 bits."""
 import ctypes
 import math
+import re
 
 import pytest
 import torch
@@ -340,3 +341,55 @@ def test_c_refusals():
         a = {**good, **kw}
         assert lib.ctattn_shared_prefix_workspace_bytes(*[a[x] for x in ("dtype", "rows", "requests", "groups", "hq", "hkv", "d",
                                                                          "page_size", "table_width", "prefix_width")]) == -1
+
+
+def needed(starts, group_starts, dtype=1, rows=32, requests=256, groups=1, hq=32, hkv=8, d=128, pages=1 << 20, page=16, width=128,
+           prefix_width=256):
+    """(bytes that the workspace query says, bytes that the call itself asks for); the call is given none and never launches."""
+    lib = _capi.load()
+    head = hkv * d
+    strides = (ctypes.c_int64 * 12)(hq * d, d, hq * d, d, page * head, head, d, page * head, head, d, width, prefix_width)
+    p = [(i + 1) << 44 for i in range(11)]
+    rc = lib.ctattn_shared_prefix_fwd(dtype, *p[:7], p[7] if group_starts else None, p[8] if starts else None, p[9], None, p[10], 0, strides,
+                                      rows, requests, groups, hq, hkv, d, pages, page, width, prefix_width, 0, None)
+    said = re.search(r"workspace too small \(0 bytes, (\d+) needed\)", _capi.last_error())
+    assert rc != 0 and said, _capi.last_error()
+    return lib.ctattn_shared_prefix_workspace_bytes(dtype, rows, requests, groups, hq, hkv, d, page, width, prefix_width), int(said[1])
+
+
+SIZES = [dict(rows=n) for n in (1, 2, 31, 32, 33, 100, 192, 255, 257, 300, 1000, 5000)]
+SIZES += [dict(rows=n, groups=8) for n in (1, 17, 64, 65, 250, 400)]
+SIZES += [dict(rows=n, requests=64, hq=16, hkv=16, d=64) for n in (1, 32, 63, 65, 2000)]
+SIZES += [dict(rows=4096, requests=16, width=1024, prefix_width=64), dict(rows=8192, requests=8, width=2048, prefix_width=64),
+          dict(rows=1800, requests=24, hq=16, hkv=16, d=64, page=32, width=22, prefix_width=129, dtype=2),
+          dict(rows=7, requests=9, hq=6, hkv=6, d=64, dtype=0), dict(rows=5, requests=3, groups=0, prefix_width=0)]
+
+
+@pytest.mark.parametrize("kw", SIZES, ids=str)
+def test_workspace_of_calls_with_starts(kw):
+    """Requests without a new token, and with several: what the query says is what the call needs."""
+    for group_starts in (False, True):
+        query, need = needed(True, group_starts, **kw)
+        assert query == need
+
+
+@pytest.mark.parametrize("kw", [dict(rows=n, requests=n, groups=g, hq=hq, hkv=8) for n in (1, 4, 48, 256) for g in (1, 3, 4) for hq in (8, 32, 512)],
+                         ids=str)
+def test_workspace_suffices_for_one_row_a_request(kw):
+    forms = [(True, True), (False, True)]
+    if kw["requests"] % kw["groups"] == 0:  # equal groups
+        forms += [(True, False), (False, False)]
+    got = [needed(*f, **kw) for f in forms]
+    assert got[0][0] == max(need for _, need in got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 32, 8, 128), (F32, 4, 4, 64)])
+def test_most_requests_have_no_new_token(dtype, hq, hkv, d):
+    """Fewer rows than requests, one group and several, a request's first token and a later one."""
+    own = [3 * i % 50 + 1 for i in range(40)]
+    for rows in ([3], [0, 39], [1, 2, 3, 20, 21]):
+        new = [int(i in rows) + (2 if i == 20 and 20 in rows else 0) for i in range(40)]
+        for prompts, sizes in (([300], [40]), ([300, 17, 0], [10, 25, 5])):
+            b = Batch(dtype, prompts, sizes, new, [max(n, m) for n, m in zip(own, new)], hq, hkv, d, 16)
+            b.check(b.call(**(dict(group_starts=None) if len(prompts) == 1 else {})))
