@@ -612,7 +612,7 @@ struct Plan {
 // 69 / 71 / 70 / 84).  At most 64 stretches.
 int64_t keys_each(int64_t tiles, int64_t most, bool tall) {
     const int64_t x = tiles * most / 4096, lo = tall ? 256 : 64, hi = tall ? 1024 : 512;
-    return (std::max(std::min(std::max(x, lo), hi), most / 64) + 63) / 64 * 64;
+    return (std::max(std::min(std::max(x, lo), hi), (most + 63) / 64) + 63) / 64 * 64;
 }
 Plan plan_of(const SharedCall &c, bool starts, bool group_starts) {
     Plan p{};

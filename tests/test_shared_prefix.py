@@ -393,3 +393,10 @@ def test_most_requests_have_no_new_token(dtype, hq, hkv, d):
         for prompts, sizes in (([300], [40]), ([300, 17, 0], [10, 25, 5])):
             b = Batch(dtype, prompts, sizes, new, [max(n, m) for n, m in zip(own, new)], hq, hkv, d, 16)
             b.check(b.call(**(dict(group_starts=None) if len(prompts) == 1 else {})))
+
+
+@pytest.mark.parametrize("width", [2047, 2048, 2049, 2050, 4097, 6145, 8191, 100001])
+def test_at_most_64_stretches(width):
+    """Of one request's own keys: each leaves 32 heads of 128 fp32 numbers, a maximum and a sum."""
+    query, need = needed(True, False, rows=1, requests=1, groups=0, prefix_width=0, width=width)
+    assert query == need and need % (32 * (128 + 2) * 4) == 0 and need // (32 * (128 + 2) * 4) <= 64
