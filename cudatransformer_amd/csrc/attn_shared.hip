@@ -606,13 +606,21 @@ struct Plan {
     bool tall_prefix, tall_own;
     int ptiles, psplits, otiles, osplits, pper, oper, omost;
 };
-// A request's own keys that one work item takes, where `tiles` tiles of rows and key heads have up to `most` each.  Flat:
-// 4096 waves, two for every wave's place, and no more than 512 keys a wave, for lengths differ (256 requests of 1 to 2048
-// keys, 8 key heads of 128: 128 / 256 / 512 / 1024 keys 226 / 220 / 220 / 238 us; 128 requests of 1 to 1024:
-// 69 / 71 / 70 / 84).  At most 64 stretches.
-int64_t keys_each(int64_t tiles, int64_t most, bool tall) {
+int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+int64_t dp_of(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
+// A request's own keys that one work item takes, where `tiles` tiles of rows and key heads have up to `most` each and all rows'
+// O is `bytes`.  Flat: 4096 waves, two for every wave's place, and no more than 512 keys a wave, for lengths differ (256
+// requests of 1 to 2048 keys, 8 key heads of 128: 128 / 256 / 512 / 1024 keys 226 / 220 / 220 / 238 us; 128 requests of
+// 1 to 1024: 69 / 71 / 70 / 84).  At most 64 stretches, and no more than leave 256 MB of partial O, whatever the table's width:
+// with as many rows the chip is full, and every stretch writes and reads them (tables of 32768 tokens, 32/8 heads of 128, bf16,
+// on a prompt of 512; bound of 64 / 256 / 1024 MB, and none: 8192 rows of 8 full requests 4.7 / 4.7 / 4.9 and 6.3 ms, of
+// short ones 348 / 348 / 415 and 780 us; 1024 rows of one request each of 1 to 4000 tokens 1.55 / 1.54 / 1.87 and 1.87 ms, with
+// one of 32768 among short ones 970 / 740 / 970 and 970 us; tables of 131072, 75 rows of each of 24 requests, one of them full:
+// 1540 / 570 / 520 and 620 us).
+int64_t keys_each(int64_t tiles, int64_t most, bool tall, int64_t bytes) {
     const int64_t x = tiles * most / 4096, lo = tall ? 256 : 64, hi = tall ? 1024 : 512;
-    return (std::max(std::min(std::max(x, lo), hi), (most + 63) / 64) + 63) / 64 * 64;
+    const int64_t parts = std::min(int64_t(64), std::max(int64_t(1), (int64_t(256) << 20) / bytes));
+    return (std::max(std::min(std::max(x, lo), hi), (most + parts - 1) / parts) + 63) / 64 * 64;
 }
 Plan plan_of(const SharedCall &c, bool starts, bool group_starts) {
     Plan p{};
@@ -624,7 +632,7 @@ Plan plan_of(const SharedCall &c, bool starts, bool group_starts) {
         const int64_t bm = p.tall_own ? 128 : 32;
         p.oper = starts ? 0 : int(div(c.group(), bm));
         p.otiles = int(p.oper > 0 ? p.oper * c.requests : work_rows / bm + c.requests);
-        p.omost = int(keys_each(p.otiles * c.hkv, c.max_own(), p.tall_own));
+        p.omost = int(keys_each(p.otiles * c.hkv, c.max_own(), p.tall_own, c.rows * c.hq * dp_of(c.d) * 4));
         p.osplits = int(std::max<int64_t>(1, div(c.max_own(), p.omost)));
     }
     if (c.max_prefix() > 0) {
@@ -641,8 +649,6 @@ Plan plan_of(const SharedCall &c, bool starts, bool group_starts) {
     return p;
 }
 Plan plan_of(const SharedCall &c) { return plan_of(c, c.starts != nullptr, c.group_starts != nullptr); }
-int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
-int64_t dp_of(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 int64_t workspace_of(const SharedCall &c, const Plan &p) {
     const int64_t row_heads = (p.psplits + p.osplits) * c.rows * c.hq;
     return up(row_heads * dp_of(c.d) * 4) + up(row_heads * 8);

@@ -400,3 +400,26 @@ def test_at_most_64_stretches(width):
     """Of one request's own keys: each leaves 32 heads of 128 fp32 numbers, a maximum and a sum."""
     query, need = needed(True, False, rows=1, requests=1, groups=0, prefix_width=0, width=width)
     assert query == need and need % (32 * (128 + 2) * 4) == 0 and need // (32 * (128 + 2) * 4) <= 64
+
+
+@pytest.mark.parametrize("kw", [dict(rows=8192, requests=8, width=2048), dict(rows=8192, requests=1, width=2048), dict(rows=2048, requests=1, width=8192),
+                                dict(rows=4096, requests=4096, width=2048), dict(rows=30000, requests=20, width=8192),
+                                dict(rows=256, requests=256, width=2048), dict(rows=1800, requests=24, width=8192, prefix_width=9000)], ids=str)
+def test_workspace_of_wide_tables(kw):
+    """What the splits leave is bounded by the rows, not by the width of tables made for the longest request: 256 MB of
+    partial O (a number in 32 heads of 128, with a maximum and a sum for each) or one split, and as much as the prompt's."""
+    query, need = needed(True, False, **kw)
+    one = kw["rows"] * 32 * (128 + 2) * 4
+    prompt = 512 * 128 * (128 + 2) * 4  # 512 work items of 128 rows
+    assert need <= query <= max((256 << 20) * 130 // 128, one) + max(prompt, one) + 1024
+
+
+@gpu
+def test_many_rows_on_wide_tables():
+    """So many rows that the partial O, not 64 stretches, bounds the splits of wide tables: 21 of 1472 keys, which two requests
+    pass, and 21 of which all but the first are empty."""
+    new = [700, 1, 1500, 0, 800]
+    b = Batch(BF16, [40], [5], new, [900, 70, 1500, 3, 2000], 16, 2, 64, 16)
+    for width in (1900, 120000):
+        b.table = torch.cat([b.table, torch.full((5, width - b.table.shape[1]), -1, dtype=torch.int32)], 1)
+        b.check(b.call())
