@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -194,8 +195,8 @@ def flash_attn_shared_prefix(q, k_cache, v_cache, table, lens, prefix_table=None
     table [requests, pages] and lens [requests] are the requests' pages and own tokens, the new ones among them;
     prefix_table [groups, pages] and prefix_lens [groups] the prompts' (None: no prompts); int32.  group_starts [groups + 1] are
     the first requests of the groups (None: equal groups), starts [requests + 1] the first rows of the requests, whose last
-    tokens the rows are (None: one row a request).  Rows of no request are left as they are, zeros where the
-    output is allocated here."""
+    tokens the rows are (None: one row a request).  Rows of no request are left as they are in a given output, zeros (LSE -inf) in
+    one allocated here."""
     name = "flash_attn_shared_prefix"
     if q.dim() != 3 or not q.is_cuda:
         raise ValueError(f"{name}: q must be [rows, heads, d] on the GPU, got {list(q.shape)}")
@@ -241,10 +242,15 @@ def flash_attn_shared_prefix(q, k_cache, v_cache, table, lens, prefix_table=None
 def _shared_prefix(q, k_cache, v_cache, table, lens, prefix_table, prefix_lens, group_starts, starts, out, lse, workspace, rows, n,
                    groups, hq, hkv, d, pages, page_size, stream):
     width, pwidth = table.shape[1], prefix_table.shape[1] if groups else 0
-    code, fill = _DTYPE_CODE[q.dtype], out is None
+    # The call fills rows of no request, which only starts can leave, in both outputs or in neither.
+    code, fill = _DTYPE_CODE[q.dtype], out is None and lse is None
+    mixed = starts is not None and not fill
     need = _shared_prefix_need(code, rows, n, groups, hq, hkv, d, page_size, width, pwidth)
-    out = q.new_empty((rows, hq, d)) if out is None else out
-    lse = q.new_empty((rows, hq), dtype=_stat_dtype(q.dtype)) if lse is None else lse
+    if out is None:
+        out = q.new_zeros((rows, hq, d)) if mixed else q.new_empty((rows, hq, d))
+    if lse is None:
+        stat = _stat_dtype(q.dtype)
+        lse = q.new_full((rows, hq), -math.inf, dtype=stat) if mixed else q.new_empty((rows, hq), dtype=stat)
     if workspace is None:
         workspace = q.new_empty(max(need, 1), dtype=torch.uint8)
     strides = _Strides12(*q.stride()[:2], *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0),

@@ -423,3 +423,22 @@ def test_many_rows_on_wide_tables():
     for width in (1900, 120000):
         b.table = torch.cat([b.table, torch.full((5, width - b.table.shape[1]), -1, dtype=torch.int32)], 1)
         b.check(b.call())
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 33])
+def test_one_of_two_outputs_given(d):
+    """A given one keeps its rows of no request, an allocated one has nothing seen there."""
+    b = Batch(BF16, [40], [3], [2, 1, 4], [20, 5, 64], 4, 2, d, 16)
+    rows = sum(b.new) + 6
+    q = torch.zeros((rows, 4, d), dtype=BF16, device="cuda")
+    q[:-6] = b.q.cuda()
+    kinds = dict(out=((rows, 4, d), BF16), lse=((rows, 4), F32))
+    for what, (shape, dtype) in kinds.items():
+        given = torch.full(shape, 7.0, dtype=dtype, device="cuda")
+        for other, kind in kinds.values():  # what the allocator may hand out holds 5
+            torch.full(other, 5.0, dtype=kind, device="cuda")
+        got = b.call(q=q, **{what: given})
+        b.check((got[0][:-6], got[1][:-6]))
+        assert got[what == "lse"] is given and (given[-6:] == 7).all()
+        assert (got[0][-6:] == 0).all() if what == "lse" else (got[1][-6:] == -math.inf).all()
