@@ -857,6 +857,55 @@ template <typename T> struct RowWork {
         if (sh.token < 0) largest();
         else if (t == 0) finish(sh.token, value_of(sh.key));
     }
+    // The border's bin, the pieces' sums of the tokens above it (ps) and its own tokens (comp), by this workgroup alone: the same
+    // integers, and sums in the same order, as sample_bins_kernel and sample_list_kernel leave of a row that has a place.
+    __device__ __forceinline__ int list_border(BorderBin &out) {
+        const Fixed f = fixed_of(whole);
+        const Bins bins = bins_of(top, r.scale);
+        __syncthreads();
+        for (int i = t; i < kBins; i += kThreads) {
+            sh.cnt[i] = 0;
+            sh.mass[i] = 0;
+        }
+        __syncthreads();
+        each_piece(x, np, vocab, [](int) { return true; }, [&](int, const Eight<T> &g) {
+            float v[8];
+            g.get(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (g.c0 + e < vocab) {
+                    const int b = bins.of(v[e]);
+                    atomicAdd(&sh.cnt[b], 1u);
+                    const uint64_t w = f.of(w_of(v[e]));
+                    if (w != 0) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)w);
+                }
+        });
+        __syncthreads();
+        scan_array<kBins>(sh.cnt, kBins, sh.scratch);
+        scan_array<kBins>(sh.mass, kBins, sh.scratch);
+        const double target = c.share * f.sum(sh.mass[kBins - 1]);
+        int b = first_of(kBins, sh, [&](int i) { return c.k < vocab ? int64_t(sh.cnt[i]) >= c.k : f.sum(sh.mass[i]) >= target; });
+        b = b < kBins ? b : kBins - 1;
+        out = {bins.lowest(b), bins.highest(b), b > 0 ? int64_t(sh.cnt[b - 1]) : 0, b > 0 ? f.sum(sh.mass[b - 1]) : 0.0, target};
+        __syncthreads();
+        if (t == 0) sh.count = 0;
+        __syncthreads();
+        each_piece(x, np, vocab, [](int) { return true; }, [&](int p, const Eight<T> &g) {
+            float v[8];
+            g.get(v);
+            double s = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double w = w_of(v[e]);
+                s += key_of(v[e]) > out.hi && w >= c.least ? w : 0.0;
+            }
+            s = wave_sum64(s);
+            if (lane == 0) sh.ps[p] = s;
+            append(&sh.count, sh.comp, v, g.c0, vocab, out.lo, out.hi);
+        });
+        __syncthreads();
+        return sh.count;
+    }
     // The whole row by this workgroup alone, in as many histograms as it takes.
     __device__ __forceinline__ void draw_alone() {
         Kept kept{0, 0, c.least};
@@ -1193,24 +1242,26 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_finish_
         for (int p = lane; p < np; p += kWave) top = fmaxf(top, sh.pm[p]);
         w.top = wave_max_dpp(top);
         int n = 0;
+        BorderBin b;
         if (at < a.most) {
-            w.whole = a.wide[at].whole;
-            n = together(c, vocab) ? a.wide[at].count : 0;
+            const Wide &wide = a.wide[at];
+            w.whole = wide.whole;
+            n = together(c, vocab) ? wide.count : 0;
+            if (n > 0 && n <= kList) {
+                b = wide.border;
+                for (int p = t; p < np; p += kThreads) sh.ps[p] = a.piece_sum[w.row * np + p];
+                for (int i = t; i < n; i += kThreads) sh.comp[i] = wide.list[i];
+            }
         } else {  // no place of its own: its sums are as the first pass left them
             for (int p = t; p < np; p += kThreads) sh.ps[p] = sh.pm[p] == -INFINITY ? 0.0 : a.piece_sum[w.row * np + p] * w.w_of(sh.pm[p]);
             __syncthreads();
             scan_array<kMaxPieces>(sh.ps, np, sh.scratch);
             w.whole = sh.ps[np - 1];
+            if (together(c, vocab)) n = w.list_border(b);  // which rows have a place is chance: their tokens are not
         }
         bool drawn = false;
         if (n > 0 && n <= kList) {
-            const Wide &wide = a.wide[at];
-            BorderBin b = wide.border;
-            for (int p = t; p < np; p += kThreads) {
-                sh.ps[p] = a.piece_sum[w.row * np + p];
-                sh.sums[p] = 0;
-            }
-            for (int i = t; i < n; i += kThreads) sh.comp[i] = wide.list[i];
+            for (int p = t; p < np; p += kThreads) sh.sums[p] = 0;
             __syncthreads();
             // Where min-p leaves nothing of the bin, any border in it will do.
             const bool none = !(w.w_of(value_of(b.hi)) >= c.least);

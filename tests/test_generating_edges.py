@@ -148,3 +148,26 @@ def test_lists_that_overflow_in_every_row():
     # Beside rows that draw from their list at once.
     k = torch.tensor([5, 0, 3000], dtype=torch.int32, device="cuda").repeat(100)
     check(x, u, k=k)
+
+
+@gpu
+def test_equal_rows_draw_the_same_token():
+    """1500 equal rows, all put off, more than are worked on at a time: nuclei whose border is sought to the last bit of top_p
+    draw the same token everywhere."""
+    g = torch.Generator().manual_seed(5)
+    last = float(np.nextafter(np.float32(1), np.float32(0)))  # draws the last id if the nucleus has it
+    u = torch.full((1500,), last, device="cuda")
+    for _ in range(12):
+        x = 0.05 * torch.randn(40000, generator=g)
+        r = int(torch.randint(600, 2500, (1,), generator=g))
+        top = x.sort(descending=True).values
+        x[-1] = (top[r] + top[r + 1]) / 2
+        w = np.exp((x.double() - x.max().double()).numpy())
+        share = math.fsum(w[x.numpy() > x[-1].item()]) / math.fsum(w)
+        rows = x.expand(1500, 40000).contiguous().cuda()
+        lo, hi = share - 1e-10, share + 1e-10
+        while np.nextafter(lo, 1) < hi:
+            mid = (lo + hi) / 2
+            tokens = ct.sample_tokens(rows, u, 1.0, 0, mid)[0]
+            assert (tokens == tokens[0]).all()
+            lo, hi = (lo, mid) if tokens[0] == 39999 else (mid, hi)
