@@ -1499,7 +1499,7 @@ int ctattn_sample(int dtype, const void *logits, const float *u, const float *te
         return fail(dtype == CTATTN_F64 ? hipErrorNotSupported : hipErrorInvalidValue, "%s: dtype %d unsupported (0 = f32, 1 = bf16, 2 = f16)",
                     fn, dtype);
     if (int rc = check_sizes(fn, rows, vocab)) return rc;
-    if (rows > 1 && (stride < vocab || stride > (int64_t(1) << 40)))
+    if (rows > 1 && stride != 0 && (stride < vocab || stride > (int64_t(1) << 40)))  // 0: one row for all
         return fail(hipErrorInvalidValue, "%s: rows %lld apart of %lld logits", fn, (long long)stride, (long long)vocab);
     if (rows == 0) return ok();
     if (!logits || !tokens || !logprobs) return fail(hipErrorInvalidValue, "%s: null pointer", fn);

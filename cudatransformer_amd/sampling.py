@@ -24,8 +24,8 @@ def sample_workspace_bytes(rows: int, vocab: int) -> int:
 
 def sample_tokens(logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, logprobs=None, workspace=None,
                   stream=None):
-    """(tokens, logprobs) [rows]: a token (int64) of each row of logits [rows, vocab] (float32, bfloat16 or float16; rows any
-    distance apart) from random numbers u [rows] (float32 in [0, 1)), and its log-probability (float32) among all tokens at
+    """(tokens, logprobs) [rows]: a token (int64) of each row of logits [rows, vocab] (float32, bfloat16 or float16; rows
+    apart or one expanded) from random numbers u [rows] (float32 in [0, 1)), and its log-probability (float32) among all tokens at
     the row's temperature.
 
     Tokens are ranked by logit, equal ones by the lower id.  Kept are the first top_k (0: all), of these the ranks

@@ -797,9 +797,9 @@ CTATTN_API int ctattn_shared_prefix_fwd(int dtype, const void *q, const void *k_
 CTATTN_API int64_t ctattn_sample_workspace_bytes(int64_t rows, int64_t vocab);
 
 /*
- * A token of each row of logits [rows][vocab] (f32, bf16, f16; rows `stride` elements apart; f64 is refused) from a given
- * random number u[row] in [0, 1).  With M the row's largest logit and w_i = exp((x_i - M) / T), tokens are ranked by
- * logit, equal ones by the lower id, and kept are
+ * A token of each row of logits [rows][vocab] (f32, bf16, f16; rows `stride` >= vocab elements apart, or 0: one row
+ * for all; f64 is refused) from a given random number u[row] in [0, 1).  With M the row's largest logit and
+ * w_i = exp((x_i - M) / T), tokens are ranked by logit, equal ones by the lower id, and kept are
  *   top-k  the first k ranks (k < 1: all),
  *   top-p  of these, the ranks before which less than top_p of their sum of w lies (top_p >= 1: all),
  *   min-p  of these, w >= min_p (min_p <= 0: all),

@@ -171,3 +171,14 @@ def test_equal_rows_draw_the_same_token():
             tokens = ct.sample_tokens(rows, u, 1.0, 0, mid)[0]
             assert (tokens == tokens[0]).all()
             lo, hi = (lo, mid) if tokens[0] == 39999 else (mid, hi)
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [60, 5003, 50257])
+def test_one_row_of_logits_for_many_draws(vocab):
+    """As a prompt's for its first tokens: expanded, not copied."""
+    x, _ = logits_of(1, vocab, torch.bfloat16, vocab)
+    u = torch.rand(70, generator=torch.Generator().manual_seed(1)).cuda()
+    for how in (dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.99, temperature=3.0), dict(top_k=torch.arange(70).int().cuda())):
+        got = ct.sample_tokens(x.expand(70, vocab), u, **how)
+        assert all(torch.equal(a, b) for a, b in zip(got, ct.sample_tokens(x.expand(70, vocab).contiguous(), u, **how)))
