@@ -15,10 +15,13 @@
 // put off: all workgroups together count its tokens and sum its w in bins over x, and list those of the border's bin; its
 // own workgroup then finds the border in bins over that bin's keys.  Sums that atomics make are of 64-bit integers, whose
 // order does not matter.  Few cases are left to a workgroup alone, in as many histograms as they take: top-k beyond the bound
-// together with top-p, thousands of equal logits.
+// together with top-p, thousands of equal logits.  Slow are rows with few finite logits: where fewer runs of 128 hold one than
+// ranks are asked for the bound is -inf, and every token is counted (256 rows, 20 finite logits each: top-k 50 666 us instead of
+// 55, top-p 0.9 349 instead of 173).
 //
-// Measured, 256 rows of 131072 bf16 logits: the first pass 31 us (2.1 TB/s, of 13 us at 5.1: 18 64-bit operations a logit keep
-// the vector units busy; by a table of 64 roots in LDS, 13 of them, 30), without filters 38 in all, top-k 50 54 and top-k 200
+// Measured, 256 rows of 131072 bf16 logits: the first pass 31 us (2.1 TB/s, of 13 us at 5.1: 18 64-bit operations a logit, but a
+// table of 64 roots in LDS, which spares 13 of them, takes 30; around them are two 64-bit divisions a wave and a wave's
+// reduction of a maximum and a 64-bit sum for every 8 logits a lane, not timed apart), without filters 38 in all, top-k 50 54 and top-k 200
 // 62 (the row's workgroup is latencies: LDS, barriers, a few loads one after the other), each row its own parameters 107 to
 // 113, where 18 rows are put off (10 us of bins, 16 of lists, 27 of borders; by their own workgroups alone over 200).  One row
 // of 50257, top-k 50: 3 + 18 us.  1024 threads a row instead of 512 cost 20 us more.

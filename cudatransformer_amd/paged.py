@@ -146,7 +146,8 @@ def _check_caches(name, k_cache, v_cache, dtype, device):
 
 def cache_write(k, v, k_cache, v_cache, slots, stream=None):
     """Copies k and v [rows, heads, d] (any row and head strides) to the places `slots` [rows] (int64) of the caches
-    [pages, page_size, heads, d], in place; rows with a slot outside, as -1, are skipped."""
+    [pages, page_size, heads, d], in place; rows with a slot outside, as -1, are skipped.  Autograd does not see it: no gradient
+    comes back to k and v, and the caches' versions stay."""
     name = "cache_write"
     if k.dim() != 3 or v.shape != k.shape or not k.is_cuda:
         raise ValueError(f"{name}: k and v must be [rows, heads, d] on the GPU, got {list(k.shape)} and {list(v.shape)}")
@@ -196,7 +197,7 @@ def flash_attn_shared_prefix(q, k_cache, v_cache, table, lens, prefix_table=None
     prefix_table [groups, pages] and prefix_lens [groups] the prompts' (None: no prompts); int32.  group_starts [groups + 1] are
     the first requests of the groups (None: equal groups), starts [requests + 1] the first rows of the requests, whose last
     tokens the rows are (None: one row a request).  Rows of no request are left as they are in a given output, zeros (LSE -inf) in
-    one allocated here."""
+    one allocated here.  For inference: no gradient is recorded."""
     name = "flash_attn_shared_prefix"
     if q.dim() != 3 or not q.is_cuda:
         raise ValueError(f"{name}: q must be [rows, heads, d] on the GPU, got {list(q.shape)}")
