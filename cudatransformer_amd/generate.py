@@ -58,8 +58,9 @@ def generate(model, prompts, new_tokens: int, samples: int = 1, temperature=1.0,
              generator=None, page_size: int = 16, graph: bool = True):
     """(tokens, logprobs) [len(prompts) * samples, new_tokens]: `samples` continuations of each prompt (a list of sequences of
     token ids), a prompt's behind each other, and the log-probability of each token at its temperature (``sample_tokens``,
-    whose parameters may be tensors of one number a continuation).  No token ends one: all are new_tokens long.  Random numbers come from `generator` of the model's
-    device, or are u [new_tokens, continuations].  With graph=False every step runs eagerly."""
+    whose parameters may be tensors of one number a continuation).  No token ends one: all are new_tokens long.  Random numbers
+    come from `generator` of the model's device, or are u [new_tokens, continuations].  With graph=False every step runs
+    eagerly."""
     c, p = model.config, next(model.parameters())
     if model.attention != "ctattn" or not c["causal"]:
         raise ValueError("generate: a causal model on the ctattn kernels is wanted")
